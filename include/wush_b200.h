@@ -35,6 +35,7 @@ extern "C" {
 #define WUSH_ERR_NOT_SM100 (-6)
 #define WUSH_ERR_DEVICE_TIMEOUT (-7) /* a bounded wait inside a kernel ran out (reported through `status`) */
 #define WUSH_ERR_TOO_LARGE (-8)      /* problem exceeds a fixed capacity of the entry point */
+#define WUSH_ERR_DEVICE_INDEX (-9)   /* a kernel met an index outside its table and skipped it (reported through `status`) */
 
 /* Layout of the per-group scale bytes written by the fused quantize kernels. */
 #define WUSH_SF_ROW_MAJOR 0 /* sf[row * sf_cols + group], sf_cols = ceil(C/G/4)*4 */
@@ -63,9 +64,11 @@ WUSH_API int wush_b200_arch(void);
 /*
  * Device-side errors.  The entry points that take a `status` argument (a DEVICE int, may be NULL) run kernels
  * whose waits on asynchronous copies and tensor-core completions are bounded; if one runs out, the kernel
- * unwinds, frees what it holds and sets *status = 1 (its output is then invalid).  One word may be shared by any
- * number of calls.  wush_status_check synchronizes `stream`, reads the word and returns WUSH_ERR_DEVICE_TIMEOUT
- * (clearing the word) if it was set, WUSH_OK otherwise.  The reference has no error codes; its host code raises
+ * unwinds, frees what it holds and sets *status = 1 (its output is then invalid).  The paged-cache kernels set
+ * *status = 2 (unless it is set already) when an index on the device lies outside the table it indexes; they skip
+ * what it names.  One word may be shared by any number of calls.  wush_status_check synchronizes `stream`, reads the
+ * word and returns WUSH_ERR_DEVICE_TIMEOUT or WUSH_ERR_DEVICE_INDEX (clearing the word) if it was set, WUSH_OK
+ * otherwise.  The reference has no error codes; its host code raises
  * Python exceptions (e.g. src/quantization/accumulate_hessian.py:126-127), which is what the Python layer does
  * with this return value.
  * wush_selftest_bounded_wait launches one tiny kernel that waits, with a limit of `max_polls` polls (at most
@@ -482,6 +485,106 @@ WUSH_API int wush_gptq_block_step(const double* rn, const double* ynew, const do
 WUSH_API int wush_gptq_block_prepare(const double* gram, const double* basis, int64_t ldb, int64_t basis_step,
                                      int nblocks, int format, int transform, int flags, int64_t rows, double* tmat,
                                      double* rn, double* qt, int* status, void* stream);
+
+/*
+ * Paged key-value cache of one attention layer.  Token p of sequence b lies in page block_table[b, p / page_size] at
+ * row p % page_size.  The reference has no cache (its quantized layers sit inside another library's models); these
+ * entry points serve the decode path of a block built on the quantized layers.
+ *
+ * wush_kv_pages describes the pool; strides are in elements, the channels of a head are contiguous:
+ *   k, v        [num_pages, page_size, heads, dim], any order of the first three axes (strides); 16-byte aligned, strides
+ *               multiples of 16 bytes
+ *   type        WUSH_TYPE_BF16 / WUSH_TYPE_FP16 / WUSH_TYPE_E4M3
+ *   dim         multiple of 8 (of 16 for E4M3), at most 256
+ *   k_scale, v_scale  fp32 [heads] (DEVICE) for E4M3: the value is the stored number times the scale; null otherwise
+ *   bounds      null, or contiguous [num_pages, heads, 2, dim] of bounds_type (BF16 / FP16), 16-byte aligned: smallest
+ *               and largest stored key of every channel over the filled rows of the page
+ */
+#define WUSH_TYPE_BF16 0
+#define WUSH_TYPE_FP16 1
+#define WUSH_TYPE_E4M3 2
+typedef struct wush_kv_pages {
+  void* k;
+  void* v;
+  int64_t k_page, k_row, k_head;
+  int64_t v_page, v_row, v_head;
+  const float* k_scale;
+  const float* v_scale;
+  void* bounds;
+  int64_t num_pages;
+  int32_t page_size, heads, dim;
+  int32_t type, bounds_type;
+} wush_kv_pages;
+
+/* int32 block_table[seqs, width] (DEVICE), row stride in elements */
+typedef struct wush_kv_table {
+  const int32_t* block_table;
+  int64_t stride, seqs, width;
+} wush_kv_table;
+
+/* [rows, heads, dim] with unit channel stride; 16-byte aligned, strides (elements) multiples of 16 bytes */
+typedef struct wush_heads {
+  void* data;
+  int64_t row, head;
+} wush_heads;
+
+/*
+ * Rotate the new queries and keys by their positions and write keys and values into their pages, in one launch.
+ *
+ *   type        BF16 / FP16: element type of q, k, v and the outputs (a 16-bit cache has the same)
+ *   q           [rows, q_heads, dim] or null data; q_out receives the rotated queries (may be q itself, else disjoint)
+ *   k, v        [rows, kv->heads, dim]; k_out null data or receives the rotated keys (may be k itself)
+ *   rope        fp32 [rope_rows, rotary]: cosines of the rotary/2 angles of a position, then sines; null: no rotation.
+ *               rotary % 16 == 0, rotary <= dim; the channels behind it are copied.
+ *   interleaved 0: channel i turns with i + rotary/2; 1: channel 2i with 2i + 1
+ *   seq_ids, positions  int32 [rows].  A row with a negative id or position is padding: nothing of it is read or
+ *               written.  An id, position or page outside its table sets *status = 2 and the row is skipped.
+ * No two rows may name the same token.  Arithmetic: products and their sum each rounded to fp32, stored rounded once
+ * to the cache's type (E4M3: divided by the head's scale, saturated at +-448).
+ */
+WUSH_API int wush_kv_append(const wush_kv_pages* kv, const wush_kv_table* table, int type, const wush_heads* q, int q_heads,
+                            const wush_heads* q_out, const wush_heads* k, const wush_heads* v, const wush_heads* k_out,
+                            const float* rope, int64_t rope_rows, int rotary, int interleaved, const int32_t* seq_ids,
+                            const int32_t* positions, int64_t rows, int* status, void* stream);
+
+/*
+ * Recompute kv->bounds for the pages that hold the last `new_tokens` of the seq_lens[b] tokens of every sequence
+ * (a sequence with fewer: all its pages).  A NaN key makes the bound NaN.
+ */
+WUSH_API int wush_kv_bounds(const wush_kv_pages* kv, const wush_kv_table* table, const int32_t* seq_lens, int64_t new_tokens,
+                            int* status, void* stream);
+
+/*
+ * Select, for every sequence and key head, at most `top` pages to attend to: the first `sink` and the last `recent`
+ * pages of the sequence, then those with the largest scores; equal scores: the lowest page.
+ * score = max over the head's queries of sum_d max(q_d lower_d, q_d upper_d), an upper bound of every logit on the page
+ * (before the softmax scale), accumulated in 64 bits; a NaN score counts as +infinity.
+ *   q        [seqs, q_heads, dim] of `type`; q_heads % kv->heads == 0
+ *   pages    int32 [seqs, kv->heads, top] out: logical pages in ascending order, then -1
+ *   counts   int32 [seqs, kv->heads] out: how many
+ *   workspace  wush_kv_select_workspace_bytes(seqs, heads, width) bytes
+ */
+WUSH_API size_t wush_kv_select_workspace_bytes(int64_t seqs, int heads, int64_t width);
+WUSH_API int wush_kv_select_pages(const wush_kv_pages* kv, const wush_kv_table* table, int type, const wush_heads* q, int q_heads,
+                                  const int32_t* seq_lens, int top, int sink, int recent, int32_t* pages, int32_t* counts,
+                                  void* workspace, size_t workspace_bytes, int* status, void* stream);
+
+/*
+ * Attention of one new token per sequence over its pages: out = softmax(scale * q K^T) V over the tokens
+ * [max(0, len - window), len) (window 0: all), or over the tokens of selected pages.
+ *   q, out     [seqs, q_heads, dim] of `type`; query head h reads key head h / (q_heads / kv->heads)
+ *   lse        null, or fp32 [seqs, q_heads] out: log of the sum of exponentials (-infinity for no tokens)
+ *   seq_lens   int32 [seqs]; a sequence without tokens (len <= 0) gives zeros
+ *   pages, counts  null (all pages), or what wush_kv_select_pages writes: for every sequence and key head the first
+ *              counts[b, h] entries of pages[b, h, top] are attended to, each cut at len (window must be 0)
+ * A length beyond the table, or an entry outside it, sets *status = 2; tokens on such pages are left out.
+ *   workspace  wush_kv_attention_workspace_bytes(kv, q_heads) bytes
+ */
+WUSH_API size_t wush_kv_attention_workspace_bytes(const wush_kv_pages* kv, int q_heads);
+WUSH_API int wush_kv_attention(const wush_kv_pages* kv, const wush_kv_table* table, int type, const wush_heads* q, int q_heads,
+                               const wush_heads* out, float* lse, const int32_t* seq_lens, float scale, int64_t window,
+                               const int32_t* pages, const int32_t* counts, int top, void* workspace, size_t workspace_bytes,
+                               int* status, void* stream);
 
 #ifdef __cplusplus
 }

@@ -17,6 +17,7 @@ ERRORS = {
     -1: "null pointer", -2: "bad shape", -3: "bad alignment", -4: "bad flag or layout",
     -5: "workspace too small", -6: "device is not sm_100", -7: "device-side bounded wait timed out",
     -8: "problem exceeds a fixed capacity of the entry point",
+    -9: "an index on the device lies outside its table (skipped)",
 }
 
 SF_ROW_MAJOR, SF_BLOCKED = 0, 1
@@ -34,6 +35,24 @@ _lib = None
 
 class WushB200Error(RuntimeError):
     pass
+
+
+class KVPages(ctypes.Structure):
+    """wush_kv_pages"""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("k", "v")]
+                + [(n, ctypes.c_int64) for n in ("k_page", "k_row", "k_head", "v_page", "v_row", "v_head")]
+                + [(n, ctypes.c_void_p) for n in ("k_scale", "v_scale", "bounds")] + [("num_pages", ctypes.c_int64)]
+                + [(n, ctypes.c_int32) for n in ("page_size", "heads", "dim", "type", "bounds_type")])
+
+
+class KVTable(ctypes.Structure):
+    """wush_kv_table"""
+    _fields_ = [("block_table", ctypes.c_void_p), ("stride", ctypes.c_int64), ("seqs", ctypes.c_int64), ("width", ctypes.c_int64)]
+
+
+class Heads(ctypes.Structure):
+    """wush_heads"""
+    _fields_ = [("data", ctypes.c_void_p), ("row", ctypes.c_int64), ("head", ctypes.c_int64)]
 
 
 def declared_symbols(header: str = HEADER_PATH) -> list[str]:
@@ -85,6 +104,14 @@ def load() -> ctypes.CDLL:
         "wush_gptq_block_step": [vp, vp, vp, vp, i32, i32, i64, i64, i32, i32, vp, vp, vp, vp, vp],
         "wush_gptq_block_prepare": [vp, vp, i64, i64, i32, i32, i32, i32, i64, vp, vp, vp, vp, vp],
     }
+    f32, size = ctypes.c_float, ctypes.c_size_t
+    pages, table, heads = ctypes.POINTER(KVPages), ctypes.POINTER(KVTable), ctypes.POINTER(Heads)
+    sigs |= {
+        "wush_kv_append": [pages, table, i32, heads, i32, heads, heads, heads, heads, vp, i64, i32, i32, vp, vp, i64, vp, vp],
+        "wush_kv_bounds": [pages, table, vp, i64, vp, vp],
+        "wush_kv_select_pages": [pages, table, i32, heads, i32, vp, i32, i32, i32, vp, vp, vp, size, vp, vp],
+        "wush_kv_attention": [pages, table, i32, heads, i32, heads, vp, vp, f32, i64, vp, vp, i32, vp, size, vp, vp],
+    }
     for name, args in sigs.items():
         fn = getattr(lib, name)
         fn.argtypes = args
@@ -93,6 +120,10 @@ def load() -> ctypes.CDLL:
     lib.wush_gemm_mxf4_bf16_tn_noalloc.restype = ctypes.c_int
     lib.wush_gemm_workspace_bytes.argtypes = [i64, i64, i64, i32]
     lib.wush_gemm_workspace_bytes.restype = ctypes.c_size_t
+    lib.wush_kv_select_workspace_bytes.argtypes = [i64, i32, i64]
+    lib.wush_kv_select_workspace_bytes.restype = ctypes.c_size_t
+    lib.wush_kv_attention_workspace_bytes.argtypes = [pages, i32]
+    lib.wush_kv_attention_workspace_bytes.restype = ctypes.c_size_t
     lib.wush_hessian_tile_count.argtypes = [i64]
     lib.wush_hessian_tile_count.restype = ctypes.c_int64
     _lib = lib
@@ -102,7 +133,7 @@ def load() -> ctypes.CDLL:
 def check(rc: int, what: str) -> None:
     if rc == 0:
         return
-    if rc in (-6, -7):
+    if rc in (-6, -7, -9):
         raise WushB200Error(f"{what}: {ERRORS[rc]}")
     if rc < 0:
         raise WushB200Error(f"{what}: rejected argument ({ERRORS.get(rc, rc)})")

@@ -42,7 +42,8 @@ extern "C" int wush_status_check(int* status_dev, void* stream) {
     e = cudaMemsetAsync(status_dev, 0, sizeof(int), (cudaStream_t)stream);
     if (e != cudaSuccess) return (int)e;
   }
-  return WUSH_ERR_DEVICE_TIMEOUT;
+  // 2: an index outside its table (a timeout, 1, outranks it: kernels set 2 only in a clear word)
+  return host == 2 && quant == 0 ? WUSH_ERR_DEVICE_INDEX : WUSH_ERR_DEVICE_TIMEOUT;
 }
 
 extern "C" int wush_selftest_bounded_wait(int* status_dev, int max_polls, void* stream) {

@@ -1,0 +1,325 @@
+"""Paged key-value cache of a decoder layer, and the attention of new tokens over it.
+
+Decoding one token at a time needs, next to the quantized linear layers, a cache of the keys and values of every
+sequence.  It is kept in pages of a common pool, so that sequences grow without moving: token p of sequence b lies in
+page ``block_table[b, p // page_size]`` at row ``p % page_size``.  The operators:
+
+  paged_kv_append         rotate new queries and keys by their positions, write keys and values into their pages
+  paged_kv_bounds         smallest and largest value of every key channel of the pages the newest tokens lie in
+  paged_select_pages      the pages on which a new query can have its largest logits
+  paged_decode_attention  attention of one new token per sequence over all its tokens, the last `window` of them, or the
+                          selected pages
+
+The reference has no counterpart: its quantized layers (inference_lib/src/fp_quant/module/linear.py:51-386) run inside
+another library's models, whose cache and attention they use.  ``wush_b200.block.ShardedDecoderBlock`` calls these
+operators (``prefill`` and ``decode``); they can equally be called by themselves.
+
+Every operator runs on the current stream of its tensors' device, without a host synchronization, and can be captured
+into a CUDA graph.  Lengths, positions, tables and selected pages are int32 tensors on the device.  An entry that lies
+outside what it indexes (a page outside the pool, a length beyond the table, ...) is skipped by the kernels and
+reported by ``_lib.check_status(device)``.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+
+TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float8_e4m3fn: 2}
+MAX_DIM = 256
+
+
+def rope_table(max_positions: int, rotary_dim: int, base: float = 10000.0, device=None) -> torch.Tensor:
+    """fp32 [max_positions, rotary_dim]: the cosines of the rotary_dim / 2 angles of every position, then the sines.
+    Pair i of position p turns by p * base^(-2 i / rotary_dim); angles are computed in float64.  Any table of this
+    layout can be passed to ``paged_kv_append``, so scaled or multi-axis positions are a matter of its rows."""
+    if rotary_dim <= 0 or rotary_dim % 2 or max_positions <= 0:
+        raise ValueError("rotary_dim must be even and positive, max_positions positive")
+    freq = float(base) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device) / rotary_dim)
+    angle = torch.arange(max_positions, dtype=torch.float64, device=device)[:, None] * freq
+    return torch.cat([angle.cos(), angle.sin()], dim=1).to(torch.float32)
+
+
+class PagedKVCache:
+    """The pool of pages of one layer: ``k`` and ``v`` [num_pages, page_size, n_kv_heads, head_dim], bfloat16, float16 or
+    float8_e4m3fn, with unit channel stride and any order of the other axes (``allocate(layout="hnd")`` keeps a head's
+    rows of a page together).  head_dim is a multiple of 8 (16 for 8-bit pages) and at most 256.
+
+    8-bit pages hold key / k_scale and value / v_scale (float32 [n_kv_heads], given by the caller).  ``bounds``
+    [num_pages, n_kv_heads, 2, head_dim] (bfloat16 or float16; the type of 16-bit pages) is what ``paged_kv_bounds``
+    fills and ``paged_select_pages`` reads.  The object keeps references to its tensors; replacing them needs a new one."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
+                 v_scale: Optional[torch.Tensor] = None, bounds: Optional[torch.Tensor] = None):
+        for t in (k, v, k_scale, v_scale, bounds):
+            if t is not None and not t.is_cuda:
+                raise _lib.WushB200Error("wush_b200 ops need CUDA tensors; there is no CPU fallback")
+        _check_pool(k, v, k_scale, v_scale, bounds)
+        self.k, self.v, self.k_scale, self.v_scale, self.bounds = k, v, k_scale, v_scale, bounds
+        self.num_pages, self.page_size, self.n_kv_heads, self.head_dim = k.shape
+        self.dtype, self.device = k.dtype, k.device
+        ptr = lambda t: t.data_ptr() if t is not None else None
+        self._desc = _lib.KVPages(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), v.stride(0), v.stride(1),
+                                  v.stride(2), ptr(k_scale), ptr(v_scale), ptr(bounds), *k.shape, TYPES[k.dtype],
+                                  TYPES[bounds.dtype] if bounds is not None else 0)
+        self._ref = ctypes.byref(self._desc)
+        self._status = _lib.status_word(self.device).data_ptr()
+
+    @classmethod
+    def allocate(cls, num_pages: int, page_size: int, n_kv_heads: int, head_dim: int, dtype=torch.bfloat16, device=None,
+                 layout: str = "nhd", k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None,
+                 bounds: bool = False) -> "PagedKVCache":
+        """A pool of its own; layout "nhd": [pages, rows, heads, channels] in memory, "hnd": [pages, heads, rows, channels]."""
+        if layout not in ("nhd", "hnd"):
+            raise ValueError(f"layout must be 'nhd' or 'hnd', not {layout!r}")
+        if dtype not in TYPES:
+            raise ValueError(f"unsupported cache dtype: {dtype}")
+
+        def pool():
+            if layout == "nhd":
+                return torch.zeros(num_pages, page_size, n_kv_heads, head_dim, dtype=dtype, device=device)
+            return torch.zeros(num_pages, n_kv_heads, page_size, head_dim, dtype=dtype, device=device).transpose(1, 2)
+        bt = torch.bfloat16 if dtype == torch.float8_e4m3fn else dtype
+        b = torch.zeros(num_pages, n_kv_heads, 2, head_dim, dtype=bt, device=device) if bounds else None
+        return cls(pool(), pool(), k_scale=k_scale, v_scale=v_scale, bounds=b)
+
+
+def _check_pool(k, v, k_scale, v_scale, bounds) -> None:
+    if k.dim() != 4 or k.shape != v.shape or min(k.shape) < 1:
+        raise ValueError("k and v must be [num_pages, page_size, n_kv_heads, head_dim] tensors of one shape")
+    if k.dtype not in TYPES or v.dtype != k.dtype:
+        raise ValueError("k and v must be of one type: bfloat16, float16 or float8_e4m3fn")
+    d, e = k.shape[3], k.element_size()
+    if d > MAX_DIM or (d * e) % 16:
+        raise ValueError(f"head_dim must be a multiple of {16 // e} and at most {MAX_DIM}")
+    for t in (k, v):
+        if t.stride(3) != 1:
+            raise ValueError("the channels of a head must be contiguous")
+        if t.data_ptr() % 16 or any((s * e) % 16 for s in t.stride()[:3]):
+            raise ValueError("pages, rows and heads must start on 16-byte boundaries")
+    eight = k.dtype == torch.float8_e4m3fn
+    for t in (k_scale, v_scale):
+        if (t is not None) != eight:
+            raise ValueError("k_scale and v_scale go with 8-bit pages, and only with them")
+        if eight and (t.dtype != torch.float32 or tuple(t.shape) != (k.shape[2],) or not t.is_contiguous()):
+            raise ValueError("k_scale and v_scale must be contiguous float32 [n_kv_heads] tensors")
+    if bounds is not None:
+        if tuple(bounds.shape) != (k.shape[0], k.shape[2], 2, d) or not bounds.is_contiguous() or bounds.data_ptr() % 16:
+            raise ValueError("bounds must be a contiguous [num_pages, n_kv_heads, 2, head_dim] tensor")
+        if bounds.dtype not in ((torch.bfloat16, torch.float16) if eight else (k.dtype,)):
+            raise ValueError("bounds must be of the pages' type (bfloat16 or float16 for 8-bit pages)")
+    if any(t is not None and t.device != k.device for t in (v, k_scale, v_scale, bounds)):
+        raise ValueError("the tensors of a cache must be on one device")
+
+
+def _int32(t: torch.Tensor, shape, what: str, device) -> int:
+    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{what} must be a contiguous int32 tensor of shape {shape} on {device}")
+    return t.data_ptr()
+
+
+def _table(cache: PagedKVCache, block_table: torch.Tensor) -> "_lib.KVTable":
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.device != cache.device \
+            or block_table.shape[1] < 1 or (block_table.stride(1) != 1 and block_table.shape[1] > 1):
+        raise ValueError(f"block_table must be an int32 [sequences, pages] tensor on {cache.device} with unit column stride")
+    seqs, width = block_table.shape
+    if width * cache.page_size > 2 ** 31 - 1:
+        raise ValueError("a block table can hold at most 2^31 - 1 tokens per sequence")
+    return _lib.KVTable(block_table.data_ptr(), block_table.stride(0), seqs, width)
+
+
+def _heads(cache: PagedKVCache, t: torch.Tensor, rows: int, heads: Optional[int], dtype, what: str) -> "_lib.Heads":
+    if t.dim() != 3 or t.shape[0] != rows or t.shape[2] != cache.head_dim or (heads is not None and t.shape[1] != heads):
+        raise ValueError(f"{what} must be a [{rows}, {'heads' if heads is None else heads}, {cache.head_dim}] tensor")
+    if t.device != cache.device:
+        if not t.is_cuda:
+            raise _lib.WushB200Error("wush_b200 ops need CUDA tensors; there is no CPU fallback")
+        raise ValueError(f"{what} is on {t.device}, the cache on {cache.device}")
+    if t.dtype != dtype:
+        raise ValueError(f"{what} must be {dtype}")
+    s = t.stride()
+    p = t.data_ptr()
+    if s[2] != 1 or p & 15 or s[0] & 7 or s[1] & 7:
+        raise ValueError(f"{what}: channels must be contiguous, and rows and heads start on 16-byte boundaries")
+    return _lib.Heads(p, s[0], s[1])
+
+
+def _query_type(cache: PagedKVCache, t: torch.Tensor, what: str):
+    """Element type of a call's queries, keys and values: that of 16-bit pages, either 16-bit type for 8-bit pages."""
+    if t.dtype not in (torch.bfloat16, torch.float16) or (cache.dtype != torch.float8_e4m3fn and t.dtype != cache.dtype):
+        raise ValueError(f"{what} must be {'bfloat16 or float16' if cache.dtype == torch.float8_e4m3fn else cache.dtype}")
+    return t.dtype
+
+
+def _q_heads(cache: PagedKVCache, q: torch.Tensor) -> int:
+    if q.dim() != 3 or q.shape[1] < 1 or q.shape[1] % cache.n_kv_heads:
+        raise ValueError(f"q must be [rows, heads, {cache.head_dim}] with a multiple of {cache.n_kv_heads} heads")
+    return q.shape[1]
+
+
+def _finish(cache: PagedKVCache, rc: int, what: str) -> None:
+    _lib.check(rc, what)
+    if _lib.CHECK_EVERY_OP:
+        _lib.check_status(cache.device, what)
+
+
+def paged_kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, seq_ids: torch.Tensor,
+                    positions: torch.Tensor, q: Optional[torch.Tensor] = None, rope: Optional[torch.Tensor] = None,
+                    interleaved: bool = False, q_out: Optional[torch.Tensor] = None,
+                    k_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Write the keys and values of new tokens into their pages, rotated by their positions; returns the rotated
+    queries (None without ``q``).
+
+    k, v       [rows, n_kv_heads, head_dim], q [rows, heads, head_dim]: slices of one fused projection will do
+    seq_ids    int32 [rows]: row of ``block_table`` (int32 [sequences, pages]) the token belongs to
+    positions  int32 [rows]: its position in that sequence.  A row with a negative id or position is padding: nothing is
+               read from it or written for it.  No two rows may name the same token.
+    rope       fp32 [positions, rotary_dim] (see ``rope_table``), rotary_dim a multiple of 16; None: no rotation.
+               Channels behind rotary_dim are copied.  ``interleaved`` False: channel i turns with i + rotary_dim/2,
+               True: channel 2i with 2i + 1.
+    q_out      receives the rotated queries instead of a new (zeroed) tensor and may be ``q``; ``k_out`` likewise receives
+               the rotated keys and may be ``k``.  Otherwise outputs must not overlap inputs.
+    """
+    typ = _query_type(cache, k, "k")
+    rows = k.shape[0] if k.dim() == 3 else -1
+    hk = _heads(cache, k, rows, cache.n_kv_heads, typ, "k")
+    hv = _heads(cache, v, rows, cache.n_kv_heads, typ, "v")
+    table = _table(cache, block_table)
+    ids = _int32(seq_ids, (rows,), "seq_ids", cache.device)
+    pos = _int32(positions, (rows,), "positions", cache.device)
+    hq = hqo = hko = None
+    n_heads = 0
+    if q is not None:
+        n_heads = _q_heads(cache, q)
+        hq = _heads(cache, q, rows, n_heads, typ, "q")
+        if q_out is None:
+            q_out = torch.zeros(q.shape, dtype=typ, device=cache.device)
+        hqo = _heads(cache, q_out, rows, n_heads, typ, "q_out")
+    elif q_out is not None:
+        raise ValueError("q_out goes with q")
+    if k_out is not None:
+        hko = _heads(cache, k_out, rows, cache.n_kv_heads, typ, "k_out")
+    rope_ptr, rope_rows, rotary = None, 0, 0
+    if rope is not None:
+        if rope.dim() != 2 or rope.dtype != torch.float32 or not rope.is_contiguous() or rope.device != cache.device \
+                or rope.data_ptr() % 16:
+            raise ValueError(f"rope must be a contiguous float32 [positions, rotary_dim] tensor on {cache.device}")
+        rope_rows, rotary = rope.shape
+        if rope_rows < 1 or rotary < 16 or rotary % 16 or rotary > cache.head_dim:
+            raise ValueError("rotary_dim must be a multiple of 16 and at most head_dim")
+        rope_ptr = rope.data_ptr()
+    if rows == 0:
+        return q_out
+    ref = ctypes.byref
+    with torch.cuda.device(cache.device):
+        rc = _lib.load().wush_kv_append(
+            cache._ref, ref(table), TYPES[typ], ref(hq) if hq is not None else None, n_heads,
+            ref(hqo) if hqo is not None else None, ref(hk), ref(hv), ref(hko) if hko is not None else None, rope_ptr, rope_rows,
+            rotary, int(interleaved), ids, pos, rows, cache._status, torch.cuda.current_stream().cuda_stream)
+    _finish(cache, rc, "wush_kv_append")
+    return q_out
+
+
+def paged_kv_bounds(cache: PagedKVCache, block_table: torch.Tensor, seq_lens: torch.Tensor, new_tokens: int = 1) -> None:
+    """Recompute ``cache.bounds`` for the pages that hold the last ``new_tokens`` of the ``seq_lens`` tokens of every
+    sequence: the smallest and the largest stored key of every channel over the page's filled rows (NaN if one is).
+    Call it after ``paged_kv_append``, with the largest number of tokens a sequence received."""
+    if cache.bounds is None:
+        raise ValueError("the cache has no bounds")
+    if new_tokens < 0:
+        raise ValueError("new_tokens must not be negative")
+    table = _table(cache, block_table)
+    lens = _int32(seq_lens, (table.seqs,), "seq_lens", cache.device)
+    with torch.cuda.device(cache.device):
+        rc = _lib.load().wush_kv_bounds(cache._ref, ctypes.byref(table), lens, new_tokens, cache._status,
+                                        torch.cuda.current_stream().cuda_stream)
+    _finish(cache, rc, "wush_kv_bounds")
+
+
+def paged_select_pages(q: torch.Tensor, cache: PagedKVCache, block_table: torch.Tensor, seq_lens: torch.Tensor, top: int,
+                       sink: int = 1, recent: int = 1) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The pages worth attending to: (pages int32 [sequences, n_kv_heads, top], counts int32 [sequences, n_kv_heads]).
+
+    For every sequence and key head: its first ``sink`` and last ``recent`` pages, then the pages with the largest
+    scores up to ``top`` in all (equal scores: the lowest page first).  A page's score is the largest, over the queries
+    that share the key head, of sum_d max(q_d lower_d, q_d upper_d): no logit on the page exceeds it.  It is summed in
+    64 bits, so that the choice does not depend on the order of the sum; a NaN counts as +infinity.  Pages come in
+    ascending order, followed by -1; a sequence of at most ``top`` pages gets all of them.  q: [sequences, heads,
+    head_dim], as ``paged_decode_attention`` takes it; ``cache.bounds`` must be up to date (``paged_kv_bounds``)."""
+    if cache.bounds is None:
+        raise ValueError("the cache has no bounds")
+    if top < 1 or sink < 0 or recent < 0 or sink + recent > top:
+        raise ValueError("top must be at least 1 and at least sink + recent, which must not be negative")
+    typ = _query_type(cache, q, "q")
+    table = _table(cache, block_table)
+    n_heads = _q_heads(cache, q)
+    hq = _heads(cache, q, table.seqs, n_heads, typ, "q")
+    lens = _int32(seq_lens, (table.seqs,), "seq_lens", cache.device)
+    pages = torch.empty(table.seqs, cache.n_kv_heads, top, dtype=torch.int32, device=cache.device)
+    counts = torch.empty(table.seqs, cache.n_kv_heads, dtype=torch.int32, device=cache.device)
+    if table.seqs == 0:
+        return pages, counts
+    lib = _lib.load()
+    with torch.cuda.device(cache.device):
+        nbytes = lib.wush_kv_select_workspace_bytes(table.seqs, cache.n_kv_heads, table.width)
+        work = _lib.gemm_workspace(cache.device, nbytes)
+        rc = lib.wush_kv_select_pages(cache._ref, ctypes.byref(table), TYPES[typ], ctypes.byref(hq), n_heads, lens, top, sink,
+                                      recent, pages.data_ptr(), counts.data_ptr(), work.data_ptr(), work.numel(), cache._status,
+                                      torch.cuda.current_stream().cuda_stream)
+    _finish(cache, rc, "wush_kv_select_pages")
+    return pages, counts
+
+
+def paged_decode_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                           scale: Optional[float] = None, window: int = 0, pages: Optional[torch.Tensor] = None,
+                           counts: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                           return_lse: bool = False):
+    """softmax(scale * q K^T) V for one new token per sequence: [sequences, heads, head_dim] in q's type (and, with
+    ``return_lse``, float32 [sequences, heads]: the log of the sum of exponentials).
+
+    q          [sequences, heads, head_dim]; query head h reads key head h // (heads / n_kv_heads)
+    seq_lens   int32 [sequences]: tokens in the cache, the new one included.  No token (<= 0): zeros, and -inf.
+    scale      softmax scale, 1 / sqrt(head_dim) by default
+    window     only the last ``window`` tokens; 0: all
+    pages, counts  attend to the tokens of these pages only: for every sequence and key head the first counts[b, h]
+               entries of pages[b, h], logical page numbers as ``paged_select_pages`` returns them (any order; a page
+               listed twice counts twice).  Not together with a window.
+    out        receives the result instead of a new tensor; it may be ``q``, and must not overlap it otherwise
+    """
+    typ = _query_type(cache, q, "q")
+    table = _table(cache, block_table)
+    n_heads = _q_heads(cache, q)
+    hq = _heads(cache, q, table.seqs, n_heads, typ, "q")
+    lens = _int32(seq_lens, (table.seqs,), "seq_lens", cache.device)
+    if window < 0:
+        raise ValueError("window must not be negative")
+    top, pages_ptr, counts_ptr = 0, None, None
+    if (pages is None) != (counts is None):
+        raise ValueError("pages and counts go together")
+    if pages is not None:
+        if window:
+            raise ValueError("a window and selected pages exclude each other")
+        if pages.dim() != 3 or pages.shape[2] < 1 or pages.shape[2] * cache.page_size > 2 ** 31 - 1:
+            raise ValueError("pages must be [sequences, n_kv_heads, top] and hold at most 2^31 - 1 tokens")
+        top = pages.shape[2]
+        pages_ptr = _int32(pages, (table.seqs, cache.n_kv_heads, top), "pages", cache.device)
+        counts_ptr = _int32(counts, (table.seqs, cache.n_kv_heads), "counts", cache.device)
+    if out is None:
+        out = torch.empty(q.shape, dtype=typ, device=cache.device)
+    ho = _heads(cache, out, table.seqs, n_heads, typ, "out")
+    lse = torch.empty(table.seqs, n_heads, dtype=torch.float32, device=cache.device) if return_lse else None
+    if table.seqs > 0:
+        lib = _lib.load()
+        with torch.cuda.device(cache.device):
+            nbytes = lib.wush_kv_attention_workspace_bytes(cache._ref, n_heads)
+            work = _lib.gemm_workspace(cache.device, nbytes) if nbytes else None
+            rc = lib.wush_kv_attention(
+                cache._ref, ctypes.byref(table), TYPES[typ], ctypes.byref(hq), n_heads, ctypes.byref(ho),
+                lse.data_ptr() if return_lse else None, lens, cache.head_dim ** -0.5 if scale is None else scale, window,
+                pages_ptr, counts_ptr, top, work.data_ptr() if work is not None else None,
+                work.numel() if work is not None else 0, cache._status, torch.cuda.current_stream().cuda_stream)
+        _finish(cache, rc, "wush_kv_attention")
+    return (out, lse) if return_lse else out
