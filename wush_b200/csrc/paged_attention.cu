@@ -1,10 +1,31 @@
 // Attention of one new token per sequence over a paged key-value cache: out = softmax(scale * q K^T) V.
-// One block per (sequence, query head); each warp walks every fourth token with the running maximum and sum of the
-// softmax, and the warps' parts are joined at the end.
+//
+// The kernel reads every key and value once and does 4 * G * bytes-worth of multiplications with them (G = query heads
+// that share a key head), so it is bound by HBM as long as the products run on the tensor cores and enough loads are in
+// flight.  Two decisions follow:
+//
+// Products.  All G queries of a key head are worked on together, with the tokens as the rows of m16n8k16 products:
+//     S^T [16 tokens x 8 heads] = K [16 tokens x 16 channels] . Q^T,     O^T [16 channels x 8 heads] += V^T . P^T.
+// A product does not care in which order its contracted index runs, nor which row is which channel, so a lane's fragment
+// of K is a 16-byte piece of a key row and its fragment of V eight neighbouring channels of four tokens: both come
+// straight from global memory into registers with 16-byte loads (eight for 8-bit values), without shared memory, and the
+// queries are loaded in the matching order.  P is turned from the layout of an accumulator into that of an operand by
+// movmatrix.  8-bit pages are widened to fp16 (exact) in registers.
+//
+// Work.  The tokens of all (sequence, key head, chunk of queries) items are cut into units of 4 tiles (one per warp), the
+// units of all items are numbered through, and every block of a grid that fills the GPU exactly once takes an equal run
+// of them; lengths are read on the device.  A block that holds a whole item writes its result; a part of an item goes to
+// the workspace, and a second kernel joins the parts (every block has at most two: its first and its last item).
+#include <type_traits>
+
 #include "paged_kv.cuh"
 
 namespace wush {
 namespace kv {
+
+constexpr int WARPS = 4;
+constexpr int MIN_UNITS = 2;            // smallest run of units a block takes while others idle
+constexpr int WHOLE_UNITS = 4;          // items of at most this many units are not split at all
 
 struct AttentionParams {
   wush_kv_pages kv;
@@ -14,93 +35,655 @@ struct AttentionParams {
   const int32_t* seq_lens;
   const int32_t* pages;
   const int32_t* counts;
+  float* part_o;                        // [slots][heads of a chunk][DP]
+  float* part_ml;                       // [slots][heads of a chunk][2]
   int* status;
   float scale;
   int64_t window;
-  int q_heads, top;
+  int q_heads, group, chunks, top;
+  int whole;                            // one block per item, no parts
+  int64_t entries;                      // sequences, or (sequence, key head) pairs when pages are selected
 };
 
-constexpr int WARPS = 4;
+// resident blocks per SM, by the registers of the fragments
+__host__ __device__ constexpr int blocks_per_sm(int dp, int nt) { return dp == 64 ? (nt == 1 ? 4 : 3) : (dp == 128 && nt == 1 ? 3 : 2); }
 
-template <typename T, typename C>
-__global__ void __launch_bounds__(WARPS * 32) attention_kernel(const AttentionParams p) {
-  __shared__ float sm_m[WARPS], sm_l[WARPS];
-  __shared__ float sm_o[WARPS][MAX_DIM];
+// ---- shape of an instantiation -----------------------------------------------------------------------------------------
+// T: queries and result; C: pages; DP: channels, rounded up to 64, 128 or 256; NT: tiles of 8 query heads.
+template <typename T, typename C, int DP, int NT>
+struct Shape {
+  static constexpr bool E8 = sizeof(C) == 1;
+  // tokens a warp holds at a time: 4 KB of keys and as much of values, in 32 + 32 registers of a lane (128 channels)
+  static constexpr int TT = (DP < 256 && (E8 || DP == 64)) ? 32 : 16;
+  static constexpr int MT = TT / 16;
+  static constexpr int KJ = DP * (int)sizeof(C) / 64;       // 16-byte pieces of a key row per lane
+  static constexpr int VJ = DP / 64;                        // pieces of 8 channels of a value row per lane
+  static constexpr int HEADS = NT * 8;
+  static constexpr int UNIT = WARPS * TT;                   // tokens of a unit
+  static constexpr bool OVERLAP = DP < 256 || E8;           // next keys are loaded while the values are worked on
+  // P as two 16-bit terms: one term costs 2^-9 (bf16) or 2^-12 (fp16) of a weight, which a bf16 result hides only with fp16
+  static constexpr bool TWO = !(E8 && sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value);
+  using M = typename std::conditional<E8, __half, T>::type; // operand type of the products
+  // fp16 weights are scaled by 2^14 so that small ones stay normal numbers
+  static constexpr float BIAS = std::is_same<M, __half>::value ? 14.0f : 0.0f;
+  static constexpr int BLOCKS = blocks_per_sm(DP, NT);
+  static constexpr int PITCH = DP + 4;                      // floats of a head's row in shared memory
+};
+
+__host__ __device__ inline int pad_dim(int d) { return d <= 64 ? 64 : (d <= 128 ? 128 : 256); }
+__host__ __device__ inline int head_tiles(int dp, int group) { return dp == 256 || group <= 8 ? 1 : 2; }
+
+// ---- instructions ------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint4 load16(const void* p, bool ok) {
+  uint4 v;
+  asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %5, 0;\nmov.b32 %0, 0;\nmov.b32 %1, 0;\nmov.b32 %2, 0;\nmov.b32 %3, 0;\n"
+               "@p ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n}\n"
+               : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
+               : "l"(p), "r"((int)ok));
+  return v;
+}
+__device__ __forceinline__ uint2 load8b(const void* p, bool ok) {
+  uint2 v;
+  asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %3, 0;\nmov.b32 %0, 0;\nmov.b32 %1, 0;\n"
+               "@p ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];\n}\n"
+               : "=&r"(v.x), "=&r"(v.y)
+               : "l"(p), "r"((int)ok));
+  return v;
+}
+
+template <typename M>
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if (std::is_same<M, __half>::value)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// transpose of an 8 x 8 matrix of 16-bit numbers held by the warp (row = lane / 4, two columns per lane)
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// 2^x to 2 units in the last place; 0 for -infinity
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// ---- numbering of the work ---------------------------------------------------------------------------------------------
+struct Work {
+  int len;                              // tokens of the sequence
+  int begin;                            // first position (window); 0 when pages are selected
+  int tokens;                           // tokens to walk: positions, or rows of the selected pages
+};
+
+__device__ __forceinline__ Work work_of(const AttentionParams& p, int64_t entry) {
+  const int64_t b = p.pages ? entry / p.kv.heads : entry;
+  Work w;
+  w.len = clamp_length(p.seq_lens[b], p.table.width * p.kv.page_size, p.status);
+  w.begin = p.window > 0 && w.len > p.window ? (int)(w.len - p.window) : 0;
+  w.tokens = p.pages ? max(0, min(p.counts[entry], p.top)) * p.kv.page_size : w.len - w.begin;
+  return w;
+}
+
+// an item without tokens has one unit: somebody has to write its zeros
+template <int UNIT>
+__device__ __forceinline__ int64_t units_of(const AttentionParams& p, int64_t entry) {
+  return entry < p.entries ? max(1, (work_of(p, entry).tokens + UNIT - 1) / UNIT) : 0;
+}
+
+struct Place {
+  int64_t entry, base;                  // entry that holds a unit, and the number of its first unit
+  int64_t units;                        // units of one item of the entry
+};
+
+// Total number of units, by one warp.
+template <int UNIT>
+__device__ int64_t total_units(const AttentionParams& p, int copies) {
+  const int lane = threadIdx.x & 31;
+  int64_t sum = 0;
+  for (int64_t e = lane; e < p.entries; e += 32) sum += units_of<UNIT>(p, e);
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum * copies;
+}
+
+// The entry that unit t lies in, by one warp; `copies` items per entry.
+template <int UNIT>
+__device__ Place locate(const AttentionParams& p, int copies, int64_t t) {
+  const int lane = threadIdx.x & 31;
+  int64_t before = 0;
+  for (int64_t e0 = 0; e0 < p.entries; e0 += 32) {
+    const int64_t u = units_of<UNIT>(p, e0 + lane);
+    int64_t sum = u * copies;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += x;
+    }
+    const unsigned beyond = __ballot_sync(0xffffffffu, before + sum > t);
+    if (beyond) {
+      const int at = __ffs(beyond) - 1;
+      const int64_t units = __shfl_sync(0xffffffffu, u, at);
+      return {e0 + at, before + __shfl_sync(0xffffffffu, sum, at) - units * copies, units};
+    }
+    before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return {p.entries, before, 1};
+}
+
+__device__ __forceinline__ int64_t units_per_block(int64_t total, int64_t blocks) {
+  const int64_t per = (total + blocks - 1) / blocks;
+  return per < MIN_UNITS ? MIN_UNITS : per;
+}
+
+struct Item {
+  int64_t b;
+  int hk, first_head, heads;            // key head; first query head and number of query heads of the chunk
+};
+
+template <int HEADS>
+__device__ __forceinline__ Item item_of(const AttentionParams& p, int64_t entry, int64_t copy) {
+  Item it;
+  it.b = p.pages ? entry / p.kv.heads : entry;
+  it.hk = p.pages ? (int)(entry % p.kv.heads) : (int)(copy / p.chunks);
+  const int chunk = p.pages ? (int)copy : (int)(copy % p.chunks);
+  it.first_head = it.hk * p.group + chunk * HEADS;
+  it.heads = min(HEADS, p.group - chunk * HEADS);
+  return it;
+}
+
+// ---- the kernel --------------------------------------------------------------------------------------------------------
+template <typename T, typename C, int DP, int NT>
+__global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) attention_kernel(const AttentionParams p) {
+  using S = Shape<T, C, DP, NT>;
+  using M = typename S::M;
+  constexpr int MT = S::MT, KJ = S::KJ, VJ = S::VJ, TT = S::TT;
+  extern __shared__ float smem[];
+  float* sm_o = smem;                                        // [WARPS][HEADS][PITCH]
+  float* sm_m = smem + WARPS * S::HEADS * S::PITCH;          // [WARPS][HEADS]
+  float* sm_l = sm_m + WARPS * S::HEADS;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int h = blockIdx.x % p.q_heads, group = p.q_heads / p.kv.heads, hk = h / group, d = p.kv.dim;
-  const int64_t b = blockIdx.x / p.q_heads;
-  const int len = clamp_length(p.seq_lens[b], p.table.width * p.kv.page_size, p.status);
-  const int begin = p.window > 0 && len > p.window ? (int)(len - p.window) : 0;
-  const int64_t entry = b * p.kv.heads + hk;
-  const int64_t n = p.pages ? (int64_t)max(0, min(p.counts[entry], p.top)) * p.kv.page_size : len - begin;
-  float q[8];
-  const bool mine = lane * 8 < d;
+  const int r = lane >> 2, c = lane & 3;
+  const int d = p.kv.dim, page_size = p.kv.page_size;
+  const int copies = p.pages ? p.chunks : p.kv.heads * p.chunks;
+
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+
+  int64_t t, t_end, t_first;
+  Place at;
+  if (p.whole) {
+    const int64_t entry = blockIdx.x / copies;
+    at = {entry, 0, units_of<S::UNIT>(p, entry)};
+    t = t_first = (int64_t)(blockIdx.x % copies) * at.units;
+    t_end = t + at.units;
+  } else {
+    const int64_t total = total_units<S::UNIT>(p, copies);
+    const int64_t per = units_per_block(total, gridDim.x);
+    t = t_first = (int64_t)blockIdx.x * per;
+    t_end = min(total, t + per);
+    if (t >= t_end) return;
+    at = locate<S::UNIT>(p, copies, t);
+  }
+
+  while (t < t_end) {
+    if (t >= at.base + at.units * copies) {                  // the next entry
+      at.base += at.units * copies;
+      at.entry += 1;
+      at.units = units_of<S::UNIT>(p, at.entry);
+    }
+    const Work w = work_of(p, at.entry);
+    const int64_t copy = (t - at.base) / at.units;
+    const int64_t u0 = t - at.base - copy * at.units;
+    const int64_t u1 = min(at.units, u0 + (t_end - t));
+    const Item it = item_of<S::HEADS>(p, at.entry, copy);
+    const int s1 = (int)min((int64_t)w.tokens, u1 * S::UNIT);
+
+    // -- queries, in the order of the key fragments ----------------------------------------------------------------------
+    uint32_t qf[NT][DP / 16][2];
+    float factor[NT][2];                                     // logit -> exponent of 2, for the heads 2c and 2c + 1
 #pragma unroll
-  for (int j = 0; j < 8; ++j) q[j] = 0.0f;
-  if (mine) load8(reinterpret_cast<const T*>(p.q.data) + b * p.q.row + (int64_t)h * p.q.head + lane * 8, q);
-  const float factor = p.scale * (sizeof(C) == 1 ? p.kv.k_scale[hk] : 1.0f);
-  float m = -INFINITY, l = 0.0f, o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  for (int64_t t = warp; t < n; t += WARPS) {
-    int lp = (int)((p.pages ? t : begin + t) / p.kv.page_size);
-    const int row = (int)((p.pages ? t : begin + t) - (int64_t)lp * p.kv.page_size);
-    if (p.pages) {
-      lp = p.pages[entry * p.top + lp];
+    for (int nt = 0; nt < NT; ++nt) {
+      const int h = nt * 8 + r;
+      const T* row = reinterpret_cast<const T*>(p.q.data) + it.b * p.q.row + (int64_t)(it.first_head + h) * p.q.head;
+      const float to_exp2 = p.scale * 1.4426950408889634f;
+      if (!S::E8) {
+#pragma unroll
+        for (int j = 0; j < KJ; ++j) {
+          const int ch = (j * 4 + c) * 8;
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (h < it.heads && ch < d) v = *reinterpret_cast<const uint4*>(row + ch);
+          qf[nt][2 * j][0] = v.x;
+          qf[nt][2 * j][1] = v.y;
+          qf[nt][2 * j + 1][0] = v.z;
+          qf[nt][2 * j + 1][1] = v.w;
+        }
+        factor[nt][0] = factor[nt][1] = to_exp2;
+      } else {
+        // fp16 operands: every query is divided by the power of two below its largest element, so that nothing overflows
+        // and what underflows is below 2^-24 of that element
+        float x[KJ][16];
+        float top = 0.0f;
+#pragma unroll
+        for (int j = 0; j < KJ; ++j) {
+          const int ch = (j * 4 + c) * 16;
+#pragma unroll
+          for (int k = 0; k < 16; ++k) x[j][k] = 0.0f;
+          if (h < it.heads && ch < d) {
+            load8(row + ch, *reinterpret_cast<float(*)[8]>(&x[j][0]));
+            load8(row + ch + 8, *reinterpret_cast<float(*)[8]>(&x[j][8]));
+          }
+#pragma unroll
+          for (int k = 0; k < 16; ++k) top = fmaxf(top, fabsf(x[j][k]));
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // exponent field of the largest element, kept where 2^e and 2^-e are normal numbers; infinities stay infinite
+        const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 253);
+        const float down = __uint_as_float((uint32_t)(254 - e) << 23);
+        const float up = __uint_as_float((uint32_t)e << 23) * to_exp2 * p.kv.k_scale[it.hk];
+#pragma unroll
+        for (int j = 0; j < KJ; ++j)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) qf[nt][j * 4 + (k >> 1)][k & 1] = pack2<__half>(x[j][2 * k] * down, x[j][2 * k + 1] * down);
+        factor[nt][0] = __shfl_sync(0xffffffffu, up, 8 * c);         // lane 4 h holds head h
+        factor[nt][1] = __shfl_sync(0xffffffffu, up, 8 * c + 4);
+      }
+    }
+
+    // -- the walk --------------------------------------------------------------------------------------------------------
+    float m[NT][2], l[NT][2], o[NT][VJ][4][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < VJ; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[nt][j][i][0] = o[nt][j][i][1] = o[nt][j][i][2] = o[nt][j][i][3] = 0.0f;
+    }
+    uint4 kf[MT][2][KJ];
+    using VT = typename std::conditional<S::E8, uint2, uint4>::type;
+    VT vf[MT][4][VJ];
+    const C* k_head = reinterpret_cast<const C*>(p.kv.k) + it.hk * p.kv.k_head;
+    const C* v_head = reinterpret_cast<const C*>(p.kv.v) + it.hk * p.kv.v_head;
+    const int32_t* list = p.pages ? p.pages + at.entry * p.top : nullptr;
+    const int32_t* table = p.table.block_table + it.b * p.table.stride;
+    const int step = S::UNIT;
+
+    // the lane's token of a tile, one level of the lookup at a time: logical page (-1: none), then physical page
+    struct Row { int page, row; };
+    auto logical = [&](int64_t base) -> Row {
+      const int64_t v = base + (lane & (TT - 1));
+      if (v >= s1) return {-1, 0};
+      const int pos = (int)v + w.begin, li = pos / page_size, row = pos - li * page_size;
+      if (!list) return {li, row};
+      const int lp = list[li];
       if (lp < 0 || lp >= p.table.width) {
         report_index(p.status);
-        continue;
+        return {-1, 0};
       }
-      if ((int64_t)lp * p.kv.page_size + row >= len) continue;
-    }
-    const int page = lookup_page(p.table, b, lp, p.kv.num_pages, p.status);
-    if (page < 0) continue;
-    float k[8], v[8], s = 0.0f;
-    if (mine) {
-      load8(reinterpret_cast<const C*>(p.kv.k) + page * p.kv.k_page + row * p.kv.k_row + hk * p.kv.k_head + lane * 8, k);
-      load8(reinterpret_cast<const C*>(p.kv.v) + page * p.kv.v_page + row * p.kv.v_row + hk * p.kv.v_head + lane * 8, v);
+      return {(int64_t)lp * page_size + row < w.len ? lp : -1, row};
+    };
+    auto physical = [&](Row x) -> Row { return {x.page >= 0 ? table[x.page] : -2, x.row}; };
+    int64_t k_at, v_at;                                      // the lane's token: element offsets of its rows
+    unsigned seen = 0, seen_next = 0;                        // tokens of the tile that count
+    auto resolve = [&](Row x) {
+      bool ok = x.page >= 0 && x.page < p.kv.num_pages;
+      if (!ok && x.page != -2) report_index(p.status);
+      k_at = ok ? x.page * p.kv.k_page + x.row * p.kv.k_row : 0;
+      v_at = ok ? x.page * p.kv.v_page + x.row * p.kv.v_row : 0;
+      seen_next = __ballot_sync(0xffffffffu, ok);
+    };
+    auto load_keys = [&](unsigned mask) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s = fmaf(q[j], k[j], s);
-    }
+      for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    s *= factor;
-    const float top = fmaxf(m, s);
-    const float base = top == -INFINITY ? 0.0f : top;
-    const float keep = expf(m - base), e = expf(s - base);
+        for (int half = 0; half < 2; ++half) {
+          const int tok = mt * 16 + half * 8 + r;
+          const C* row = k_head + __shfl_sync(0xffffffffu, k_at, tok);
+          const bool ok = mask >> tok & 1;
+#pragma unroll
+          for (int j = 0; j < KJ; ++j) {
+            const int ch = (j * 4 + c) * (16 / (int)sizeof(C));
+            kf[mt][half][j] = load16(row + ch, ok && ch < d);
+          }
+        }
+    };
+    auto load_values = [&](unsigned mask) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int tok = mt * 16 + 2 * c + (x & 1) + (x >> 1) * 8;
+          const C* row = v_head + __shfl_sync(0xffffffffu, v_at, tok);
+          const bool ok = mask >> tok & 1;
+#pragma unroll
+          for (int j = 0; j < VJ; ++j) {
+            const int ch = j * 64 + r * 8;
+            if constexpr (S::E8) vf[mt][x][j] = load8b(row + ch, ok && ch < d);
+            else vf[mt][x][j] = load16(row + ch, ok && ch < d);
+          }
+        }
+    };
+
+    int64_t base = u0 * S::UNIT + warp * TT;
+    Row next, after;                                         // physical rows of the next tile, logical ones of that after it
+    {
+      const Row first = physical(logical(base));
+      next = physical(logical(base + step));
+      after = logical(base + 2 * step);
+      resolve(first);
+    }
+    if (base < s1) {
+      load_keys(seen_next);
+      if (S::OVERLAP) load_values(seen_next);
+    }
+    for (; base < s1; base += step) {
+      seen = seen_next;
+      // logits
+      float s[MT][NT][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          s[mt][nt][0] = s[mt][nt][1] = s[mt][nt][2] = s[mt][nt][3] = 0.0f;
+#pragma unroll
+          for (int j = 0; j < KJ; ++j) {
+            const uint32_t lo[4] = {kf[mt][0][j].x, kf[mt][0][j].y, kf[mt][0][j].z, kf[mt][0][j].w};
+            const uint32_t hi[4] = {kf[mt][1][j].x, kf[mt][1][j].y, kf[mt][1][j].z, kf[mt][1][j].w};
+            if constexpr (S::E8) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                mma<M>(s[mt][nt], e4m3x2_to_f16x2(lo[i]), e4m3x2_to_f16x2(hi[i]), e4m3x2_to_f16x2(lo[i] >> 16),
+                       e4m3x2_to_f16x2(hi[i] >> 16), qf[nt][j * 4 + i][0], qf[nt][j * 4 + i][1]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+                mma<M>(s[mt][nt], lo[2 * i], hi[2 * i], lo[2 * i + 1], hi[2 * i + 1], qf[nt][2 * j + i][0], qf[nt][2 * j + i][1]);
+            }
+          }
+        }
+      if (!S::OVERLAP) load_values(seen);
+      resolve(next);                                         // from here on k_at and v_at are the next tile's
+      if (S::OVERLAP && base + step < s1) load_keys(seen_next);
+      next = physical(after);
+      after = logical(base + 3 * step);
+
+      // softmax: running maximum per head, weights relative to it
+      float top[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float x = -INFINITY;
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              float& y = s[mt][nt][half * 2 + e];
+              y = seen >> (mt * 16 + half * 8 + r) & 1 ? y * factor[nt][e] : -INFINITY;
+              x = fmaxf(x, y);
+            }
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+          top[nt][e] = fmaxf(m[nt][e], x);
+        }
+      bool rises = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) rises |= top[nt][0] > m[nt][0] || top[nt][1] > m[nt][1];
+      if (__any_sync(0xffffffffu, rises)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float keep = top[nt][e] == m[nt][e] ? 1.0f : exp2_fast(m[nt][e] - top[nt][e]);
+            l[nt][e] *= keep;
+            m[nt][e] = top[nt][e];
+#pragma unroll
+            for (int j = 0; j < VJ; ++j)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                o[nt][j][i][e] *= keep;
+                o[nt][j][i][2 + e] *= keep;
+              }
+          }
+      }
+      uint32_t ph[MT][NT][2], pl[MT][NT][2];                 // weights as operands: tokens 2c, 2c + 1 (+8) of head r
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float base0 = (m[nt][0] == -INFINITY ? 0.0f : m[nt][0]) - S::BIAS;
+        const float base1 = (m[nt][1] == -INFINITY ? 0.0f : m[nt][1]) - S::BIAS;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const float p0 = exp2_fast(s[mt][nt][half * 2] - base0), p1 = exp2_fast(s[mt][nt][half * 2 + 1] - base1);
+            l[nt][0] += p0;
+            l[nt][1] += p1;
+            const uint32_t hi = pack2<M>(p0, p1);
+            ph[mt][nt][half] = transpose8(hi);
+            if (S::TWO) {
+              const float2 back = to_float2<M>(hi);
+              pl[mt][nt][half] = transpose8(pack2<M>(p0 - back.x, p1 - back.y));
+            }
+          }
+      }
+
+      // values
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int j = 0; j < VJ; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t a0, a1, a2, a3;                         // channels 2i and 2i + 1 of the lane's eight
+            if constexpr (S::E8) {
+              const uint32_t sel = i & 1 ? 0x7362 : 0x5140;  // bytes of tokens t, t + 1 side by side
+              const uint32_t x = __byte_perm(i < 2 ? vf[mt][0][j].x : vf[mt][0][j].y, i < 2 ? vf[mt][1][j].x : vf[mt][1][j].y, sel);
+              const uint32_t y = __byte_perm(i < 2 ? vf[mt][2][j].x : vf[mt][2][j].y, i < 2 ? vf[mt][3][j].x : vf[mt][3][j].y, sel);
+              a0 = e4m3x2_to_f16x2(x);
+              a1 = e4m3x2_to_f16x2(x >> 16);
+              a2 = e4m3x2_to_f16x2(y);
+              a3 = e4m3x2_to_f16x2(y >> 16);
+            } else {
+              auto word = [&](const uint4& q) { return i == 0 ? q.x : (i == 1 ? q.y : (i == 2 ? q.z : q.w)); };
+              const uint32_t t0 = word(vf[mt][0][j]), t1 = word(vf[mt][1][j]), t2 = word(vf[mt][2][j]), t3 = word(vf[mt][3][j]);
+              a0 = __byte_perm(t0, t1, 0x5410);
+              a1 = __byte_perm(t0, t1, 0x7632);
+              a2 = __byte_perm(t2, t3, 0x5410);
+              a3 = __byte_perm(t2, t3, 0x7632);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma<M>(o[nt][j][i], a0, a1, a2, a3, ph[mt][nt][0], ph[mt][nt][1]);
+              if (S::TWO) mma<M>(o[nt][j][i], a0, a1, a2, a3, pl[mt][nt][0], pl[mt][nt][1]);
+            }
+          }
+      if (base + step < s1) {
+        if (S::OVERLAP) load_values(seen_next);
+        else load_keys(seen_next);
+      }
+    }
+
+    // -- join the warps --------------------------------------------------------------------------------------------------
+    __syncthreads();                                         // the previous item's shared memory has been read
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float x = l[nt][e];
+        x += __shfl_xor_sync(0xffffffffu, x, 4);
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        const int h = nt * 8 + 2 * c + e;
+        if (r == 0) {
+          sm_m[warp * S::HEADS + h] = m[nt][e];
+          sm_l[warp * S::HEADS + h] = x;
+        }
+        float* row = sm_o + (warp * S::HEADS + h) * S::PITCH + r * 8;
+#pragma unroll
+        for (int j = 0; j < VJ; ++j) {
+          *reinterpret_cast<float4*>(row + j * 64) = make_float4(o[nt][j][0][e], o[nt][j][0][2 + e], o[nt][j][1][e], o[nt][j][1][2 + e]);
+          *reinterpret_cast<float4*>(row + j * 64 + 4) = make_float4(o[nt][j][2][e], o[nt][j][2][2 + e], o[nt][j][3][e], o[nt][j][3][2 + e]);
+        }
+      }
+    __syncthreads();
+    const bool all = u0 == 0 && u1 == at.units;
+    const int64_t slot = 2 * (int64_t)blockIdx.x + (t > t_first ? 1 : 0);
+    for (int x = threadIdx.x; x < S::HEADS * (DP / 8); x += WARPS * 32) {
+      const int h = x / (DP / 8), ch = (x % (DP / 8)) * 8;
+      if (h >= it.heads || ch >= d) continue;
+      float top = sm_m[h];
+#pragma unroll
+      for (int k = 1; k < WARPS; ++k) top = fmaxf(top, sm_m[k * S::HEADS + h]);
+      float total = 0.0f, y[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+      for (int k = 0; k < WARPS; ++k) {
+        const float mk = sm_m[k * S::HEADS + h];
+        const float keep = mk == top ? 1.0f : exp2_fast(mk - top);
+        total = fmaf(sm_l[k * S::HEADS + h], keep, total);
+        const float* row = sm_o + (k * S::HEADS + h) * S::PITCH + ch;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = fmaf(row[i], keep, y[i]);
+      }
+      if (all) {
+        const float scale = (S::E8 ? p.kv.v_scale[it.hk] : 1.0f) / (total == 0.0f ? 1.0f : total);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] *= scale;
+        store8(reinterpret_cast<T*>(p.out.data) + it.b * p.out.row + (int64_t)(it.first_head + h) * p.out.head + ch, y);
+        if (ch == 0 && p.lse)
+          p.lse[it.b * p.q_heads + it.first_head + h] =
+              total == 0.0f ? -INFINITY : (top - S::BIAS + log2f(total)) * 0.6931471805599453f;
+      } else {
+        float* row = p.part_o + (slot * S::HEADS + h) * DP + ch;
+        *reinterpret_cast<float4*>(row) = make_float4(y[0], y[1], y[2], y[3]);
+        *reinterpret_cast<float4*>(row + 4) = make_float4(y[4], y[5], y[6], y[7]);
+        if (ch == 0) {
+          p.part_ml[(slot * S::HEADS + h) * 2] = top;
+          p.part_ml[(slot * S::HEADS + h) * 2 + 1] = total;
+        }
+      }
+    }
+    t += u1 - u0;
+  }
+}
+
+// ---- join of the parts -------------------------------------------------------------------------------------------------
+// An item that was split holds a boundary between two blocks; block (k, h) of this grid looks at the boundary between
+// blocks k and k + 1 and, when it is the first one inside its item, joins the item's parts for query head h of the chunk.
+template <typename T, typename C, int DP, int NT>
+__global__ void __launch_bounds__(WARPS * 32) join_kernel(const AttentionParams p, int blocks) {
+  using S = Shape<T, C, DP, NT>;
+  __shared__ float sm_o[WARPS][DP];
+  __shared__ float sm_m[WARPS], sm_l[WARPS];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, h = blockIdx.y;
+  const int copies = p.pages ? p.chunks : p.kv.heads * p.chunks;
+  const int64_t total_work = total_units<S::UNIT>(p, copies);
+  const int64_t per = units_per_block(total_work, blocks);
+  const int64_t t = (int64_t)(blockIdx.x + 1) * per;
+  if (t >= total_work) return;
+  const Place at = locate<S::UNIT>(p, copies, t);
+  const int64_t copy = (t - at.base) / at.units, first = at.base + copy * at.units;   // the item and its first unit
+  if (first == t || first < t - per) return;               // not split here, or another block of this grid joins it
+  const Item it = item_of<S::HEADS>(p, at.entry, copy);
+  if (h >= it.heads) return;
+  const int64_t last = (first + at.units - 1) / per;       // last block with a part
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  constexpr int E = DP / 32;                               // channels per lane
+  float m = -INFINITY, l = 0.0f, o[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) o[i] = 0.0f;
+  for (int64_t k = blockIdx.x + warp; k <= last; k += WARPS) {
+    // the item begins inside block blockIdx.x (slot 1, unless with its run) and at the start of the later blocks' runs
+    const int64_t slot = 2 * k + (k == blockIdx.x && first > k * per ? 1 : 0);
+    const float* ml = p.part_ml + (slot * S::HEADS + h) * 2;
+    const float* row = p.part_o + (slot * S::HEADS + h) * DP;
+    const float mk = ml[0], lk = ml[1];
+    const float top = fmaxf(m, mk);
+    const float keep = m == top ? 1.0f : exp2_fast(m - top), add = mk == top ? 1.0f : exp2_fast(mk - top);
     m = top;
-    l = l * keep + e;
-    if (mine) {
+    l = l * keep + lk * add;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) o[j] = o[j] * keep + e * v[j];
+    for (int i = 0; i < E; ++i) {
+      const int ch = i * 32 + lane;
+      o[i] = o[i] * keep + (ch < p.kv.dim ? row[ch] : 0.0f) * add;
     }
   }
   if (lane == 0) {
     sm_m[warp] = m;
     sm_l[warp] = l;
   }
-  if (mine) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sm_o[warp][lane * 8 + j] = o[j];
-  }
+  for (int i = 0; i < E; ++i) sm_o[warp][i * 32 + lane] = o[i];
   __syncthreads();
   float top = sm_m[0], total = 0.0f, part[WARPS];
-  for (int w = 1; w < WARPS; ++w) top = fmaxf(top, sm_m[w]);
-  const float base = top == -INFINITY ? 0.0f : top;
-  for (int w = 0; w < WARPS; ++w) {
-    part[w] = expf(sm_m[w] - base);
-    total += sm_l[w] * part[w];
-  }
-  const float scale = (sizeof(C) == 1 ? p.kv.v_scale[hk] : 1.0f) / (total == 0.0f ? 1.0f : total);
-  if (warp == 0 && mine) {
-    float r[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      r[j] = 0.0f;
-      for (int w = 0; w < WARPS; ++w) r[j] += sm_o[w][lane * 8 + j] * part[w];
-      r[j] *= scale;
-    }
-    store8(reinterpret_cast<T*>(p.out.data) + b * p.out.row + (int64_t)h * p.out.head + lane * 8, r);
+  for (int w = 1; w < WARPS; ++w) top = fmaxf(top, sm_m[w]);
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    part[w] = sm_m[w] == top ? 1.0f : exp2_fast(sm_m[w] - top);
+    total = fmaf(sm_l[w], part[w], total);
   }
-  if (threadIdx.x == 0 && p.lse) p.lse[b * p.q_heads + h] = total == 0.0f ? -INFINITY : base + logf(total);
+  const float scale = (S::E8 ? p.kv.v_scale[it.hk] : 1.0f) / (total == 0.0f ? 1.0f : total);
+  for (int ch = threadIdx.x; ch < p.kv.dim; ch += WARPS * 32) {
+    float y = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) y = fmaf(sm_o[w][ch], part[w], y);
+    T* out = reinterpret_cast<T*>(p.out.data) + it.b * p.out.row + (int64_t)(it.first_head + h) * p.out.head + ch;
+    if constexpr (std::is_same<T, __half>::value) *out = __float2half_rn(y * scale);
+    else *out = __float2bfloat16_rn(y * scale);
+  }
+  if (threadIdx.x == 0 && p.lse)
+    p.lse[it.b * p.q_heads + it.first_head + h] = total == 0.0f ? -INFINITY : (top - S::BIAS + log2f(total)) * 0.6931471805599453f;
+}
+
+// Blocks of the persistent grid (also the number of pairs of workspace slots).
+inline int grid_blocks(int dp, int nt) { return sm_count() * blocks_per_sm(dp, nt); }
+
+template <typename T, typename C, int DP, int NT>
+static int launch(AttentionParams p, int64_t most_tokens, cudaStream_t stream) {
+  using S = Shape<T, C, DP, NT>;
+  constexpr int smem = (WARPS * S::HEADS * S::PITCH + 2 * WARPS * S::HEADS) * 4;
+  auto kern = attention_kernel<T, C, DP, NT>;
+  static_assert(smem <= 48 * 1024, "more shared memory than a launch gets without asking");
+  const int64_t items = p.entries * (p.pages ? p.chunks : p.kv.heads * p.chunks);
+  const int64_t most_units = (most_tokens + S::UNIT - 1) / S::UNIT;
+  p.whole = most_units <= WHOLE_UNITS;
+  if (p.whole) {
+    kern<<<(unsigned)items, WARPS * 32, smem, stream>>>(p);
+    return (int)cudaGetLastError();
+  }
+  const int64_t most_blocks = (items * most_units + MIN_UNITS - 1) / MIN_UNITS;
+  const int blocks = (int)min((int64_t)grid_blocks(DP, NT), most_blocks);
+  kern<<<blocks, WARPS * 32, smem, stream>>>(p);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || blocks == 1) return (int)e;
+  // the join may start while the last blocks still run: it finds its item, then waits for them
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks - 1, min(S::HEADS, p.group));
+  cfg.blockDim = dim3(WARPS * 32);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return (int)cudaLaunchKernelEx(&cfg, join_kernel<T, C, DP, NT>, p, blocks);
+}
+
+template <typename T, typename C>
+static int dispatch(const AttentionParams& p, int64_t most_tokens, cudaStream_t stream) {
+  const int dp = pad_dim(p.kv.dim), nt = head_tiles(dp, p.group);
+  if (dp == 64) return nt == 1 ? launch<T, C, 64, 1>(p, most_tokens, stream) : launch<T, C, 64, 2>(p, most_tokens, stream);
+  if (dp == 128) return nt == 1 ? launch<T, C, 128, 1>(p, most_tokens, stream) : launch<T, C, 128, 2>(p, most_tokens, stream);
+  return launch<T, C, 256, 1>(p, most_tokens, stream);
 }
 
 }  // namespace kv
@@ -109,7 +692,11 @@ __global__ void __launch_bounds__(WARPS * 32) attention_kernel(const AttentionPa
 using namespace wush;
 using namespace wush::kv;
 
-extern "C" size_t wush_kv_attention_workspace_bytes(const wush_kv_pages*, int) { return 0; }
+extern "C" size_t wush_kv_attention_workspace_bytes(const wush_kv_pages* kv, int q_heads) {
+  if (!kv || kv->heads <= 0 || q_heads <= 0 || kv->dim <= 0 || kv->dim > MAX_DIM) return 0;
+  const int dp = pad_dim(kv->dim), nt = head_tiles(dp, q_heads / kv->heads);
+  return (size_t)2 * grid_blocks(dp, nt) * nt * 8 * (dp + 2) * sizeof(float);
+}
 
 extern "C" int wush_kv_attention(const wush_kv_pages* kv, const wush_kv_table* table, int type, const wush_heads* q, int q_heads,
                                  const wush_heads* out, float* lse, const int32_t* seq_lens, float scale, int64_t window,
@@ -123,17 +710,35 @@ extern "C" int wush_kv_attention(const wush_kv_pages* kv, const wush_kv_table* t
   if (pages && window != 0) return WUSH_ERR_BAD_FLAG;
   if (table->seqs == 0) return WUSH_OK;
   if ((rc = check_heads(q, 2)) != 0 || (rc = check_heads(out, 2)) != 0) return rc;
-  if (!seq_lens) return WUSH_ERR_NULL_POINTER;
+  if (!seq_lens || !workspace) return WUSH_ERR_NULL_POINTER;
+  if (!aligned16(workspace)) return WUSH_ERR_BAD_ALIGNMENT;
   if (workspace_bytes < wush_kv_attention_workspace_bytes(kv, q_heads)) return WUSH_ERR_WORKSPACE_TOO_SMALL;
   if (table->seqs * q_heads > INT32_MAX) return WUSH_ERR_TOO_LARGE;
   if ((rc = require_sm100()) != 0) return rc;
-  const AttentionParams p{*kv, *table, *q, *out, lse, seq_lens, pages, counts, status, scale, window, q_heads, top};
-  auto go = [&](auto kern) {
-    kern<<<(unsigned)(table->seqs * q_heads), WARPS * 32, 0, (cudaStream_t)stream>>>(p);
-    return (int)cudaGetLastError();
-  };
+  AttentionParams p{};
+  p.kv = *kv;
+  p.table = *table;
+  p.q = *q;
+  p.out = *out;
+  p.lse = lse;
+  p.seq_lens = seq_lens;
+  p.pages = pages;
+  p.counts = counts;
+  p.status = status;
+  p.scale = scale;
+  p.window = window;
+  p.q_heads = q_heads;
+  p.group = q_heads / kv->heads;
+  p.top = top;
+  const int dp = pad_dim(kv->dim), nt = head_tiles(dp, p.group), heads = nt * 8;
+  p.chunks = (p.group + heads - 1) / heads;
+  p.entries = pages ? table->seqs * kv->heads : table->seqs;
+  p.part_o = reinterpret_cast<float*>(workspace);
+  p.part_ml = p.part_o + (size_t)2 * grid_blocks(dp, nt) * heads * dp;
+  int64_t most = pages ? (int64_t)top * kv->page_size : table->width * kv->page_size;   // tokens an item can have
+  if (window > 0 && window < most) most = window;
+  cudaStream_t s = (cudaStream_t)stream;
   if (type == WUSH_TYPE_BF16)
-    return kv->type == WUSH_TYPE_E4M3 ? go(attention_kernel<__nv_bfloat16, __nv_fp8_e4m3>)
-                                      : go(attention_kernel<__nv_bfloat16, __nv_bfloat16>);
-  return kv->type == WUSH_TYPE_E4M3 ? go(attention_kernel<__half, __nv_fp8_e4m3>) : go(attention_kernel<__half, __half>);
+    return kv->type == WUSH_TYPE_E4M3 ? dispatch<__nv_bfloat16, __nv_fp8_e4m3>(p, most, s) : dispatch<__nv_bfloat16, __nv_bfloat16>(p, most, s);
+  return kv->type == WUSH_TYPE_E4M3 ? dispatch<__half, __nv_fp8_e4m3>(p, most, s) : dispatch<__half, __half>(p, most, s);
 }
