@@ -74,20 +74,14 @@ __host__ __device__ inline int pad_dim(int d) { return d <= 64 ? 64 : (d <= 128 
 __host__ __device__ inline int head_tiles(int dp, int group) { return dp == 256 || group <= 8 ? 1 : 2; }
 
 // ---- instructions ------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ uint4 load16(const void* p, bool ok) {
+__device__ __forceinline__ uint4 load16(const void* p) {
   uint4 v;
-  asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %5, 0;\nmov.b32 %0, 0;\nmov.b32 %1, 0;\nmov.b32 %2, 0;\nmov.b32 %3, 0;\n"
-               "@p ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n}\n"
-               : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
-               : "l"(p), "r"((int)ok));
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
 }
-__device__ __forceinline__ uint2 load8b(const void* p, bool ok) {
+__device__ __forceinline__ uint2 load8b(const void* p) {
   uint2 v;
-  asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %3, 0;\nmov.b32 %0, 0;\nmov.b32 %1, 0;\n"
-               "@p ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];\n}\n"
-               : "=&r"(v.x), "=&r"(v.y)
-               : "l"(p), "r"((int)ok));
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "l"(p));
   return v;
 }
 
@@ -340,34 +334,34 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
       v_at = ok ? x.page * p.kv.v_page + x.row * p.kv.v_row : 0;
       seen_next = __ballot_sync(0xffffffffu, ok);
     };
-    auto load_keys = [&](unsigned mask) {
+    // Loads are never predicated: a token that does not count is read from the first row of the pool, a channel behind the
+    // last from the first one.  (Zeroing in the load made the compiler wait for it on the spot.)
+    auto load_keys = [&]() {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const int tok = mt * 16 + half * 8 + r;
           const C* row = k_head + __shfl_sync(0xffffffffu, k_at, tok);
-          const bool ok = mask >> tok & 1;
 #pragma unroll
           for (int j = 0; j < KJ; ++j) {
             const int ch = (j * 4 + c) * (16 / (int)sizeof(C));
-            kf[mt][half][j] = load16(row + ch, ok && ch < d);
+            kf[mt][half][j] = load16(row + (ch < d ? ch : 0));
           }
         }
     };
-    auto load_values = [&](unsigned mask) {
+    auto load_values = [&]() {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const int tok = mt * 16 + 2 * c + (x & 1) + (x >> 1) * 8;
           const C* row = v_head + __shfl_sync(0xffffffffu, v_at, tok);
-          const bool ok = mask >> tok & 1;
 #pragma unroll
           for (int j = 0; j < VJ; ++j) {
-            const int ch = j * 64 + r * 8;
-            if constexpr (S::E8) vf[mt][x][j] = load8b(row + ch, ok && ch < d);
-            else vf[mt][x][j] = load16(row + ch, ok && ch < d);
+            const int ch = j * 64 + r * 8 < d ? j * 64 + r * 8 : 0;
+            if constexpr (S::E8) vf[mt][x][j] = load8b(row + ch);
+            else vf[mt][x][j] = load16(row + ch);
           }
         }
     };
@@ -381,12 +375,21 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
       resolve(first);
     }
     if (base < s1) {
-      load_keys(seen_next);
-      if (S::OVERLAP) load_values(seen_next);
+      load_keys();
+      if (S::OVERLAP) load_values();
     }
     for (; base < s1; base += step) {
       seen = seen_next;
-      // logits
+      // logits; the queries are zero behind channel d, and the keys read there must not turn that into NaN
+      if (d != DP) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int j = 0; j < KJ; ++j)
+              if ((j * 4 + c) * (16 / (int)sizeof(C)) >= d) kf[mt][half][j] = make_uint4(0, 0, 0, 0);
+      }
       float s[MT][NT][4];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
@@ -409,9 +412,9 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
             }
           }
         }
-      if (!S::OVERLAP) load_values(seen);
+      if (!S::OVERLAP) load_values();
       resolve(next);                                         // from here on k_at and v_at are the next tile's
-      if (S::OVERLAP && base + step < s1) load_keys(seen_next);
+      if (S::OVERLAP && base + step < s1) load_keys();
       next = physical(after);
       after = logical(base + 3 * step);
 
@@ -476,7 +479,17 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
           }
       }
 
-      // values
+      // values; those of tokens that do not count must not meet their zero weights as NaN
+      if (seen != 0xffffffffu) {                             // (lanes 16 to 31 repeat the tokens of 0 to 15 when TT is 16)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (!(seen >> (mt * 16 + 2 * c + (x & 1) + (x >> 1) * 8) & 1)) {
+#pragma unroll
+              for (int j = 0; j < VJ; ++j) vf[mt][x][j] = VT{};
+            }
+      }
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -507,8 +520,8 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
             }
           }
       if (base + step < s1) {
-        if (S::OVERLAP) load_values(seen_next);
-        else load_keys(seen_next);
+        if (S::OVERLAP) load_values();
+        else load_keys();
       }
     }
 
