@@ -7,10 +7,10 @@
 // Products.  All G queries of a key head are worked on together, with the tokens as the rows of m16n8k16 products:
 //     S^T [16 tokens x 8 heads] = K [16 tokens x 16 channels] . Q^T,     O^T [16 channels x 8 heads] += V^T . P^T.
 // A product does not care in which order its contracted index runs, nor which row is which channel, so a lane's fragment
-// of K is a 16-byte piece of a key row and its fragment of V eight neighbouring channels of four tokens: both come
-// straight from global memory into registers with 16-byte loads (eight for 8-bit values), without shared memory, and the
-// queries are loaded in the matching order.  P is turned from the layout of an accumulator into that of an operand by
-// movmatrix.  8-bit pages are widened to fp16 (exact) in registers.
+// of K is a 16-byte piece of a key row and its fragment of V neighbouring channels of four tokens.  Every lane copies its
+// own pieces into shared memory asynchronously, two tiles ahead, and reads back what it copied: the ring is an extension
+// of its registers, free of bank conflicts, barriers and swizzles, and the queries are loaded in the matching order.  P is
+// turned from the layout of an accumulator into that of an operand by movmatrix.  8-bit pages are widened to fp16 (exact).
 //
 // Work.  The tokens of all (sequence, key head, chunk of queries) items are cut into units of 4 tiles (one per warp), the
 // units of all items are numbered through, and every block of a grid that fills the GPU exactly once takes an equal run
@@ -45,8 +45,13 @@ struct AttentionParams {
   int64_t entries;                      // sequences, or (sequence, key head) pairs when pages are selected
 };
 
-// resident blocks per SM, by the registers of the fragments
-__host__ __device__ constexpr int blocks_per_sm(int dp, int nt) { return dp == 64 ? (nt == 1 ? 4 : 3) : (dp == 128 && nt == 1 ? 3 : 2); }
+// Tokens of a tile, and resident blocks per SM: by the rings of their warps (three tiles each) in 227 KB of shared memory,
+// and by the registers where a key head has more than 8 queries.
+__host__ __device__ constexpr int tile_tokens(int dp, int esize) { return dp < 256 && (esize == 1 || dp == 64) ? 32 : 16; }
+__host__ __device__ constexpr int blocks_per_sm(int dp, int esize, int nt) {
+  const int fit = 18 * 1024 / (2 * tile_tokens(dp, esize) * dp * esize);
+  return nt == 2 && fit > 3 ? 3 : fit;
+}
 
 // ---- shape of an instantiation -----------------------------------------------------------------------------------------
 // T: queries and result; C: pages; DP: channels, rounded up to 64, 128 or 256; NT: tiles of 8 query heads.
@@ -54,36 +59,42 @@ template <typename T, typename C, int DP, int NT>
 struct Shape {
   static constexpr bool E8 = sizeof(C) == 1;
   // tokens a warp holds at a time: 4 KB of keys and as much of values, in 32 + 32 registers of a lane (128 channels)
-  static constexpr int TT = (DP < 256 && (E8 || DP == 64)) ? 32 : 16;
+  static constexpr int TT = tile_tokens(DP, (int)sizeof(C));
   static constexpr int MT = TT / 16;
   static constexpr int KJ = DP * (int)sizeof(C) / 64;       // 16-byte pieces of a key row per lane
-  static constexpr int VJ = DP / 64;                        // pieces of 8 channels of a value row per lane
+  static constexpr int VC = E8 && DP >= 128 ? 16 : 8;       // channels of a piece of a value row
+  static constexpr int VB = VC * (int)sizeof(C);            // its bytes: 16, or 8 for short rows of 8-bit values
+  static constexpr int VJ = DP / (8 * VC);                  // pieces per lane
+  static constexpr int VI = VC / 2;                         // products of 16 channels they make
+  static constexpr int K_BYTES = MT * 2 * KJ * 512, V_BYTES = MT * 4 * VJ * 32 * VB;   // of a tile
+  static constexpr int STAGE = K_BYTES + V_BYTES;
   static constexpr int HEADS = NT * 8;
   static constexpr int UNIT = WARPS * TT;                   // tokens of a unit
-  static constexpr bool OVERLAP = DP < 256 || E8;           // next keys are loaded while the values are worked on
+  static constexpr int STAGES = 3;                          // tiles of a warp in shared memory or on the way there
   // P as two 16-bit terms: one term costs 2^-9 (bf16) or 2^-12 (fp16) of a weight, which a bf16 result hides only with fp16
   static constexpr bool TWO = !(E8 && sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value);
   using M = typename std::conditional<E8, __half, T>::type; // operand type of the products
   // fp16 weights are scaled by 2^14 so that small ones stay normal numbers
   static constexpr float BIAS = std::is_same<M, __half>::value ? 14.0f : 0.0f;
-  static constexpr int BLOCKS = blocks_per_sm(DP, NT);
+  static constexpr int BLOCKS = blocks_per_sm(DP, (int)sizeof(C), NT);
   static constexpr int PITCH = DP + 4;                      // floats of a head's row in shared memory
+  static constexpr int RING = STAGES * STAGE > HEADS * PITCH * 4 ? STAGES * STAGE : HEADS * PITCH * 4;   // bytes of a warp
 };
 
 __host__ __device__ inline int pad_dim(int d) { return d <= 64 ? 64 : (d <= 128 ? 128 : 256); }
 __host__ __device__ inline int head_tiles(int dp, int group) { return dp == 256 || group <= 8 ? 1 : 2; }
 
 // ---- instructions ------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ uint4 load16(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
+// asynchronous copy of a lane's piece into shared memory; zeros when !ok
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ uint2 load8b(const void* p) {
-  uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "l"(p));
-  return v;
+__device__ __forceinline__ void copy8(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(dst), "l"(src), "r"(ok ? 8 : 0) : "memory");
 }
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
 
 template <typename M>
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -197,13 +208,14 @@ template <typename T, typename C, int DP, int NT>
 __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) attention_kernel(const AttentionParams p) {
   using S = Shape<T, C, DP, NT>;
   using M = typename S::M;
-  constexpr int MT = S::MT, KJ = S::KJ, VJ = S::VJ, TT = S::TT;
-  extern __shared__ float smem[];
-  float* sm_o = smem;                                        // [WARPS][HEADS][PITCH]
-  float* sm_m = smem + WARPS * S::HEADS * S::PITCH;          // [WARPS][HEADS]
-  float* sm_l = sm_m + WARPS * S::HEADS;
+  constexpr int MT = S::MT, KJ = S::KJ, VJ = S::VJ, VI = S::VI, TT = S::TT;
+  // every warp's ring of tiles; between walks it holds the warp's part of the result, [HEADS][PITCH] floats
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ float sm_m[WARPS * S::HEADS], sm_l[WARPS * S::HEADS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int r = lane >> 2, c = lane & 3;
+  uint8_t* ring = smem + warp * S::RING;
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
   const int d = p.kv.dim, page_size = p.kv.page_size;
   const int copies = p.pages ? p.chunks : p.kv.heads * p.chunks;
 
@@ -291,7 +303,7 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
     }
 
     // -- the walk --------------------------------------------------------------------------------------------------------
-    float m[NT][2], l[NT][2], o[NT][VJ][4][4];
+    float m[NT][2], l[NT][2], o[NT][VJ][VI][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       m[nt][0] = m[nt][1] = -INFINITY;
@@ -299,11 +311,8 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
 #pragma unroll
       for (int j = 0; j < VJ; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[nt][j][i][0] = o[nt][j][i][1] = o[nt][j][i][2] = o[nt][j][i][3] = 0.0f;
+        for (int i = 0; i < VI; ++i) o[nt][j][i][0] = o[nt][j][i][1] = o[nt][j][i][2] = o[nt][j][i][3] = 0.0f;
     }
-    uint4 kf[MT][2][KJ];
-    using VT = typename std::conditional<S::E8, uint2, uint4>::type;
-    VT vf[MT][4][VJ];
     const C* k_head = reinterpret_cast<const C*>(p.kv.k) + it.hk * p.kv.k_head;
     const C* v_head = reinterpret_cast<const C*>(p.kv.v) + it.hk * p.kv.v_head;
     const int32_t* list = p.pages ? p.pages + at.entry * p.top : nullptr;
@@ -325,18 +334,14 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
       return {(int64_t)lp * page_size + row < w.len ? lp : -1, row};
     };
     auto physical = [&](Row x) -> Row { return {x.page >= 0 ? table[x.page] : -2, x.row}; };
-    int64_t k_at, v_at;                                      // the lane's token: element offsets of its rows
-    unsigned seen = 0, seen_next = 0;                        // tokens of the tile that count
-    auto resolve = [&](Row x) {
-      bool ok = x.page >= 0 && x.page < p.kv.num_pages;
+    // the copies of a tile into a stage of the ring, piece by piece [piece][lane]; returns the tokens that count
+    auto fetch = [&](Row x, int stage) -> unsigned {
+      const bool ok = x.page >= 0 && x.page < p.kv.num_pages;
       if (!ok && x.page != -2) report_index(p.status);
-      k_at = ok ? x.page * p.kv.k_page + x.row * p.kv.k_row : 0;
-      v_at = ok ? x.page * p.kv.v_page + x.row * p.kv.v_row : 0;
-      seen_next = __ballot_sync(0xffffffffu, ok);
-    };
-    // Loads are never predicated: a token that does not count is read from the first row of the pool, a channel behind the
-    // last from the first one.  (Zeroing in the load made the compiler wait for it on the spot.)
-    auto load_keys = [&]() {
+      const int64_t k_at = ok ? x.page * p.kv.k_page + x.row * p.kv.k_row : 0;     // the lane's token: element offsets
+      const int64_t v_at = ok ? x.page * p.kv.v_page + x.row * p.kv.v_row : 0;
+      const unsigned mask = __ballot_sync(0xffffffffu, ok);
+      uint32_t dst = ring_at + stage * S::STAGE;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -346,77 +351,79 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
 #pragma unroll
           for (int j = 0; j < KJ; ++j) {
             const int ch = (j * 4 + c) * (16 / (int)sizeof(C));
-            kf[mt][half][j] = load16(row + (ch < d ? ch : 0));
+            copy16(dst, row + (ch < d ? ch : 0), (mask >> tok & 1) && ch < d);
+            dst += 512;
           }
         }
-    };
-    auto load_values = [&]() {
+      if (S::VB == 8) dst -= lane * 8;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int tok = mt * 16 + 2 * c + (x & 1) + (x >> 1) * 8;
+        for (int x4 = 0; x4 < 4; ++x4) {
+          const int tok = mt * 16 + 2 * c + (x4 & 1) + (x4 >> 1) * 8;
           const C* row = v_head + __shfl_sync(0xffffffffu, v_at, tok);
 #pragma unroll
           for (int j = 0; j < VJ; ++j) {
-            const int ch = j * 64 + r * 8 < d ? j * 64 + r * 8 : 0;
-            if constexpr (S::E8) vf[mt][x][j] = load8b(row + ch);
-            else vf[mt][x][j] = load16(row + ch);
+            const int ch = (j * 8 + r) * S::VC;
+            if (S::VB == 8) copy8(dst, row + (ch < d ? ch : 0), (mask >> tok & 1) && ch < d);
+            else copy16(dst, row + (ch < d ? ch : 0), (mask >> tok & 1) && ch < d);
+            dst += 32 * S::VB;
           }
         }
+      return mask;
     };
 
-    int64_t base = u0 * S::UNIT + warp * TT;
-    Row next, after;                                         // physical rows of the next tile, logical ones of that after it
-    {
-      const Row first = physical(logical(base));
-      next = physical(logical(base + step));
-      after = logical(base + 2 * step);
-      resolve(first);
+    // Tiles are fetched STAGES - 1 ahead of the one worked on.  A lane waits for and reads only what it copied itself, so
+    // the ring needs no barriers.
+    const int64_t first = u0 * S::UNIT + warp * TT;
+    unsigned seen[S::STAGES];                                // tokens that count of the tiles in the ring, oldest first
+    Row next = physical(logical(first)), after = logical(first + step);
+#pragma unroll
+    for (int i = 0; i < S::STAGES - 1; ++i) {
+      seen[i] = 0;
+      if (first + i * step < s1) seen[i] = fetch(next, i);
+      copy_commit();
+      next = physical(after);
+      after = logical(first + (i + 2) * step);
     }
-    if (base < s1) {
-      load_keys();
-      if (S::OVERLAP) load_values();
-    }
-    for (; base < s1; base += step) {
-      seen = seen_next;
-      // logits; the queries are zero behind channel d, and the keys read there must not turn that into NaN
-      if (d != DP) {
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int j = 0; j < KJ; ++j)
-              if ((j * 4 + c) * (16 / (int)sizeof(C)) >= d) kf[mt][half][j] = make_uint4(0, 0, 0, 0);
-      }
+    int stage = 0;
+    for (int64_t base = first; base < s1; base += step) {
+      seen[S::STAGES - 1] = 0;
+      if (base + (S::STAGES - 1) * step < s1) seen[S::STAGES - 1] = fetch(next, stage == 0 ? S::STAGES - 1 : stage - 1);
+      copy_commit();
+      next = physical(after);
+      after = logical(base + (S::STAGES + 1) * step);
+      copy_wait<S::STAGES - 1>();
+      const uint8_t* tile = ring + stage * S::STAGE + lane * 16;
+      stage = stage + 1 == S::STAGES ? 0 : stage + 1;
+      // logits
       float s[MT][NT][4];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          s[mt][nt][0] = s[mt][nt][1] = s[mt][nt][2] = s[mt][nt][3] = 0.0f;
+        for (int nt = 0; nt < NT; ++nt) s[mt][nt][0] = s[mt][nt][1] = s[mt][nt][2] = s[mt][nt][3] = 0.0f;
 #pragma unroll
-          for (int j = 0; j < KJ; ++j) {
-            const uint32_t lo[4] = {kf[mt][0][j].x, kf[mt][0][j].y, kf[mt][0][j].z, kf[mt][0][j].w};
-            const uint32_t hi[4] = {kf[mt][1][j].x, kf[mt][1][j].y, kf[mt][1][j].z, kf[mt][1][j].w};
-            if constexpr (S::E8) {
+        for (int j = 0; j < KJ; ++j) {
+          const uint4 k0 = *reinterpret_cast<const uint4*>(tile + ((mt * 2 + 0) * KJ + j) * 512);
+          const uint4 k1 = *reinterpret_cast<const uint4*>(tile + ((mt * 2 + 1) * KJ + j) * 512);
+          const uint32_t lo[4] = {k0.x, k0.y, k0.z, k0.w}, hi[4] = {k1.x, k1.y, k1.z, k1.w};
+          if constexpr (S::E8) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                mma<M>(s[mt][nt], e4m3x2_to_f16x2(lo[i]), e4m3x2_to_f16x2(hi[i]), e4m3x2_to_f16x2(lo[i] >> 16),
-                       e4m3x2_to_f16x2(hi[i] >> 16), qf[nt][j * 4 + i][0], qf[nt][j * 4 + i][1]);
-            } else {
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t a0 = e4m3x2_to_f16x2(lo[i]), a1 = e4m3x2_to_f16x2(hi[i]), a2 = e4m3x2_to_f16x2(lo[i] >> 16),
+                             a3 = e4m3x2_to_f16x2(hi[i] >> 16);
 #pragma unroll
-              for (int i = 0; i < 2; ++i)
-                mma<M>(s[mt][nt], lo[2 * i], hi[2 * i], lo[2 * i + 1], hi[2 * i + 1], qf[nt][2 * j + i][0], qf[nt][2 * j + i][1]);
+              for (int nt = 0; nt < NT; ++nt) mma<M>(s[mt][nt], a0, a1, a2, a3, qf[nt][j * 4 + i][0], qf[nt][j * 4 + i][1]);
             }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                mma<M>(s[mt][nt], lo[2 * i], hi[2 * i], lo[2 * i + 1], hi[2 * i + 1], qf[nt][2 * j + i][0], qf[nt][2 * j + i][1]);
           }
         }
-      if (!S::OVERLAP) load_values();
-      resolve(next);                                         // from here on k_at and v_at are the next tile's
-      if (S::OVERLAP && base + step < s1) load_keys();
-      next = physical(after);
-      after = logical(base + 3 * step);
+      }
 
       // softmax: running maximum per head, weights relative to it
       float top[NT][2];
@@ -430,7 +437,7 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
               float& y = s[mt][nt][half * 2 + e];
-              y = seen >> (mt * 16 + half * 8 + r) & 1 ? y * factor[nt][e] : -INFINITY;
+              y = seen[0] >> (mt * 16 + half * 8 + r) & 1 ? y * factor[nt][e] : -INFINITY;
               x = fmaxf(x, y);
             }
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
@@ -452,7 +459,7 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
 #pragma unroll
             for (int j = 0; j < VJ; ++j)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
+              for (int i = 0; i < VI; ++i) {
                 o[nt][j][i][e] *= keep;
                 o[nt][j][i][2 + e] *= keep;
               }
@@ -479,39 +486,42 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
           }
       }
 
-      // values; those of tokens that do not count must not meet their zero weights as NaN
-      if (seen != 0xffffffffu) {                             // (lanes 16 to 31 repeat the tokens of 0 to 15 when TT is 16)
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-            if (!(seen >> (mt * 16 + 2 * c + (x & 1) + (x >> 1) * 8) & 1)) {
-#pragma unroll
-              for (int j = 0; j < VJ; ++j) vf[mt][x][j] = VT{};
-            }
-      }
+      // values
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int j = 0; j < VJ; ++j)
+        for (int j = 0; j < VJ; ++j) {
+          uint32_t w[4][4];                                  // the pieces of tokens 2c, 2c + 1, 2c + 8, 2c + 9
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t a0, a1, a2, a3;                         // channels 2i and 2i + 1 of the lane's eight
+          for (int x = 0; x < 4; ++x) {
+            const uint8_t* at_v = tile + S::K_BYTES + ((mt * 4 + x) * VJ + j) * (32 * S::VB);
+            if constexpr (S::VB == 8) {
+              const uint2 v = *reinterpret_cast<const uint2*>(at_v - lane * 8);
+              w[x][0] = v.x;
+              w[x][1] = v.y;
+            } else {
+              const uint4 v = *reinterpret_cast<const uint4*>(at_v);
+              w[x][0] = v.x;
+              w[x][1] = v.y;
+              w[x][2] = v.z;
+              w[x][3] = v.w;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < VI; ++i) {
+            uint32_t a0, a1, a2, a3;                         // channels 2i and 2i + 1 of the lane's piece
             if constexpr (S::E8) {
               const uint32_t sel = i & 1 ? 0x7362 : 0x5140;  // bytes of tokens t, t + 1 side by side
-              const uint32_t x = __byte_perm(i < 2 ? vf[mt][0][j].x : vf[mt][0][j].y, i < 2 ? vf[mt][1][j].x : vf[mt][1][j].y, sel);
-              const uint32_t y = __byte_perm(i < 2 ? vf[mt][2][j].x : vf[mt][2][j].y, i < 2 ? vf[mt][3][j].x : vf[mt][3][j].y, sel);
+              const uint32_t x = __byte_perm(w[0][i >> 1], w[1][i >> 1], sel), y = __byte_perm(w[2][i >> 1], w[3][i >> 1], sel);
               a0 = e4m3x2_to_f16x2(x);
               a1 = e4m3x2_to_f16x2(x >> 16);
               a2 = e4m3x2_to_f16x2(y);
               a3 = e4m3x2_to_f16x2(y >> 16);
             } else {
-              auto word = [&](const uint4& q) { return i == 0 ? q.x : (i == 1 ? q.y : (i == 2 ? q.z : q.w)); };
-              const uint32_t t0 = word(vf[mt][0][j]), t1 = word(vf[mt][1][j]), t2 = word(vf[mt][2][j]), t3 = word(vf[mt][3][j]);
-              a0 = __byte_perm(t0, t1, 0x5410);
-              a1 = __byte_perm(t0, t1, 0x7632);
-              a2 = __byte_perm(t2, t3, 0x5410);
-              a3 = __byte_perm(t2, t3, 0x7632);
+              a0 = __byte_perm(w[0][i], w[1][i], 0x5410);
+              a1 = __byte_perm(w[0][i], w[1][i], 0x7632);
+              a2 = __byte_perm(w[2][i], w[3][i], 0x5410);
+              a3 = __byte_perm(w[2][i], w[3][i], 0x7632);
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -519,14 +529,13 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
               if (S::TWO) mma<M>(o[nt][j][i], a0, a1, a2, a3, pl[mt][nt][0], pl[mt][nt][1]);
             }
           }
-      if (base + step < s1) {
-        if (S::OVERLAP) load_values();
-        else load_keys();
-      }
+        }
+#pragma unroll
+      for (int i = 0; i < S::STAGES - 1; ++i) seen[i] = seen[i + 1];
     }
 
     // -- join the warps --------------------------------------------------------------------------------------------------
-    __syncthreads();                                         // the previous item's shared memory has been read
+    copy_wait<0>();
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -540,12 +549,13 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
           sm_m[warp * S::HEADS + h] = m[nt][e];
           sm_l[warp * S::HEADS + h] = x;
         }
-        float* row = sm_o + (warp * S::HEADS + h) * S::PITCH + r * 8;
+        float* row = reinterpret_cast<float*>(ring) + h * S::PITCH + r * S::VC;
 #pragma unroll
-        for (int j = 0; j < VJ; ++j) {
-          *reinterpret_cast<float4*>(row + j * 64) = make_float4(o[nt][j][0][e], o[nt][j][0][2 + e], o[nt][j][1][e], o[nt][j][1][2 + e]);
-          *reinterpret_cast<float4*>(row + j * 64 + 4) = make_float4(o[nt][j][2][e], o[nt][j][2][2 + e], o[nt][j][3][e], o[nt][j][3][2 + e]);
-        }
+        for (int j = 0; j < VJ; ++j)
+#pragma unroll
+          for (int i = 0; i < VI; i += 2)
+            *reinterpret_cast<float4*>(row + j * 8 * S::VC + 2 * i) =
+                make_float4(o[nt][j][i][e], o[nt][j][i][2 + e], o[nt][j][i + 1][e], o[nt][j][i + 1][2 + e]);
       }
     __syncthreads();
     const bool all = u0 == 0 && u1 == at.units;
@@ -562,7 +572,7 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
         const float mk = sm_m[k * S::HEADS + h];
         const float keep = mk == top ? 1.0f : exp2_fast(mk - top);
         total = fmaf(sm_l[k * S::HEADS + h], keep, total);
-        const float* row = sm_o + (k * S::HEADS + h) * S::PITCH + ch;
+        const float* row = reinterpret_cast<const float*>(smem + k * S::RING) + h * S::PITCH + ch;
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = fmaf(row[i], keep, y[i]);
       }
@@ -585,6 +595,7 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
       }
     }
     t += u1 - u0;
+    __syncthreads();                                         // the rings are free again
   }
 }
 
@@ -658,14 +669,15 @@ __global__ void __launch_bounds__(WARPS * 32) join_kernel(const AttentionParams 
 }
 
 // Blocks of the persistent grid (also the number of pairs of workspace slots).
-inline int grid_blocks(int dp, int nt) { return sm_count() * blocks_per_sm(dp, nt); }
+inline int grid_blocks(int dp, int esize, int nt) { return sm_count() * blocks_per_sm(dp, esize, nt); }
 
 template <typename T, typename C, int DP, int NT>
 static int launch(AttentionParams p, int64_t most_tokens, cudaStream_t stream) {
   using S = Shape<T, C, DP, NT>;
-  constexpr int smem = (WARPS * S::HEADS * S::PITCH + 2 * WARPS * S::HEADS) * 4;
+  constexpr int smem = WARPS * S::RING;
   auto kern = attention_kernel<T, C, DP, NT>;
-  static_assert(smem <= 48 * 1024, "more shared memory than a launch gets without asking");
+  static PerDevice opted;
+  if (const int rc = opt_in_smem(opted, kern, smem)) return rc;
   const int64_t items = p.entries * (p.pages ? p.chunks : p.kv.heads * p.chunks);
   const int64_t most_units = (most_tokens + S::UNIT - 1) / S::UNIT;
   p.whole = most_units <= WHOLE_UNITS;
@@ -674,7 +686,7 @@ static int launch(AttentionParams p, int64_t most_tokens, cudaStream_t stream) {
     return (int)cudaGetLastError();
   }
   const int64_t most_blocks = (items * most_units + MIN_UNITS - 1) / MIN_UNITS;
-  const int blocks = (int)min((int64_t)grid_blocks(DP, NT), most_blocks);
+  const int blocks = (int)min((int64_t)grid_blocks(DP, (int)sizeof(C), NT), most_blocks);
   kern<<<blocks, WARPS * 32, smem, stream>>>(p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || blocks == 1) return (int)e;
@@ -706,9 +718,9 @@ using namespace wush;
 using namespace wush::kv;
 
 extern "C" size_t wush_kv_attention_workspace_bytes(const wush_kv_pages* kv, int q_heads) {
-  if (!kv || kv->heads <= 0 || q_heads <= 0 || kv->dim <= 0 || kv->dim > MAX_DIM) return 0;
+  if (!kv || kv->heads <= 0 || q_heads <= 0 || kv->dim <= 0 || kv->dim > MAX_DIM || q_heads < kv->heads) return 0;
   const int dp = pad_dim(kv->dim), nt = head_tiles(dp, q_heads / kv->heads);
-  return (size_t)2 * grid_blocks(dp, nt) * nt * 8 * (dp + 2) * sizeof(float);
+  return (size_t)2 * grid_blocks(dp, element_bytes(kv->type), nt) * nt * 8 * (dp + 2) * sizeof(float);
 }
 
 extern "C" int wush_kv_attention(const wush_kv_pages* kv, const wush_kv_table* table, int type, const wush_heads* q, int q_heads,
@@ -747,7 +759,7 @@ extern "C" int wush_kv_attention(const wush_kv_pages* kv, const wush_kv_table* t
   p.chunks = (p.group + heads - 1) / heads;
   p.entries = pages ? table->seqs * kv->heads : table->seqs;
   p.part_o = reinterpret_cast<float*>(workspace);
-  p.part_ml = p.part_o + (size_t)2 * grid_blocks(dp, nt) * heads * dp;
+  p.part_ml = p.part_o + (size_t)2 * grid_blocks(dp, element_bytes(kv->type), nt) * heads * dp;
   int64_t most = pages ? (int64_t)top * kv->page_size : table->width * kv->page_size;   // tokens an item can have
   if (window > 0 && window < most) most = window;
   cudaStream_t s = (cudaStream_t)stream;
