@@ -24,7 +24,8 @@ namespace wush {
 namespace kv {
 
 constexpr int WARPS = 4;
-constexpr int MIN_UNITS = 2;            // smallest run of units a block takes while others idle
+constexpr int START = 4;                // units that an item is worth beyond its tokens
+constexpr int MIN_UNITS = 2;            // smallest number of units a block takes while others idle
 constexpr int WHOLE_UNITS = 4;          // items of at most this many units are not split at all
 
 struct AttentionParams {
@@ -74,8 +75,9 @@ struct Shape {
   // P as two 16-bit terms: one term costs 2^-9 (bf16) or 2^-12 (fp16) of a weight, which a bf16 result hides only with fp16
   static constexpr bool TWO = !(E8 && sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value);
   using M = typename std::conditional<E8, __half, T>::type; // operand type of the products
-  // fp16 weights are scaled by 2^14 so that small ones stay normal numbers
-  static constexpr float BIAS = std::is_same<M, __half>::value ? 14.0f : 0.0f;
+  static constexpr float RISE = 8.0f;                       // exponent that a weight may reach
+  // fp16 weights are scaled by 2^7: the largest then are 2^15, and small ones stay normal numbers down to 2^-21
+  static constexpr float BIAS = std::is_same<M, __half>::value ? 7.0f : 0.0f;
   static constexpr int BLOCKS = blocks_per_sm(DP, (int)sizeof(C), NT);
   static constexpr int PITCH = DP + 4;                      // floats of a head's row in shared memory
   static constexpr int RING = STAGES * STAGE > HEADS * PITCH * 4 ? STAGES * STAGE : HEADS * PITCH * 4;   // bytes of a warp
@@ -123,50 +125,55 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 
 // ---- numbering of the work ---------------------------------------------------------------------------------------------
+// An item is worth START units for looking up its first pages, filling the ring and writing its result, and then one unit
+// for each UNIT tokens.  Without START a block whose run held a dozen short sequences finished long after the others.
 struct Work {
   int len;                              // tokens of the sequence
-  int begin;                            // first position (window); 0 when pages are selected
+  int begin;                            // first position that counts (window); 0 when pages are selected
+  int origin;                           // first position that is walked: begin, or the 16 tokens that hold it
   int tokens;                           // tokens to walk: positions, or rows of the selected pages
 };
 
+template <bool FAST>
 __device__ __forceinline__ Work work_of(const AttentionParams& p, int64_t entry) {
   const int64_t b = p.pages ? entry / p.kv.heads : entry;
   Work w;
   w.len = clamp_length(p.seq_lens[b], p.table.width * p.kv.page_size, p.status);
   w.begin = p.window > 0 && w.len > p.window ? (int)(w.len - p.window) : 0;
-  w.tokens = p.pages ? max(0, min(p.counts[entry], p.top)) * p.kv.page_size : w.len - w.begin;
+  w.origin = FAST ? w.begin & ~15 : w.begin;
+  w.tokens = p.pages ? max(0, min(p.counts[entry], p.top)) * p.kv.page_size : w.len - w.origin;
   return w;
 }
 
 // an item without tokens has one unit: somebody has to write its zeros
-template <int UNIT>
+template <bool FAST, int UNIT>
 __device__ __forceinline__ int64_t units_of(const AttentionParams& p, int64_t entry) {
-  return entry < p.entries ? max(1, (work_of(p, entry).tokens + UNIT - 1) / UNIT) : 0;
+  return entry < p.entries ? max(1, (work_of<FAST>(p, entry).tokens + UNIT - 1) / UNIT) : 0;
 }
 
 struct Place {
   int64_t entry, base;                  // entry that holds a unit, and the number of its first unit
-  int64_t units;                        // units of one item of the entry
+  int64_t units;                        // units of one item of the entry, without START
 };
 
 // Total number of units, by one warp.
-template <int UNIT>
+template <bool FAST, int UNIT>
 __device__ int64_t total_units(const AttentionParams& p, int copies) {
   const int lane = threadIdx.x & 31;
   int64_t sum = 0;
-  for (int64_t e = lane; e < p.entries; e += 32) sum += units_of<UNIT>(p, e);
+  for (int64_t e = lane; e < p.entries; e += 32) sum += START + units_of<FAST, UNIT>(p, e);
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   return sum * copies;
 }
 
 // The entry that unit t lies in, by one warp; `copies` items per entry.
-template <int UNIT>
+template <bool FAST, int UNIT>
 __device__ Place locate(const AttentionParams& p, int copies, int64_t t) {
   const int lane = threadIdx.x & 31;
   int64_t before = 0;
   for (int64_t e0 = 0; e0 < p.entries; e0 += 32) {
-    const int64_t u = units_of<UNIT>(p, e0 + lane);
-    int64_t sum = u * copies;
+    const int64_t u = units_of<FAST, UNIT>(p, e0 + lane);
+    int64_t sum = e0 + lane < p.entries ? (START + u) * copies : 0;
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t x = __shfl_up_sync(0xffffffffu, sum, o);
       if (lane >= o) sum += x;
@@ -175,7 +182,7 @@ __device__ Place locate(const AttentionParams& p, int copies, int64_t t) {
     if (beyond) {
       const int at = __ffs(beyond) - 1;
       const int64_t units = __shfl_sync(0xffffffffu, u, at);
-      return {e0 + at, before + __shfl_sync(0xffffffffu, sum, at) - units * copies, units};
+      return {e0 + at, before + __shfl_sync(0xffffffffu, sum, at) - (START + units) * copies, units};
     }
     before += __shfl_sync(0xffffffffu, sum, 31);
   }
@@ -184,7 +191,7 @@ __device__ Place locate(const AttentionParams& p, int copies, int64_t t) {
 
 __device__ __forceinline__ int64_t units_per_block(int64_t total, int64_t blocks) {
   const int64_t per = (total + blocks - 1) / blocks;
-  return per < MIN_UNITS ? MIN_UNITS : per;
+  return per < START + MIN_UNITS ? START + MIN_UNITS : per;
 }
 
 struct Item {
@@ -204,11 +211,13 @@ __device__ __forceinline__ Item item_of(const AttentionParams& p, int64_t entry,
 }
 
 // ---- the kernel --------------------------------------------------------------------------------------------------------
-template <typename T, typename C, int DP, int NT>
+// FAST: page_size is a multiple of 16, so that 16 consecutive tokens lie in one page and are looked up together.
+template <typename T, typename C, int DP, int NT, bool FAST>
 __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) attention_kernel(const AttentionParams p) {
   using S = Shape<T, C, DP, NT>;
   using M = typename S::M;
-  constexpr int MT = S::MT, KJ = S::KJ, VJ = S::VJ, VI = S::VI, TT = S::TT;
+  constexpr int MT = S::MT, KJ = S::KJ, VJ = S::VJ, VI = S::VI, TT = S::TT, CB = (int)sizeof(C);
+  constexpr unsigned FULL = TT == 32 ? 0xffffffffu : 0xffffu;
   // every warp's ring of tiles; between walks it holds the warp's part of the result, [HEADS][PITCH] floats
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float sm_m[WARPS * S::HEADS], sm_l[WARPS * S::HEADS];
@@ -218,6 +227,7 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
   const int d = p.kv.dim, page_size = p.kv.page_size;
   const int copies = p.pages ? p.chunks : p.kv.heads * p.chunks;
+  const int64_t k_row = p.kv.k_row * CB, v_row = p.kv.v_row * CB;         // bytes
 
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
 
@@ -225,30 +235,161 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
   Place at;
   if (p.whole) {
     const int64_t entry = blockIdx.x / copies;
-    at = {entry, 0, units_of<S::UNIT>(p, entry)};
-    t = t_first = (int64_t)(blockIdx.x % copies) * at.units;
-    t_end = t + at.units;
+    at = {entry, 0, units_of<FAST, S::UNIT>(p, entry)};
+    t = t_first = (int64_t)(blockIdx.x % copies) * (START + at.units);
+    t_end = t + START + at.units;
   } else {
-    const int64_t total = total_units<S::UNIT>(p, copies);
+    const int64_t total = total_units<FAST, S::UNIT>(p, copies);
     const int64_t per = units_per_block(total, gridDim.x);
     t = t_first = (int64_t)blockIdx.x * per;
     t_end = min(total, t + per);
     if (t >= t_end) return;
-    at = locate<S::UNIT>(p, copies, t);
+    at = locate<FAST, S::UNIT>(p, copies, t);
   }
 
-  while (t < t_end) {
-    if (t >= at.base + at.units * copies) {                  // the next entry
-      at.base += at.units * copies;
+  for (int64_t t_next; t < t_end; t = t_next) {
+    if (t >= at.base + (START + at.units) * copies) {        // the next entry
+      at.base += (START + at.units) * copies;
       at.entry += 1;
-      at.units = units_of<S::UNIT>(p, at.entry);
+      at.units = units_of<FAST, S::UNIT>(p, at.entry);
     }
-    const Work w = work_of(p, at.entry);
-    const int64_t copy = (t - at.base) / at.units;
-    const int64_t u0 = t - at.base - copy * at.units;
-    const int64_t u1 = min(at.units, u0 + (t_end - t));
+    const int64_t copy = (t - at.base) / (START + at.units);
+    const int64_t within = t - at.base - copy * (START + at.units);
+    t_next = t + min(START + at.units - within, t_end - t);
+    const int64_t u0 = max((int64_t)0, within - START), u1 = within + (t_next - t) - START;
+    if (u1 <= u0) continue;                                  // only the item's START: the next block has its first tokens
+    const Work w = work_of<FAST>(p, at.entry);
     const Item it = item_of<S::HEADS>(p, at.entry, copy);
     const int s1 = (int)min((int64_t)w.tokens, u1 * S::UNIT);
+
+    // -- where the tokens are --------------------------------------------------------------------------------------------
+    const uint8_t* k_head = reinterpret_cast<const uint8_t*>(p.kv.k) + it.hk * p.kv.k_head * CB;
+    const uint8_t* v_head = reinterpret_cast<const uint8_t*>(p.kv.v) + it.hk * p.kv.v_head * CB;
+    const int32_t* list = p.pages ? p.pages + at.entry * p.top : nullptr;
+    const int32_t* table = p.table.block_table + it.b * p.table.stride;
+    constexpr int STEP = S::UNIT;
+    const int first = (int)u0 * S::UNIT + warp * TT;         // the warp's tiles are first, first + STEP, ... below s1
+    // A lookup goes in levels, each of which loads for the next: walked token -> logical page and row -> physical page.
+    struct Row { int page, row, pos; };                      // page -1: outside the table, -2: nothing there
+    auto logical = [&](int v) -> Row {
+      if (v >= s1) return {-2, 0, 0};
+      const int at_v = v + w.origin, li = at_v / page_size, row = at_v - li * page_size;
+      if (!list) return {li, row, at_v};
+      const int lp = list[li];
+      if (lp < 0 || lp >= p.table.width) {
+        report_index(p.status);
+        return {-2, 0, 0};
+      }
+      return {lp, row, lp * page_size + row};
+    };
+    auto physical = [&](Row x) -> Row { return {x.page >= 0 && x.pos < w.len ? table[x.page] : -2, x.row, x.pos}; };
+    // byte offsets of the rows, and the tokens that count: one, or with FAST the 16 from there
+    int64_t k_at = 0, v_at = 0;
+    unsigned counts16 = 0;
+    auto resolve = [&](Row x) {
+      const bool ok = x.page >= 0 && x.page < p.kv.num_pages;
+      if (!ok && x.page != -2) report_index(p.status);
+      k_at = ok ? (x.page * p.kv.k_page + x.row * p.kv.k_row) * CB : 0;
+      v_at = ok ? (x.page * p.kv.v_page + x.row * p.kv.v_row) * CB : 0;
+      const int lo = max(0, w.begin - x.pos), hi = min(16, w.len - x.pos);
+      counts16 = !ok ? 0 : (FAST ? (0xffffu >> (16 - hi)) & (0xffffu << lo) : 1);
+    };
+    // FAST: lane i holds the warp's i-th group of 16 tokens of the current 32, the levels of the next 32 and of those after
+    // them are under way.  Else: lane i holds the i-th token of the next tile.
+    auto token_of = [&](int i) { return FAST ? first + i / MT * STEP + i % MT * 16 : first + i / TT * STEP + i % TT; };
+    const int held = FAST ? lane : lane & (TT - 1), hold = FAST ? 32 : TT;
+    Row next = physical(logical(token_of(held))), after = logical(token_of(hold + held));
+    auto advance = [&](int i) {                              // make the lookups from i on the current ones
+      resolve(next);
+      next = physical(after);
+      after = logical(token_of(i + 2 * hold + held));
+    };
+
+    // the copies of tile i into a stage of the ring, piece by piece [piece][lane]; returns the tokens that count
+    auto fetch = [&](int i, int stage) -> unsigned {
+      uint32_t dst = ring_at + stage * S::STAGE;
+      const uint32_t dst_v = dst + S::K_BYTES - (S::VB == 8 ? lane * 8 : 0);
+      if constexpr (FAST) {
+        if (i * MT % 32 == 0) advance(i * MT);
+        unsigned mask = 0;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          const int from = (i * MT + mt) & 31;
+          const unsigned counts = __shfl_sync(0xffffffffu, counts16, from);
+          mask |= counts << (16 * mt);
+          const uint8_t* kp = k_head + __shfl_sync(0xffffffffu, k_at, from) + r * k_row;
+          const uint8_t* vp = v_head + __shfl_sync(0xffffffffu, v_at, from) + 2 * c * v_row;
+          const uint32_t dk = dst + mt * (2 * KJ * 512), dv = dst_v + mt * (4 * VJ * 32 * S::VB);
+          const bool whole = counts == 0xffffu && d == DP;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint8_t* row = kp + half * 8 * k_row;
+            if (whole) {
+#pragma unroll
+              for (int j = 0; j < KJ; ++j) copy16(dk + (half * KJ + j) * 512, row + c * 16 + j * 64, true);
+            } else {
+#pragma unroll
+              for (int j = 0; j < KJ; ++j) {
+                const bool in = (j * 4 + c) * 16 < d * CB;
+                copy16(dk + (half * KJ + j) * 512, row + (in ? (j * 4 + c) * 16 : 0), in && (counts >> (half * 8 + r) & 1));
+              }
+            }
+          }
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const uint8_t* row = vp + ((x & 1) + (x >> 1) * 8) * v_row;
+#pragma unroll
+            for (int j = 0; j < VJ; ++j) {
+              const bool in = whole || (j * 8 + r) * S::VC < d;
+              const bool ok = whole || (in && (counts >> (2 * c + (x & 1) + (x >> 1) * 8) & 1));
+              const uint8_t* src = row + (in ? (j * 8 + r) * S::VB : 0);
+              if constexpr (S::VB == 8) copy8(dv + (x * VJ + j) * 256, src, ok);
+              else copy16(dv + (x * VJ + j) * 512, src, ok);
+            }
+          }
+        }
+        return mask;
+      } else {
+        advance(i * TT);
+        const unsigned mask = __ballot_sync(0xffffffffu, counts16 != 0);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int tok = mt * 16 + half * 8 + r;
+            const uint8_t* row = k_head + __shfl_sync(0xffffffffu, k_at, tok);
+#pragma unroll
+            for (int j = 0; j < KJ; ++j) {
+              const bool in = (j * 4 + c) * 16 < d * CB;
+              copy16(dst + ((mt * 2 + half) * KJ + j) * 512, row + (in ? (j * 4 + c) * 16 : 0), in && (mask >> tok & 1));
+            }
+          }
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int tok = mt * 16 + 2 * c + (x & 1) + (x >> 1) * 8;
+            const uint8_t* row = v_head + __shfl_sync(0xffffffffu, v_at, tok);
+#pragma unroll
+            for (int j = 0; j < VJ; ++j) {
+              const bool in = (j * 8 + r) * S::VC < d;
+              const uint8_t* src = row + (in ? (j * 8 + r) * S::VB : 0);
+              if constexpr (S::VB == 8) copy8(dst_v + ((mt * 4 + x) * VJ + j) * 256, src, in && (mask >> tok & 1));
+              else copy16(dst_v + ((mt * 4 + x) * VJ + j) * 512, src, in && (mask >> tok & 1));
+            }
+          }
+        }
+        return mask & FULL;
+      }
+    };
+
+    // Tiles are fetched STAGES - 1 ahead of the one worked on.  A lane waits for and reads only what it copied itself, so
+    // the ring needs no barriers.
+    unsigned seen[S::STAGES];                                // tokens that count of the tiles in the ring, oldest first
+#pragma unroll
+    for (int i = 0; i < S::STAGES - 1; ++i) {
+      seen[i] = 0;
+      if (first + i * STEP < s1) seen[i] = fetch(i, i);
+      copy_commit();
+    }
 
     // -- queries, in the order of the key fragments ----------------------------------------------------------------------
     uint32_t qf[NT][DP / 16][2];
@@ -313,95 +454,24 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
 #pragma unroll
         for (int i = 0; i < VI; ++i) o[nt][j][i][0] = o[nt][j][i][1] = o[nt][j][i][2] = o[nt][j][i][3] = 0.0f;
     }
-    const C* k_head = reinterpret_cast<const C*>(p.kv.k) + it.hk * p.kv.k_head;
-    const C* v_head = reinterpret_cast<const C*>(p.kv.v) + it.hk * p.kv.v_head;
-    const int32_t* list = p.pages ? p.pages + at.entry * p.top : nullptr;
-    const int32_t* table = p.table.block_table + it.b * p.table.stride;
-    const int step = S::UNIT;
-
-    // the lane's token of a tile, one level of the lookup at a time: logical page (-1: none), then physical page
-    struct Row { int page, row; };
-    auto logical = [&](int64_t base) -> Row {
-      const int64_t v = base + (lane & (TT - 1));
-      if (v >= s1) return {-1, 0};
-      const int pos = (int)v + w.begin, li = pos / page_size, row = pos - li * page_size;
-      if (!list) return {li, row};
-      const int lp = list[li];
-      if (lp < 0 || lp >= p.table.width) {
-        report_index(p.status);
-        return {-1, 0};
-      }
-      return {(int64_t)lp * page_size + row < w.len ? lp : -1, row};
-    };
-    auto physical = [&](Row x) -> Row { return {x.page >= 0 ? table[x.page] : -2, x.row}; };
-    // the copies of a tile into a stage of the ring, piece by piece [piece][lane]; returns the tokens that count
-    auto fetch = [&](Row x, int stage) -> unsigned {
-      const bool ok = x.page >= 0 && x.page < p.kv.num_pages;
-      if (!ok && x.page != -2) report_index(p.status);
-      const int64_t k_at = ok ? x.page * p.kv.k_page + x.row * p.kv.k_row : 0;     // the lane's token: element offsets
-      const int64_t v_at = ok ? x.page * p.kv.v_page + x.row * p.kv.v_row : 0;
-      const unsigned mask = __ballot_sync(0xffffffffu, ok);
-      uint32_t dst = ring_at + stage * S::STAGE;
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int tok = mt * 16 + half * 8 + r;
-          const C* row = k_head + __shfl_sync(0xffffffffu, k_at, tok);
-#pragma unroll
-          for (int j = 0; j < KJ; ++j) {
-            const int ch = (j * 4 + c) * (16 / (int)sizeof(C));
-            copy16(dst, row + (ch < d ? ch : 0), (mask >> tok & 1) && ch < d);
-            dst += 512;
-          }
-        }
-      if (S::VB == 8) dst -= lane * 8;
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int x4 = 0; x4 < 4; ++x4) {
-          const int tok = mt * 16 + 2 * c + (x4 & 1) + (x4 >> 1) * 8;
-          const C* row = v_head + __shfl_sync(0xffffffffu, v_at, tok);
-#pragma unroll
-          for (int j = 0; j < VJ; ++j) {
-            const int ch = (j * 8 + r) * S::VC;
-            if (S::VB == 8) copy8(dst, row + (ch < d ? ch : 0), (mask >> tok & 1) && ch < d);
-            else copy16(dst, row + (ch < d ? ch : 0), (mask >> tok & 1) && ch < d);
-            dst += 32 * S::VB;
-          }
-        }
-      return mask;
-    };
-
-    // Tiles are fetched STAGES - 1 ahead of the one worked on.  A lane waits for and reads only what it copied itself, so
-    // the ring needs no barriers.
-    const int64_t first = u0 * S::UNIT + warp * TT;
-    unsigned seen[S::STAGES];                                // tokens that count of the tiles in the ring, oldest first
-    Row next = physical(logical(first)), after = logical(first + step);
-#pragma unroll
-    for (int i = 0; i < S::STAGES - 1; ++i) {
-      seen[i] = 0;
-      if (first + i * step < s1) seen[i] = fetch(next, i);
-      copy_commit();
-      next = physical(after);
-      after = logical(first + (i + 2) * step);
-    }
-    int stage = 0;
-    for (int64_t base = first; base < s1; base += step) {
+    int stage = 0, ahead = S::STAGES - 1;
+    for (int base = first; base < s1; base += STEP, ++ahead) {
       seen[S::STAGES - 1] = 0;
-      if (base + (S::STAGES - 1) * step < s1) seen[S::STAGES - 1] = fetch(next, stage == 0 ? S::STAGES - 1 : stage - 1);
+      if (base + (S::STAGES - 1) * STEP < s1) seen[S::STAGES - 1] = fetch(ahead, stage == 0 ? S::STAGES - 1 : stage - 1);
       copy_commit();
-      next = physical(after);
-      after = logical(base + (S::STAGES + 1) * step);
       copy_wait<S::STAGES - 1>();
       const uint8_t* tile = ring + stage * S::STAGE + lane * 16;
       stage = stage + 1 == S::STAGES ? 0 : stage + 1;
-      // logits
+      // logits; two sums where a single chain of products would be waited for
+      constexpr int CHAINS = MT * NT == 1 ? 2 : 1;
       float s[MT][NT][4];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
+        float part[CHAINS][NT][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) s[mt][nt][0] = s[mt][nt][1] = s[mt][nt][2] = s[mt][nt][3] = 0.0f;
+        for (int x = 0; x < CHAINS; ++x)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) part[x][nt][0] = part[x][nt][1] = part[x][nt][2] = part[x][nt][3] = 0.0f;
 #pragma unroll
         for (int j = 0; j < KJ; ++j) {
           const uint4 k0 = *reinterpret_cast<const uint4*>(tile + ((mt * 2 + 0) * KJ + j) * 512);
@@ -413,49 +483,64 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
               const uint32_t a0 = e4m3x2_to_f16x2(lo[i]), a1 = e4m3x2_to_f16x2(hi[i]), a2 = e4m3x2_to_f16x2(lo[i] >> 16),
                              a3 = e4m3x2_to_f16x2(hi[i] >> 16);
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma<M>(s[mt][nt], a0, a1, a2, a3, qf[nt][j * 4 + i][0], qf[nt][j * 4 + i][1]);
+              for (int nt = 0; nt < NT; ++nt) mma<M>(part[i % CHAINS][nt], a0, a1, a2, a3, qf[nt][j * 4 + i][0], qf[nt][j * 4 + i][1]);
             }
           } else {
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt)
-                mma<M>(s[mt][nt], lo[2 * i], hi[2 * i], lo[2 * i + 1], hi[2 * i + 1], qf[nt][2 * j + i][0], qf[nt][2 * j + i][1]);
+                mma<M>(part[i % CHAINS][nt], lo[2 * i], hi[2 * i], lo[2 * i + 1], hi[2 * i + 1], qf[nt][2 * j + i][0], qf[nt][2 * j + i][1]);
           }
         }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) s[mt][nt][x] = CHAINS == 2 ? part[0][nt][x] + part[CHAINS - 1][nt][x] : part[0][nt][x];
       }
 
-      // softmax: running maximum per head, weights relative to it
-      float top[NT][2];
+      // Softmax: weights relative to a reference per head, which is raised to the running maximum only when a logit passes it
+      // by more than RISE; weights then stay below 2^RISE, and most tiles need no exchange between lanes.
+      bool rises = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) s[mt][nt][x] *= factor[nt][x & 1];
+      if (seen[0] != FULL) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              if (!(seen[0] >> (mt * 16 + (x >> 1) * 8 + r) & 1)) s[mt][nt][x] = -INFINITY;
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float x = -INFINITY;
+          float x = fmaxf(s[0][nt][e], s[0][nt][2 + e]);
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              float& y = s[mt][nt][half * 2 + e];
-              y = seen[0] >> (mt * 16 + half * 8 + r) & 1 ? y * factor[nt][e] : -INFINITY;
-              x = fmaxf(x, y);
-            }
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          top[nt][e] = fmaxf(m[nt][e], x);
+          for (int mt = 1; mt < MT; ++mt) x = fmaxf(x, fmaxf(s[mt][nt][e], s[mt][nt][2 + e]));
+          rises |= x > m[nt][e] + S::RISE;
         }
-      bool rises = false;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) rises |= top[nt][0] > m[nt][0] || top[nt][1] > m[nt][1];
       if (__any_sync(0xffffffffu, rises)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float keep = top[nt][e] == m[nt][e] ? 1.0f : exp2_fast(m[nt][e] - top[nt][e]);
+            float x = fmaxf(s[0][nt][e], s[0][nt][2 + e]);
+#pragma unroll
+            for (int mt = 1; mt < MT; ++mt) x = fmaxf(x, fmaxf(s[mt][nt][e], s[mt][nt][2 + e]));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            const float top = fmaxf(m[nt][e], x);
+            const float keep = top == m[nt][e] ? 1.0f : exp2_fast(m[nt][e] - top);
             l[nt][e] *= keep;
-            m[nt][e] = top[nt][e];
+            m[nt][e] = top;
 #pragma unroll
             for (int j = 0; j < VJ; ++j)
 #pragma unroll
@@ -559,7 +644,7 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
       }
     __syncthreads();
     const bool all = u0 == 0 && u1 == at.units;
-    const int64_t slot = 2 * (int64_t)blockIdx.x + (t > t_first ? 1 : 0);
+    const int64_t slot = 2 * (int64_t)blockIdx.x + (t > t_first ? 1 : 0);   // (the block's first item, or its last)
     for (int x = threadIdx.x; x < S::HEADS * (DP / 8); x += WARPS * 32) {
       const int h = x / (DP / 8), ch = (x % (DP / 8)) * 8;
       if (h >= it.heads || ch >= d) continue;
@@ -594,39 +679,39 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
         }
       }
     }
-    t += u1 - u0;
     __syncthreads();                                         // the rings are free again
   }
 }
 
 // ---- join of the parts -------------------------------------------------------------------------------------------------
-// An item that was split holds a boundary between two blocks; block (k, h) of this grid looks at the boundary between
-// blocks k and k + 1 and, when it is the first one inside its item, joins the item's parts for query head h of the chunk.
-template <typename T, typename C, int DP, int NT>
+// The parts of an item lie in the blocks from the one that has its first tokens, f, to the one that has its last; block
+// (k, h) of this grid looks at the boundary between blocks k and k + 1 and joins the parts of the item there, for query
+// head h of the chunk, when k is f.
+template <typename T, typename C, int DP, int NT, bool FAST>
 __global__ void __launch_bounds__(WARPS * 32) join_kernel(const AttentionParams p, int blocks) {
   using S = Shape<T, C, DP, NT>;
   __shared__ float sm_o[WARPS][DP];
   __shared__ float sm_m[WARPS], sm_l[WARPS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, h = blockIdx.y;
   const int copies = p.pages ? p.chunks : p.kv.heads * p.chunks;
-  const int64_t total_work = total_units<S::UNIT>(p, copies);
+  const int64_t total_work = total_units<FAST, S::UNIT>(p, copies);
   const int64_t per = units_per_block(total_work, blocks);
   const int64_t t = (int64_t)(blockIdx.x + 1) * per;
   if (t >= total_work) return;
-  const Place at = locate<S::UNIT>(p, copies, t);
-  const int64_t copy = (t - at.base) / at.units, first = at.base + copy * at.units;   // the item and its first unit
-  if (first == t || first < t - per) return;               // not split here, or another block of this grid joins it
+  const Place at = locate<FAST, S::UNIT>(p, copies, t);
+  const int64_t copy = (t - at.base) / (START + at.units), first = at.base + copy * (START + at.units);
+  if (first == t || first + START < t - per || first + START >= t) return;   // not split here, or another block joins it
   const Item it = item_of<S::HEADS>(p, at.entry, copy);
   if (h >= it.heads) return;
-  const int64_t last = (first + at.units - 1) / per;       // last block with a part
+  const int64_t last = (first + START + at.units - 1) / per;
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
   constexpr int E = DP / 32;                               // channels per lane
   float m = -INFINITY, l = 0.0f, o[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) o[i] = 0.0f;
   for (int64_t k = blockIdx.x + warp; k <= last; k += WARPS) {
-    // the item begins inside block blockIdx.x (slot 1, unless with its run) and at the start of the later blocks' runs
-    const int64_t slot = 2 * k + (k == blockIdx.x && first > k * per ? 1 : 0);
+    // slot 1 where the item begins behind the first unit of the block's run, slot 0 where it is there from the first on
+    const int64_t slot = 2 * k + (first > k * per ? 1 : 0);
     const float* ml = p.part_ml + (slot * S::HEADS + h) * 2;
     const float* row = p.part_o + (slot * S::HEADS + h) * DP;
     const float mk = ml[0], lk = ml[1];
@@ -671,11 +756,11 @@ __global__ void __launch_bounds__(WARPS * 32) join_kernel(const AttentionParams 
 // Blocks of the persistent grid (also the number of pairs of workspace slots).
 inline int grid_blocks(int dp, int esize, int nt) { return sm_count() * blocks_per_sm(dp, esize, nt); }
 
-template <typename T, typename C, int DP, int NT>
+template <typename T, typename C, int DP, int NT, bool FAST>
 static int launch(AttentionParams p, int64_t most_tokens, cudaStream_t stream) {
   using S = Shape<T, C, DP, NT>;
   constexpr int smem = WARPS * S::RING;
-  auto kern = attention_kernel<T, C, DP, NT>;
+  auto kern = attention_kernel<T, C, DP, NT, FAST>;
   static PerDevice opted;
   if (const int rc = opt_in_smem(opted, kern, smem)) return rc;
   const int64_t items = p.entries * (p.pages ? p.chunks : p.kv.heads * p.chunks);
@@ -700,15 +785,20 @@ static int launch(AttentionParams p, int64_t most_tokens, cudaStream_t stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return (int)cudaLaunchKernelEx(&cfg, join_kernel<T, C, DP, NT>, p, blocks);
+  return (int)cudaLaunchKernelEx(&cfg, join_kernel<T, C, DP, NT, FAST>, p, blocks);
+}
+
+template <typename T, typename C, int DP, int NT>
+static int by_page(const AttentionParams& p, int64_t most_tokens, cudaStream_t stream) {
+  return p.kv.page_size % 16 == 0 ? launch<T, C, DP, NT, true>(p, most_tokens, stream) : launch<T, C, DP, NT, false>(p, most_tokens, stream);
 }
 
 template <typename T, typename C>
 static int dispatch(const AttentionParams& p, int64_t most_tokens, cudaStream_t stream) {
   const int dp = pad_dim(p.kv.dim), nt = head_tiles(dp, p.group);
-  if (dp == 64) return nt == 1 ? launch<T, C, 64, 1>(p, most_tokens, stream) : launch<T, C, 64, 2>(p, most_tokens, stream);
-  if (dp == 128) return nt == 1 ? launch<T, C, 128, 1>(p, most_tokens, stream) : launch<T, C, 128, 2>(p, most_tokens, stream);
-  return launch<T, C, 256, 1>(p, most_tokens, stream);
+  if (dp == 64) return nt == 1 ? by_page<T, C, 64, 1>(p, most_tokens, stream) : by_page<T, C, 64, 2>(p, most_tokens, stream);
+  if (dp == 128) return nt == 1 ? by_page<T, C, 128, 1>(p, most_tokens, stream) : by_page<T, C, 128, 2>(p, most_tokens, stream);
+  return by_page<T, C, 256, 1>(p, most_tokens, stream);
 }
 
 }  // namespace kv
@@ -731,7 +821,7 @@ extern "C" int wush_kv_attention(const wush_kv_pages* kv, const wush_kv_table* t
   if (rc != 0) return rc;
   if (q_heads <= 0 || q_heads % kv->heads || window < 0) return WUSH_ERR_BAD_SHAPE;
   if ((pages == nullptr) != (counts == nullptr)) return WUSH_ERR_NULL_POINTER;
-  if (pages && (top <= 0 || (int64_t)top * kv->page_size > INT32_MAX)) return WUSH_ERR_BAD_SHAPE;
+  if (pages && (top <= 0 || (int64_t)top * kv->page_size > MAX_TOKENS)) return WUSH_ERR_BAD_SHAPE;
   if (pages && window != 0) return WUSH_ERR_BAD_FLAG;
   if (table->seqs == 0) return WUSH_OK;
   if ((rc = check_heads(q, 2)) != 0 || (rc = check_heads(out, 2)) != 0) return rc;

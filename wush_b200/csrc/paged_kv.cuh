@@ -13,6 +13,7 @@ namespace wush {
 namespace kv {
 
 constexpr int MAX_DIM = 256;
+constexpr int64_t MAX_TOKENS = INT32_MAX - (1 << 16);
 constexpr int STATUS_INDEX = 2;   // an index outside its table; a timeout (1) already in the word stays
 
 __device__ __forceinline__ void report_index(int* status) {
@@ -52,8 +53,8 @@ inline int check_pages(const wush_kv_pages* kv, const wush_kv_table* t, int type
     if (!aligned16(kv->bounds)) return WUSH_ERR_BAD_ALIGNMENT;
   }
   if (t->seqs < 0 || t->width <= 0 || t->stride < 0 || (t->seqs > 0 && !t->block_table)) return WUSH_ERR_BAD_SHAPE;
-  // positions and lengths are 32-bit
-  if (t->seqs > INT32_MAX || t->width > INT32_MAX || t->width * kv->page_size > INT32_MAX) return WUSH_ERR_TOO_LARGE;
+  // positions and lengths are 32-bit, and kernels look some tiles ahead
+  if (t->seqs > INT32_MAX || t->width > INT32_MAX || t->width * kv->page_size > MAX_TOKENS) return WUSH_ERR_TOO_LARGE;
   return WUSH_OK;
 }
 

@@ -30,6 +30,7 @@ from . import _lib
 
 TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float8_e4m3fn: 2}
 MAX_DIM = 256
+MAX_TOKENS = 2 ** 31 - 1 - 2 ** 16      # of a sequence
 
 
 def rope_table(max_positions: int, rotary_dim: int, base: float = 10000.0, device=None) -> torch.Tensor:
@@ -126,8 +127,8 @@ def _table(cache: PagedKVCache, block_table: torch.Tensor) -> "_lib.KVTable":
             or block_table.shape[1] < 1 or (block_table.stride(1) != 1 and block_table.shape[1] > 1):
         raise ValueError(f"block_table must be an int32 [sequences, pages] tensor on {cache.device} with unit column stride")
     seqs, width = block_table.shape
-    if width * cache.page_size > 2 ** 31 - 1:
-        raise ValueError("a block table can hold at most 2^31 - 1 tokens per sequence")
+    if width * cache.page_size > MAX_TOKENS:
+        raise ValueError(f"a block table can hold at most {MAX_TOKENS} tokens per sequence")
     return _lib.KVTable(block_table.data_ptr(), block_table.stride(0), seqs, width)
 
 
@@ -302,8 +303,8 @@ def paged_decode_attention(q: torch.Tensor, cache: PagedKVCache, block_table: to
     if pages is not None:
         if window:
             raise ValueError("a window and selected pages exclude each other")
-        if pages.dim() != 3 or pages.shape[2] < 1 or pages.shape[2] * cache.page_size > 2 ** 31 - 1:
-            raise ValueError("pages must be [sequences, n_kv_heads, top] and hold at most 2^31 - 1 tokens")
+        if pages.dim() != 3 or pages.shape[2] < 1 or pages.shape[2] * cache.page_size > MAX_TOKENS:
+            raise ValueError(f"pages must be [sequences, n_kv_heads, top] and hold at most {MAX_TOKENS} tokens")
         top = pages.shape[2]
         pages_ptr = _int32(pages, (table.seqs, cache.n_kv_heads, top), "pages", cache.device)
         counts_ptr = _int32(counts, (table.seqs, cache.n_kv_heads), "counts", cache.device)
