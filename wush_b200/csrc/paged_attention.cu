@@ -480,8 +480,9 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
           if constexpr (S::E8) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const uint32_t a0 = e4m3x2_to_f16x2(lo[i]), a1 = e4m3x2_to_f16x2(hi[i]), a2 = e4m3x2_to_f16x2(lo[i] >> 16),
-                             a3 = e4m3x2_to_f16x2(hi[i] >> 16);
+              uint32_t a0, a1, a2, a3;
+              e4m3x4_to_f16x4(lo[i], a0, a2);
+              e4m3x4_to_f16x4(hi[i], a1, a3);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) mma<M>(part[i % CHAINS][nt], a0, a1, a2, a3, qf[nt][j * 4 + i][0], qf[nt][j * 4 + i][1]);
             }
@@ -598,10 +599,8 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
             if constexpr (S::E8) {
               const uint32_t sel = i & 1 ? 0x7362 : 0x5140;  // bytes of tokens t, t + 1 side by side
               const uint32_t x = __byte_perm(w[0][i >> 1], w[1][i >> 1], sel), y = __byte_perm(w[2][i >> 1], w[3][i >> 1], sel);
-              a0 = e4m3x2_to_f16x2(x);
-              a1 = e4m3x2_to_f16x2(x >> 16);
-              a2 = e4m3x2_to_f16x2(y);
-              a3 = e4m3x2_to_f16x2(y >> 16);
+              e4m3x4_to_f16x4(x, a0, a1);
+              e4m3x4_to_f16x4(y, a2, a3);
             } else {
               a0 = __byte_perm(w[0][i], w[1][i], 0x5410);
               a1 = __byte_perm(w[0][i], w[1][i], 0x7632);

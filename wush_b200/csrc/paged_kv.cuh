@@ -89,6 +89,12 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two_bytes) {
   asm("{\n.reg .b16 t;\ncvt.u16.u32 t, %1;\ncvt.rn.f16x2.e4m3x2 %0, t;\n}\n" : "=r"(h) : "r"(two_bytes));
   return h;
 }
+// the same for all four bytes of a word
+__device__ __forceinline__ void e4m3x4_to_f16x4(uint32_t four_bytes, uint32_t& lo, uint32_t& hi) {
+  asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\ncvt.rn.f16x2.e4m3x2 %0, l;\ncvt.rn.f16x2.e4m3x2 %1, h;\n}\n"
+      : "=r"(lo), "=r"(hi)
+      : "r"(four_bytes));
+}
 __device__ __forceinline__ uint32_t pack2_e4m3(float lo, float hi) {
   uint16_t h;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(h) : "f"(hi), "f"(lo));
