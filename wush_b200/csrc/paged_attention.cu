@@ -7,10 +7,15 @@
 // Products.  All G queries of a key head are worked on together, with the tokens as the rows of m16n8k16 products:
 //     S^T [16 tokens x 8 heads] = K [16 tokens x 16 channels] . Q^T,     O^T [16 channels x 8 heads] += V^T . P^T.
 // A product does not care in which order its contracted index runs, nor which row is which channel, so a lane's fragment
-// of K is a 16-byte piece of a key row and its fragment of V neighbouring channels of four tokens.  Every lane copies its
-// own pieces into shared memory asynchronously, two tiles ahead, and reads back what it copied: the ring is an extension
-// of its registers, free of bank conflicts, barriers and swizzles, and the queries are loaded in the matching order.  P is
-// turned from the layout of an accumulator into that of an operand by movmatrix.  8-bit pages are widened to fp16 (exact).
+// of K is a 16-byte piece of a key row and its fragment of V neighbouring channels of four tokens, each one load from shared
+// memory, and the queries are loaded in the matching order.  P is turned from the layout of an accumulator into that of an
+// operand by movmatrix.  8-bit pages are widened to fp16 (exact).  (tcgen05.mma has at least 64 rows and 8 columns, wants P in
+// memory, and would be idle all the same: the tensor pipe is busy a seventh of the time.)
+//
+// Copies.  Every warp has a ring of three tiles in shared memory, filled two tiles ahead by bulk tensor copies (16 rows of one
+// head of a page are one box), so a warp needs one instruction for 2 KB and no registers for what is in flight.  Measured on
+// 64 ragged sequences of up to 4096 tokens (364 MB): fragments straight into registers 110 us, per-lane 16-byte copies 90 us,
+// boxes 70 us.
 //
 // Work.  The tokens of all (sequence, key head, chunk of queries) items are cut into units of 4 tiles (one per warp), the
 // units of all items are numbered through, and every block of a grid that fills the GPU exactly once takes an equal run
@@ -19,6 +24,7 @@
 #include <type_traits>
 
 #include "paged_kv.cuh"
+#include "sm100.cuh"
 
 namespace wush {
 namespace kv {
@@ -63,12 +69,15 @@ struct Shape {
   static constexpr int TT = tile_tokens(DP, (int)sizeof(C));
   static constexpr int MT = TT / 16;
   static constexpr int KJ = DP * (int)sizeof(C) / 64;       // 16-byte pieces of a key row per lane
-  static constexpr int VC = E8 && DP >= 128 ? 16 : 8;       // channels of a piece of a value row
+  static constexpr int VC = E8 && DP >= 128 ? 16 : 8;       // channels of a lane's piece of a value row
   static constexpr int VB = VC * (int)sizeof(C);            // its bytes: 16, or 8 for short rows of 8-bit values
   static constexpr int VJ = DP / (8 * VC);                  // pieces per lane
   static constexpr int VI = VC / 2;                         // products of 16 channels they make
-  static constexpr int K_BYTES = MT * 2 * KJ * 512, V_BYTES = MT * 4 * VJ * 32 * VB;   // of a tile
-  static constexpr int STAGE = K_BYTES + V_BYTES;
+  // A tile in shared memory: for every 16 tokens the keys, then for every 16 tokens the values; 16 rows of at most 128
+  // bytes make a box, the boxes of longer rows follow each other, and the 16-byte pieces of a box are swizzled
+  static constexpr int PITCH_B = DP * (int)sizeof(C) < 128 ? DP * (int)sizeof(C) : 128;
+  static constexpr int BOXES = DP * (int)sizeof(C) / PITCH_B, BOX = 16 * PITCH_B, GROUP = BOXES * BOX;
+  static constexpr int STAGE = 2 * MT * GROUP;
   static constexpr int HEADS = NT * 8;
   static constexpr int UNIT = WARPS * TT;                   // tokens of a unit
   static constexpr int STAGES = 3;                          // tiles of a warp in shared memory or on the way there
@@ -80,23 +89,36 @@ struct Shape {
   static constexpr float BIAS = std::is_same<M, __half>::value ? 7.0f : 0.0f;
   static constexpr int BLOCKS = blocks_per_sm(DP, (int)sizeof(C), NT);
   static constexpr int PITCH = DP + 4;                      // floats of a head's row in shared memory
-  static constexpr int RING = STAGES * STAGE > HEADS * PITCH * 4 ? STAGES * STAGE : HEADS * PITCH * 4;   // bytes of a warp
+  static constexpr int RING = STAGES * STAGE;               // bytes of a warp
+  static_assert(RING >= HEADS * PITCH * 4, "the ring also holds a warp's part of the result");
 };
 
 __host__ __device__ inline int pad_dim(int d) { return d <= 64 ? 64 : (d <= 128 ? 128 : 256); }
 __host__ __device__ inline int head_tiles(int dp, int group) { return dp == 256 || group <= 8 ? 1 : 2; }
 
 // ---- instructions ------------------------------------------------------------------------------------------------------
-// asynchronous copy of a lane's piece into shared memory; zeros when !ok
+// asynchronous copy of a 16-byte piece into shared memory; zeros when !ok
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool ok) {
   asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copy8(uint32_t dst, const void* src, bool ok) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(dst), "l"(src), "r"(ok ? 8 : 0) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
+
+// box of 16 rows of one head of one page
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int row, int head, int page, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n" ::"r"(dst),
+      "l"(map), "r"(x), "r"(row), "r"(head), "r"(page), "r"(bar)
+      : "memory");
+}
+
+// place of a byte of a box: the swizzle exchanges the 16-byte pieces of a line of 128 bytes (64 where rows are that short)
+// by the line's number
+template <int PITCH_B>
+__device__ __forceinline__ constexpr int swizzled(int at) {
+  return at ^ ((at >> 3) & (PITCH_B == 128 ? 0x70 : 0x30));
+}
 
 template <typename M>
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -211,25 +233,46 @@ __device__ __forceinline__ Item item_of(const AttentionParams& p, int64_t entry,
 }
 
 // ---- the kernel --------------------------------------------------------------------------------------------------------
-// FAST: page_size is a multiple of 16, so that 16 consecutive tokens lie in one page and are looked up together.
+// FAST: page_size is a multiple of 16, so that 16 consecutive tokens lie in one page: their rows come as boxes of a tensor
+// map.  Otherwise the lanes copy them piece by piece, row by row.
 template <typename T, typename C, int DP, int NT, bool FAST>
-__global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) attention_kernel(const AttentionParams p) {
+__global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS)
+    attention_kernel(const AttentionParams p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
   using S = Shape<T, C, DP, NT>;
   using M = typename S::M;
   constexpr int MT = S::MT, KJ = S::KJ, VJ = S::VJ, VI = S::VI, TT = S::TT, CB = (int)sizeof(C);
   constexpr unsigned FULL = TT == 32 ? 0xffffffffu : 0xffffu;
   // every warp's ring of tiles; between walks it holds the warp's part of the result, [HEADS][PITCH] floats
-  extern __shared__ __align__(16) uint8_t smem[];
+  extern __shared__ uint8_t smem_raw[];
   __shared__ float sm_m[WARPS * S::HEADS], sm_l[WARPS * S::HEADS];
+  __shared__ __align__(8) uint64_t sm_bar[WARPS][S::STAGES];
+  __shared__ uint32_t sm_abort;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int r = lane >> 2, c = lane & 3;
+  uint8_t* smem = smem_raw + ((1024 - (sm100::smem_u32(smem_raw) & 1023)) & 1023);
   uint8_t* ring = smem + warp * S::RING;
-  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
+  const uint32_t ring_at = sm100::smem_u32(ring), bar_at = sm100::smem_u32(sm_bar[warp]);
   const int d = p.kv.dim, page_size = p.kv.page_size;
   const int copies = p.pages ? p.chunks : p.kv.heads * p.chunks;
-  const int64_t k_row = p.kv.k_row * CB, v_row = p.kv.v_row * CB;         // bytes
 
+  if (FAST) {
+    if (threadIdx.x == 0) sm_abort = 0;
+    if (lane == 0) {
+      for (int i = 0; i < S::STAGES; ++i) sm100::mbar_init(bar_at + 8 * i, 1);
+      sm100::mbar_init_fence();
+    }
+    __syncthreads();
+  }
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+
+  // Row r of a product is token token_row(r) of its 16 and lane 4 r + c reads piece piece_of(r) of a value row: with these
+  // orders no two lanes that read together meet in a bank.
+  const int token_row = (r >> 1) | (r & 1) << 2;                       // and token_row + 8; operand tokens c, c + 4, c + 8, c + 12
+  const int piece = S::PITCH_B == 128 ? token_row : r;
+  // byte offsets in a group of 16 tokens; 8 rows and a box further they repeat (short rows: computed apart)
+  const int k_lo = swizzled<S::PITCH_B>(token_row * S::PITCH_B + c * 16), k_hi = swizzled<S::PITCH_B>((token_row + 8) * S::PITCH_B + c * 16);
+  const int v_0 = swizzled<S::PITCH_B>(c * S::PITCH_B + piece * S::VB), v_4 = swizzled<S::PITCH_B>((c + 4) * S::PITCH_B + piece * S::VB);
+  const int v_8 = swizzled<S::PITCH_B>((c + 8) * S::PITCH_B + piece * S::VB), v_12 = swizzled<S::PITCH_B>((c + 12) * S::PITCH_B + piece * S::VB);
 
   int64_t t, t_end, t_first;
   Place at;
@@ -247,6 +290,8 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
     at = locate<FAST, S::UNIT>(p, copies, t);
   }
 
+  int stage = 0;                                             // of the ring, for the tile that is worked on next
+  uint32_t parity = 0;
   for (int64_t t_next; t < t_end; t = t_next) {
     if (t >= at.base + (START + at.units) * copies) {        // the next entry
       at.base += (START + at.units) * copies;
@@ -263,8 +308,6 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
     const int s1 = (int)min((int64_t)w.tokens, u1 * S::UNIT);
 
     // -- where the tokens are --------------------------------------------------------------------------------------------
-    const uint8_t* k_head = reinterpret_cast<const uint8_t*>(p.kv.k) + it.hk * p.kv.k_head * CB;
-    const uint8_t* v_head = reinterpret_cast<const uint8_t*>(p.kv.v) + it.hk * p.kv.v_head * CB;
     const int32_t* list = p.pages ? p.pages + at.entry * p.top : nullptr;
     const int32_t* table = p.table.block_table + it.b * p.table.stride;
     constexpr int STEP = S::UNIT;
@@ -283,14 +326,14 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
       return {lp, row, lp * page_size + row};
     };
     auto physical = [&](Row x) -> Row { return {x.page >= 0 && x.pos < w.len ? table[x.page] : -2, x.row, x.pos}; };
-    // byte offsets of the rows, and the tokens that count: one, or with FAST the 16 from there
-    int64_t k_at = 0, v_at = 0;
+    // the current page (0 where there is none) and row, and the tokens that count: one, or with FAST the 16 from there
+    int page = 0, page_row = 0;
     unsigned counts16 = 0;
     auto resolve = [&](Row x) {
       const bool ok = x.page >= 0 && x.page < p.kv.num_pages;
       if (!ok && x.page != -2) report_index(p.status);
-      k_at = ok ? (x.page * p.kv.k_page + x.row * p.kv.k_row) * CB : 0;
-      v_at = ok ? (x.page * p.kv.v_page + x.row * p.kv.v_row) * CB : 0;
+      page = ok ? x.page : 0;
+      page_row = ok ? x.row : 0;
       const int lo = max(0, w.begin - x.pos), hi = min(16, w.len - x.pos);
       counts16 = !ok ? 0 : (FAST ? (0xffffu >> (16 - hi)) & (0xffffu << lo) : 1);
     };
@@ -305,90 +348,59 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
       after = logical(token_of(i + 2 * hold + held));
     };
 
-    // the copies of tile i into a stage of the ring, piece by piece [piece][lane]; returns the tokens that count
-    auto fetch = [&](int i, int stage) -> unsigned {
-      uint32_t dst = ring_at + stage * S::STAGE;
-      const uint32_t dst_v = dst + S::K_BYTES - (S::VB == 8 ? lane * 8 : 0);
+    // the copies of tile i into stage `to` of the ring; returns the tokens that count
+    auto fetch = [&](int i, int to) -> unsigned {
+      const uint32_t dst = ring_at + to * S::STAGE;
+      unsigned mask = 0;
       if constexpr (FAST) {
+        // the lanes that hold the tile's groups start their copies, whole boxes: rows that do not count are masked later
         if (i * MT % 32 == 0) advance(i * MT);
-        unsigned mask = 0;
+        const uint32_t bar = bar_at + 8 * to;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
           const int from = (i * MT + mt) & 31;
-          const unsigned counts = __shfl_sync(0xffffffffu, counts16, from);
-          mask |= counts << (16 * mt);
-          const uint8_t* kp = k_head + __shfl_sync(0xffffffffu, k_at, from) + r * k_row;
-          const uint8_t* vp = v_head + __shfl_sync(0xffffffffu, v_at, from) + 2 * c * v_row;
-          const uint32_t dk = dst + mt * (2 * KJ * 512), dv = dst_v + mt * (4 * VJ * 32 * S::VB);
-          const bool whole = counts == 0xffffu && d == DP;
+          if (lane == from) {
+            if (mt == 0) sm100::mbar_arrive_expect_tx(bar, S::STAGE);
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint8_t* row = kp + half * 8 * k_row;
-            if (whole) {
-#pragma unroll
-              for (int j = 0; j < KJ; ++j) copy16(dk + (half * KJ + j) * 512, row + c * 16 + j * 64, true);
-            } else {
-#pragma unroll
-              for (int j = 0; j < KJ; ++j) {
-                const bool in = (j * 4 + c) * 16 < d * CB;
-                copy16(dk + (half * KJ + j) * 512, row + (in ? (j * 4 + c) * 16 : 0), in && (counts >> (half * 8 + r) & 1));
-              }
+            for (int x = 0; x < S::BOXES; ++x) {
+              tma_load_4d(dst + mt * S::GROUP + x * S::BOX, &k_map, x * (S::PITCH_B / CB), page_row, it.hk, page, bar);
+              tma_load_4d(dst + (MT + mt) * S::GROUP + x * S::BOX, &v_map, x * (S::PITCH_B / CB), page_row, it.hk, page, bar);
             }
           }
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const uint8_t* row = vp + ((x & 1) + (x >> 1) * 8) * v_row;
-#pragma unroll
-            for (int j = 0; j < VJ; ++j) {
-              const bool in = whole || (j * 8 + r) * S::VC < d;
-              const bool ok = whole || (in && (counts >> (2 * c + (x & 1) + (x >> 1) * 8) & 1));
-              const uint8_t* src = row + (in ? (j * 8 + r) * S::VB : 0);
-              if constexpr (S::VB == 8) copy8(dv + (x * VJ + j) * 256, src, ok);
-              else copy16(dv + (x * VJ + j) * 512, src, ok);
-            }
-          }
+          mask |= __shfl_sync(0xffffffffu, counts16, from) << (16 * mt);
         }
-        return mask;
       } else {
         advance(i * TT);
-        const unsigned mask = __ballot_sync(0xffffffffu, counts16 != 0);
+        mask = __ballot_sync(0xffffffffu, counts16 != 0) & FULL;
+        const int64_t k_at = (page * p.kv.k_page + page_row * p.kv.k_row + it.hk * p.kv.k_head) * CB;
+        const int64_t v_at = (page * p.kv.v_page + page_row * p.kv.v_row + it.hk * p.kv.v_head) * CB;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            const int tok = mt * 16 + half * 8 + r;
-            const uint8_t* row = k_head + __shfl_sync(0xffffffffu, k_at, tok);
+            const int row = half * 8 + r, tok = mt * 16 + row;
+            const uint8_t* k = reinterpret_cast<const uint8_t*>(p.kv.k) + __shfl_sync(0xffffffffu, k_at, tok);
+            const uint8_t* v = reinterpret_cast<const uint8_t*>(p.kv.v) + __shfl_sync(0xffffffffu, v_at, tok);
 #pragma unroll
             for (int j = 0; j < KJ; ++j) {
-              const bool in = (j * 4 + c) * 16 < d * CB;
-              copy16(dst + ((mt * 2 + half) * KJ + j) * 512, row + (in ? (j * 4 + c) * 16 : 0), in && (mask >> tok & 1));
+              const int x = (j * 4 + c) * 16;
+              const bool in = x < d * CB, ok = in && (mask >> tok & 1);
+              const uint32_t to_box = dst + mt * S::GROUP + x / S::PITCH_B * S::BOX + swizzled<S::PITCH_B>(row * S::PITCH_B + x % S::PITCH_B);
+              copy16(to_box, k + (in ? x : 0), ok);
+              copy16(to_box + MT * S::GROUP, v + (in ? x : 0), ok);
             }
           }
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int tok = mt * 16 + 2 * c + (x & 1) + (x >> 1) * 8;
-            const uint8_t* row = v_head + __shfl_sync(0xffffffffu, v_at, tok);
-#pragma unroll
-            for (int j = 0; j < VJ; ++j) {
-              const bool in = (j * 8 + r) * S::VC < d;
-              const uint8_t* src = row + (in ? (j * 8 + r) * S::VB : 0);
-              if constexpr (S::VB == 8) copy8(dst_v + ((mt * 4 + x) * VJ + j) * 256, src, in && (mask >> tok & 1));
-              else copy16(dst_v + ((mt * 4 + x) * VJ + j) * 512, src, in && (mask >> tok & 1));
-            }
-          }
-        }
-        return mask & FULL;
       }
+      return mask;
     };
 
-    // Tiles are fetched STAGES - 1 ahead of the one worked on.  A lane waits for and reads only what it copied itself, so
-    // the ring needs no barriers.
+    // Tiles are fetched STAGES - 1 ahead of the one worked on; every warp has its own ring and barriers.
     unsigned seen[S::STAGES];                                // tokens that count of the tiles in the ring, oldest first
 #pragma unroll
     for (int i = 0; i < S::STAGES - 1; ++i) {
       seen[i] = 0;
-      if (first + i * STEP < s1) seen[i] = fetch(i, i);
-      copy_commit();
+      if (first + i * STEP < s1) seen[i] = fetch(i, (stage + i) % S::STAGES);
+      if (!FAST) copy_commit();
     }
 
     // -- queries, in the order of the key fragments ----------------------------------------------------------------------
@@ -454,13 +466,25 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
 #pragma unroll
         for (int i = 0; i < VI; ++i) o[nt][j][i][0] = o[nt][j][i][1] = o[nt][j][i][2] = o[nt][j][i][3] = 0.0f;
     }
-    int stage = 0, ahead = S::STAGES - 1;
+    int ahead = S::STAGES - 1;
+    bool gave_up = false;
     for (int base = first; base < s1; base += STEP, ++ahead) {
+      __syncwarp();                                          // the stage that is fetched into has been read by every lane
       seen[S::STAGES - 1] = 0;
       if (base + (S::STAGES - 1) * STEP < s1) seen[S::STAGES - 1] = fetch(ahead, stage == 0 ? S::STAGES - 1 : stage - 1);
-      copy_commit();
-      copy_wait<S::STAGES - 1>();
-      const uint8_t* tile = ring + stage * S::STAGE + lane * 16;
+      if (FAST) {
+        const bool came = sm100::mbar_wait(bar_at + 8 * stage, parity >> stage & 1, &sm_abort);
+        if (!__all_sync(0xffffffffu, came)) {
+          gave_up = true;
+          break;
+        }
+        parity ^= 1u << stage;
+      } else {
+        copy_commit();
+        copy_wait<S::STAGES - 1>();
+        __syncwarp();
+      }
+      const uint8_t* tile = ring + stage * S::STAGE;
       stage = stage + 1 == S::STAGES ? 0 : stage + 1;
       // logits; two sums where a single chain of products would be waited for
       constexpr int CHAINS = MT * NT == 1 ? 2 : 1;
@@ -474,8 +498,10 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
           for (int nt = 0; nt < NT; ++nt) part[x][nt][0] = part[x][nt][1] = part[x][nt][2] = part[x][nt][3] = 0.0f;
 #pragma unroll
         for (int j = 0; j < KJ; ++j) {
-          const uint4 k0 = *reinterpret_cast<const uint4*>(tile + ((mt * 2 + 0) * KJ + j) * 512);
-          const uint4 k1 = *reinterpret_cast<const uint4*>(tile + ((mt * 2 + 1) * KJ + j) * 512);
+          // piece 4 j + c of the rows; pieces 4 to 7 of a line lie in its other half
+          const uint8_t* at_k = tile + mt * S::GROUP + (j >> 1) * S::BOX;
+          const uint4 k0 = *reinterpret_cast<const uint4*>(at_k + (k_lo ^ (j & 1) << 6));
+          const uint4 k1 = *reinterpret_cast<const uint4*>(at_k + (k_hi ^ (j & 1) << 6));
           const uint32_t lo[4] = {k0.x, k0.y, k0.z, k0.w}, hi[4] = {k1.x, k1.y, k1.z, k1.w};
           if constexpr (S::E8) {
 #pragma unroll
@@ -516,7 +542,7 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
           for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int x = 0; x < 4; ++x)
-              if (!(seen[0] >> (mt * 16 + (x >> 1) * 8 + r) & 1)) s[mt][nt][x] = -INFINITY;
+              if (!(seen[0] >> (mt * 16 + (x >> 1) * 8 + token_row) & 1)) s[mt][nt][x] = -INFINITY;
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -551,7 +577,7 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
               }
           }
       }
-      uint32_t ph[MT][NT][2], pl[MT][NT][2];                 // weights as operands: tokens 2c, 2c + 1 (+8) of head r
+      uint32_t ph[MT][NT][2], pl[MT][NT][2];                 // weights as operands: tokens c, c + 4 (+8) of head r
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const float base0 = (m[nt][0] == -INFINITY ? 0.0f : m[nt][0]) - S::BIAS;
@@ -577,12 +603,12 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int j = 0; j < VJ; ++j) {
-          uint32_t w[4][4];                                  // the pieces of tokens 2c, 2c + 1, 2c + 8, 2c + 9
+          uint32_t w[4][4];                                  // the pieces of tokens c, c + 4, c + 8, c + 12
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            const uint8_t* at_v = tile + S::K_BYTES + ((mt * 4 + x) * VJ + j) * (32 * S::VB);
+            const uint8_t* at_v = tile + (MT + mt) * S::GROUP + j * S::BOX + (x == 0 ? v_0 : (x == 1 ? v_4 : (x == 2 ? v_8 : v_12)));
             if constexpr (S::VB == 8) {
-              const uint2 v = *reinterpret_cast<const uint2*>(at_v - lane * 8);
+              const uint2 v = *reinterpret_cast<const uint2*>(at_v);
               w[x][0] = v.x;
               w[x][1] = v.y;
             } else {
@@ -592,12 +618,14 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
               w[x][2] = v.z;
               w[x][3] = v.w;
             }
+            // values of tokens that do not count must not meet their zero weights as NaN
+            if (FAST && seen[0] != FULL && !(seen[0] >> (mt * 16 + c + 4 * x) & 1)) w[x][0] = w[x][1] = w[x][2] = w[x][3] = 0;
           }
 #pragma unroll
           for (int i = 0; i < VI; ++i) {
             uint32_t a0, a1, a2, a3;                         // channels 2i and 2i + 1 of the lane's piece
             if constexpr (S::E8) {
-              const uint32_t sel = i & 1 ? 0x7362 : 0x5140;  // bytes of tokens t, t + 1 side by side
+              const uint32_t sel = i & 1 ? 0x7362 : 0x5140;  // bytes of two tokens side by side
               const uint32_t x = __byte_perm(w[0][i >> 1], w[1][i >> 1], sel), y = __byte_perm(w[2][i >> 1], w[3][i >> 1], sel);
               e4m3x4_to_f16x4(x, a0, a1);
               e4m3x4_to_f16x4(y, a2, a3);
@@ -619,7 +647,12 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
     }
 
     // -- join the warps --------------------------------------------------------------------------------------------------
-    copy_wait<0>();
+    if (!FAST) copy_wait<0>();
+    if (FAST && gave_up) {                                   // the copies in flight have to land before the block ends
+      for (int i = 0; i < S::STAGES; ++i)
+        for (int k = 0; k < (1 << 16) && !sm100::mbar_try_wait(bar_at + 8 * i, parity >> i & 1); ++k) __nanosleep(64);
+    }
+    __syncwarp();                                            // the ring has been read by every lane
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -633,7 +666,7 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
           sm_m[warp * S::HEADS + h] = m[nt][e];
           sm_l[warp * S::HEADS + h] = x;
         }
-        float* row = reinterpret_cast<float*>(ring) + h * S::PITCH + r * S::VC;
+        float* row = reinterpret_cast<float*>(ring) + h * S::PITCH + piece * S::VC;
 #pragma unroll
         for (int j = 0; j < VJ; ++j)
 #pragma unroll
@@ -678,7 +711,12 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS) atten
         }
       }
     }
+    if (FAST) asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");   // ... and before copies into it by the other proxy
     __syncthreads();                                         // the rings are free again
+    if (FAST && sm_abort) {                                  // a copy never came: what was written is invalid
+      if (threadIdx.x == 0 && p.status) atomicExch(p.status, 1);
+      return;
+    }
   }
 }
 
@@ -756,9 +794,9 @@ __global__ void __launch_bounds__(WARPS * 32) join_kernel(const AttentionParams 
 inline int grid_blocks(int dp, int esize, int nt) { return sm_count() * blocks_per_sm(dp, esize, nt); }
 
 template <typename T, typename C, int DP, int NT, bool FAST>
-static int launch(AttentionParams p, int64_t most_tokens, cudaStream_t stream) {
+static int launch(AttentionParams p, const CUtensorMap& k_map, const CUtensorMap& v_map, int64_t most_tokens, cudaStream_t stream) {
   using S = Shape<T, C, DP, NT>;
-  constexpr int smem = WARPS * S::RING;
+  constexpr int smem = WARPS * S::RING + 1024;
   auto kern = attention_kernel<T, C, DP, NT, FAST>;
   static PerDevice opted;
   if (const int rc = opt_in_smem(opted, kern, smem)) return rc;
@@ -766,12 +804,12 @@ static int launch(AttentionParams p, int64_t most_tokens, cudaStream_t stream) {
   const int64_t most_units = (most_tokens + S::UNIT - 1) / S::UNIT;
   p.whole = most_units <= WHOLE_UNITS;
   if (p.whole) {
-    kern<<<(unsigned)items, WARPS * 32, smem, stream>>>(p);
+    kern<<<(unsigned)items, WARPS * 32, smem, stream>>>(p, k_map, v_map);
     return (int)cudaGetLastError();
   }
   const int64_t most_blocks = (items * most_units + MIN_UNITS - 1) / MIN_UNITS;
   const int blocks = (int)min((int64_t)grid_blocks(DP, (int)sizeof(C), NT), most_blocks);
-  kern<<<blocks, WARPS * 32, smem, stream>>>(p);
+  kern<<<blocks, WARPS * 32, smem, stream>>>(p, k_map, v_map);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || blocks == 1) return (int)e;
   // the join may start while the last blocks still run: it finds its item, then waits for them
@@ -787,9 +825,31 @@ static int launch(AttentionParams p, int64_t most_tokens, cudaStream_t stream) {
   return (int)cudaLaunchKernelEx(&cfg, join_kernel<T, C, DP, NT, FAST>, p, blocks);
 }
 
+// Tensor map over a pool: boxes of 16 rows of at most 128 bytes of one head of one page.  (Lines are promoted to 128 bytes in
+// the L2 and not to 256: 8-bit rows of 128 bytes with other heads' rows between them then took 70 us instead of 61.)
+inline bool make_pool_map(CUtensorMap* map, const wush_kv_pages& kv, void* base, int64_t page, int64_t row, int64_t head, int box) {
+  EncodeTiledFn encode = tensor_map_encoder();
+  if (!encode) return false;
+  const cuuint64_t e = element_bytes(kv.type);
+  const cuuint64_t dims[4] = {(cuuint64_t)kv.dim, (cuuint64_t)kv.page_size, (cuuint64_t)kv.heads, (cuuint64_t)kv.num_pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)row * e, (cuuint64_t)head * e, (cuuint64_t)page * e};
+  const cuuint32_t boxes[4] = {(cuuint32_t)(box / e), 16, 1, 1}, steps[4] = {1, 1, 1, 1};
+  const CUtensorMapSwizzle swizzle = box == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+  return encode(map, e == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, strides, boxes, steps,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Boxes where pages are made of whole groups of 16 tokens and the strides can be described (a stride of 0 cannot), rows
+// piece by piece otherwise.
 template <typename T, typename C, int DP, int NT>
 static int by_page(const AttentionParams& p, int64_t most_tokens, cudaStream_t stream) {
-  return p.kv.page_size % 16 == 0 ? launch<T, C, DP, NT, true>(p, most_tokens, stream) : launch<T, C, DP, NT, false>(p, most_tokens, stream);
+  CUtensorMap k_map{}, v_map{};
+  constexpr int box = Shape<T, C, DP, NT>::PITCH_B;
+  if (p.kv.page_size % 16 == 0 && make_pool_map(&k_map, p.kv, p.kv.k, p.kv.k_page, p.kv.k_row, p.kv.k_head, box) &&
+      make_pool_map(&v_map, p.kv, p.kv.v, p.kv.v_page, p.kv.v_row, p.kv.v_head, box))
+    return launch<T, C, DP, NT, true>(p, k_map, v_map, most_tokens, stream);
+  return launch<T, C, DP, NT, false>(p, k_map, v_map, most_tokens, stream);
 }
 
 template <typename T, typename C>
