@@ -44,6 +44,7 @@ struct AttentionParams {
   const int32_t* counts;
   float* part_o;                        // [slots][heads of a chunk][DP]
   float* part_ml;                       // [slots][heads of a chunk][2]
+  int4* splits;                         // [blocks][2]: the item that goes on in the next block
   int* status;
   float scale;
   int64_t window;
@@ -286,6 +287,7 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS)
     const int64_t per = units_per_block(total, gridDim.x);
     t = t_first = (int64_t)blockIdx.x * per;
     t_end = min(total, t + per);
+    if (threadIdx.x == 0) p.splits[2 * blockIdx.x].w = 0;
     if (t >= t_end) return;
     at = locate<FAST, S::UNIT>(p, copies, t);
   }
@@ -676,7 +678,14 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS)
       }
     __syncthreads();
     const bool all = u0 == 0 && u1 == at.units;
-    const int64_t slot = 2 * (int64_t)blockIdx.x + (t > t_first ? 1 : 0);   // (the block's first item, or its last)
+    // Parts go to slot 0 (the block's first item) or 1 (its last).  The block with an item's first tokens leaves a note for
+    // the join: sequence, first query head, key head, number of heads; number of parts and slot of the first one.
+    const int64_t slot = 2 * (int64_t)blockIdx.x + (t > t_first ? 1 : 0);
+    if (!all && u0 == 0 && threadIdx.x == 0) {
+      const int64_t rest = at.units - u1, per = t_end - t_first;
+      p.splits[2 * blockIdx.x] = make_int4((int)it.b, it.first_head, it.hk, it.heads);
+      p.splits[2 * blockIdx.x + 1] = make_int4((int)(1 + (rest + per - 1) / per), (int)(slot & 1), 0, 0);
+    }
     for (int x = threadIdx.x; x < S::HEADS * (DP / 8); x += WARPS * 32) {
       const int h = x / (DP / 8), ch = (x % (DP / 8)) * 8;
       if (h >= it.heads || ch >= d) continue;
@@ -721,73 +730,72 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS)
 }
 
 // ---- join of the parts -------------------------------------------------------------------------------------------------
-// The parts of an item lie in the blocks from the one that has its first tokens, f, to the one that has its last; block
-// (k, h) of this grid looks at the boundary between blocks k and k + 1 and joins the parts of the item there, for query
-// head h of the chunk, when k is f.
-template <typename T, typename C, int DP, int NT, bool FAST>
-__global__ void __launch_bounds__(WARPS * 32) join_kernel(const AttentionParams p, int blocks) {
+// Block (k, h) joins the parts of the item that block k of the attention left unfinished, for query head h of its chunk: the
+// first part is block k's, the others are in slot 0 of the blocks after it.  32 parts at a time, eight a warp, all loaded
+// before the first is used: the kernel is a chain of latencies (note, parts, result).
+constexpr int JOIN_WARPS = 4, JOIN_ROWS = 32 / JOIN_WARPS;
+template <typename T, typename C, int DP, int NT>
+__global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const AttentionParams p) {
   using S = Shape<T, C, DP, NT>;
-  __shared__ float sm_o[WARPS][DP];
-  __shared__ float sm_m[WARPS], sm_l[WARPS];
+  constexpr int E = DP / 64;                                 // pairs of channels of a lane
+  __shared__ float2 sm_o[JOIN_WARPS][DP / 2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, h = blockIdx.y;
-  const int copies = p.pages ? p.chunks : p.kv.heads * p.chunks;
-  const int64_t total_work = total_units<FAST, S::UNIT>(p, copies);
-  const int64_t per = units_per_block(total_work, blocks);
-  const int64_t t = (int64_t)(blockIdx.x + 1) * per;
-  if (t >= total_work) return;
-  const Place at = locate<FAST, S::UNIT>(p, copies, t);
-  const int64_t copy = (t - at.base) / (START + at.units), first = at.base + copy * (START + at.units);
-  if (first == t || first + START < t - per || first + START >= t) return;   // not split here, or another block joins it
-  const Item it = item_of<S::HEADS>(p, at.entry, copy);
-  if (h >= it.heads) return;
-  const int64_t last = (first + START + at.units - 1) / per;
-  asm volatile("griddepcontrol.wait;\n" ::: "memory");
-  constexpr int E = DP / 32;                               // channels per lane
-  float m = -INFINITY, l = 0.0f, o[E];
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");      // (every block: none may end before the parts are there)
+  const int4 item = p.splits[2 * blockIdx.x], more = p.splits[2 * blockIdx.x + 1];
+  if (h >= item.w) return;
+  const int parts = more.x;
+  auto slot_of = [&](int i) { return (2 * ((int64_t)blockIdx.x + i) + (i == 0 ? more.y : 0)) * S::HEADS + h; };
+  float top = -INFINITY, total = 0.0f;
+  float2 o[E];
 #pragma unroll
-  for (int i = 0; i < E; ++i) o[i] = 0.0f;
-  for (int64_t k = blockIdx.x + warp; k <= last; k += WARPS) {
-    // slot 1 where the item begins behind the first unit of the block's run, slot 0 where it is there from the first on
-    const int64_t slot = 2 * k + (first > k * per ? 1 : 0);
-    const float* ml = p.part_ml + (slot * S::HEADS + h) * 2;
-    const float* row = p.part_o + (slot * S::HEADS + h) * DP;
-    const float mk = ml[0], lk = ml[1];
-    const float top = fmaxf(m, mk);
-    const float keep = m == top ? 1.0f : exp2_fast(m - top), add = mk == top ? 1.0f : exp2_fast(mk - top);
-    m = top;
-    l = l * keep + lk * add;
+  for (int i = 0; i < E; ++i) o[i] = make_float2(0.0f, 0.0f);
+  for (int base = 0; base < parts; base += 32) {
+    float2 row[JOIN_ROWS][E];
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const int ch = i * 32 + lane;
-      o[i] = o[i] * keep + (ch < p.kv.dim ? row[ch] : 0.0f) * add;
+    for (int x = 0; x < JOIN_ROWS; ++x) {
+      const int i = base + warp + x * JOIN_WARPS;
+      const float2* from = reinterpret_cast<const float2*>(p.part_o + slot_of(min(i, parts - 1)) * DP) + lane;
+#pragma unroll
+      for (int j = 0; j < E; ++j) row[x][j] = from[j * 32];
+    }
+    const bool mine = base + lane < parts;
+    const float2 ml = mine ? *reinterpret_cast<const float2*>(p.part_ml + slot_of(base + lane) * 2) : make_float2(-INFINITY, 0.0f);
+    float now = ml.x;
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, x));
+    now = fmaxf(now, top);
+    const float keep = top == now ? 1.0f : exp2_fast(top - now);
+    const float weight = !mine ? 0.0f : (ml.x == now ? 1.0f : exp2_fast(ml.x - now));
+    top = now;
+    float sum = mine ? ml.y * weight : 0.0f;
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    total = fmaf(total, keep, sum);
+#pragma unroll
+    for (int j = 0; j < E; ++j) o[j] = make_float2(o[j].x * keep, o[j].y * keep);
+#pragma unroll
+    for (int x = 0; x < JOIN_ROWS; ++x) {
+      const int i = warp + x * JOIN_WARPS;
+      const float w = __shfl_sync(0xffffffffu, weight, i);
+      if (base + i < parts) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) o[j] = make_float2(fmaf(row[x][j].x, w, o[j].x), fmaf(row[x][j].y, w, o[j].y));
+      }
     }
   }
-  if (lane == 0) {
-    sm_m[warp] = m;
-    sm_l[warp] = l;
-  }
 #pragma unroll
-  for (int i = 0; i < E; ++i) sm_o[warp][i * 32 + lane] = o[i];
+  for (int j = 0; j < E; ++j) sm_o[warp][j * 32 + lane] = o[j];
   __syncthreads();
-  float top = sm_m[0], total = 0.0f, part[WARPS];
+  const float scale = (S::E8 ? p.kv.v_scale[item.z] : 1.0f) / (total == 0.0f ? 1.0f : total);
+  for (int ch = threadIdx.x * 2; ch < p.kv.dim; ch += JOIN_WARPS * 64) {
+    float2 y = make_float2(0.0f, 0.0f);
 #pragma unroll
-  for (int w = 1; w < WARPS; ++w) top = fmaxf(top, sm_m[w]);
-#pragma unroll
-  for (int w = 0; w < WARPS; ++w) {
-    part[w] = sm_m[w] == top ? 1.0f : exp2_fast(sm_m[w] - top);
-    total = fmaf(sm_l[w], part[w], total);
-  }
-  const float scale = (S::E8 ? p.kv.v_scale[it.hk] : 1.0f) / (total == 0.0f ? 1.0f : total);
-  for (int ch = threadIdx.x; ch < p.kv.dim; ch += WARPS * 32) {
-    float y = 0.0f;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) y = fmaf(sm_o[w][ch], part[w], y);
-    T* out = reinterpret_cast<T*>(p.out.data) + it.b * p.out.row + (int64_t)(it.first_head + h) * p.out.head + ch;
-    if constexpr (std::is_same<T, __half>::value) *out = __float2half_rn(y * scale);
-    else *out = __float2bfloat16_rn(y * scale);
+    for (int w = 0; w < JOIN_WARPS; ++w) y = make_float2(y.x + sm_o[w][ch / 2].x, y.y + sm_o[w][ch / 2].y);
+    T* out = reinterpret_cast<T*>(p.out.data) + item.x * p.out.row + (int64_t)(item.y + h) * p.out.head + ch;
+    *reinterpret_cast<uint32_t*>(out) = pack2<T>(y.x * scale, y.y * scale);
   }
   if (threadIdx.x == 0 && p.lse)
-    p.lse[it.b * p.q_heads + it.first_head + h] = total == 0.0f ? -INFINITY : (top - S::BIAS + log2f(total)) * 0.6931471805599453f;
+    p.lse[(int64_t)item.x * p.q_heads + item.y + h] = total == 0.0f ? -INFINITY : (top - S::BIAS + log2f(total)) * 0.6931471805599453f;
 }
 
 // Blocks of the persistent grid (also the number of pairs of workspace slots).
@@ -812,17 +820,17 @@ static int launch(AttentionParams p, const CUtensorMap& k_map, const CUtensorMap
   kern<<<blocks, WARPS * 32, smem, stream>>>(p, k_map, v_map);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || blocks == 1) return (int)e;
-  // the join may start while the last blocks still run: it finds its item, then waits for them
+  // the join's launch overlaps the end of the attention, for which it waits
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(blocks - 1, min(S::HEADS, p.group));
-  cfg.blockDim = dim3(WARPS * 32);
+  cfg.blockDim = dim3(JOIN_WARPS * 32);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return (int)cudaLaunchKernelEx(&cfg, join_kernel<T, C, DP, NT, FAST>, p, blocks);
+  return (int)cudaLaunchKernelEx(&cfg, join_kernel<T, C, DP, NT>, p);
 }
 
 // Tensor map over a pool: boxes of 16 rows of at most 128 bytes of one head of one page.  (Lines are promoted to 128 bytes in
@@ -869,7 +877,7 @@ using namespace wush::kv;
 extern "C" size_t wush_kv_attention_workspace_bytes(const wush_kv_pages* kv, int q_heads) {
   if (!kv || kv->heads <= 0 || q_heads <= 0 || kv->dim <= 0 || kv->dim > MAX_DIM || q_heads < kv->heads) return 0;
   const int dp = pad_dim(kv->dim), nt = head_tiles(dp, q_heads / kv->heads);
-  return (size_t)2 * grid_blocks(dp, element_bytes(kv->type), nt) * nt * 8 * (dp + 2) * sizeof(float);
+  return (size_t)2 * grid_blocks(dp, element_bytes(kv->type), nt) * (nt * 8 * (dp + 2) * sizeof(float) + sizeof(int4));
 }
 
 extern "C" int wush_kv_attention(const wush_kv_pages* kv, const wush_kv_table* table, int type, const wush_heads* q, int q_heads,
@@ -908,7 +916,9 @@ extern "C" int wush_kv_attention(const wush_kv_pages* kv, const wush_kv_table* t
   p.chunks = (p.group + heads - 1) / heads;
   p.entries = pages ? table->seqs * kv->heads : table->seqs;
   p.part_o = reinterpret_cast<float*>(workspace);
-  p.part_ml = p.part_o + (size_t)2 * grid_blocks(dp, element_bytes(kv->type), nt) * heads * dp;
+  const size_t slots = (size_t)2 * grid_blocks(dp, element_bytes(kv->type), nt);
+  p.part_ml = p.part_o + slots * heads * dp;
+  p.splits = reinterpret_cast<int4*>(p.part_ml + slots * heads * 2);
   int64_t most = pages ? (int64_t)top * kv->page_size : table->width * kv->page_size;   // tokens an item can have
   if (window > 0 && window < most) most = window;
   cudaStream_t s = (cudaStream_t)stream;
