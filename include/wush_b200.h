@@ -529,11 +529,16 @@ typedef struct wush_heads {
 } wush_heads;
 
 /*
+ * The entry points take one struct each (a call from another language then converts one pointer instead of twenty).
+ * `status` (a DEVICE int) may be null; `stream` is a cudaStream_t.
+ */
+
+/*
  * Rotate the new queries and keys by their positions and write keys and values into their pages, in one launch.
  *
  *   type        BF16 / FP16: element type of q, k, v and the outputs (a 16-bit cache has the same)
  *   q           [rows, q_heads, dim] or null data; q_out receives the rotated queries (may be q itself, else disjoint)
- *   k, v        [rows, kv->heads, dim]; k_out null data or receives the rotated keys (may be k itself)
+ *   k, v        [rows, kv.heads, dim]; k_out null data or receives the rotated keys (may be k itself)
  *   rope        fp32 [rope_rows, rotary]: cosines of the rotary/2 angles of a position, then sines; null: no rotation.
  *               rotary % 16 == 0, rotary <= dim; the channels behind it are copied.
  *   interleaved 0: channel i turns with i + rotary/2; 1: channel 2i with 2i + 1
@@ -542,49 +547,89 @@ typedef struct wush_heads {
  * No two rows may name the same token.  Arithmetic: products and their sum each rounded to fp32, stored rounded once
  * to the cache's type (E4M3: divided by the head's scale, saturated at +-448).
  */
-WUSH_API int wush_kv_append(const wush_kv_pages* kv, const wush_kv_table* table, int type, const wush_heads* q, int q_heads,
-                            const wush_heads* q_out, const wush_heads* k, const wush_heads* v, const wush_heads* k_out,
-                            const float* rope, int64_t rope_rows, int rotary, int interleaved, const int32_t* seq_ids,
-                            const int32_t* positions, int64_t rows, int* status, void* stream);
+typedef struct wush_kv_append_args {
+  wush_kv_pages kv;
+  wush_kv_table table;
+  wush_heads q, q_out, k, v, k_out;
+  const float* rope;
+  const int32_t* seq_ids;
+  const int32_t* positions;
+  int* status;
+  void* stream;
+  int64_t rows, rope_rows;
+  int32_t type, q_heads, rotary, interleaved;
+} wush_kv_append_args;
+WUSH_API int wush_kv_append(const wush_kv_append_args* args);
 
 /*
- * Recompute kv->bounds for the pages that hold the last `new_tokens` of the seq_lens[b] tokens of every sequence
+ * Recompute kv.bounds for the pages that hold the last `new_tokens` of the seq_lens[b] tokens of every sequence
  * (a sequence with fewer: all its pages).  A NaN key makes the bound NaN.
  */
-WUSH_API int wush_kv_bounds(const wush_kv_pages* kv, const wush_kv_table* table, const int32_t* seq_lens, int64_t new_tokens,
-                            int* status, void* stream);
+typedef struct wush_kv_bounds_args {
+  wush_kv_pages kv;
+  wush_kv_table table;
+  const int32_t* seq_lens;
+  int* status;
+  void* stream;
+  int64_t new_tokens;
+} wush_kv_bounds_args;
+WUSH_API int wush_kv_bounds(const wush_kv_bounds_args* args);
 
 /*
  * Select, for every sequence and key head, at most `top` pages to attend to: the first `sink` and the last `recent`
  * pages of the sequence, then those with the largest scores; equal scores: the lowest page.
  * score = max over the head's queries of sum_d max(q_d lower_d, q_d upper_d), an upper bound of every logit on the page
  * (before the softmax scale), accumulated in 64 bits; a NaN score counts as +infinity.
- *   q        [seqs, q_heads, dim] of `type`; q_heads % kv->heads == 0
- *   pages    int32 [seqs, kv->heads, top] out: logical pages in ascending order, then -1
- *   counts   int32 [seqs, kv->heads] out: how many
- *   workspace  wush_kv_select_workspace_bytes(seqs, heads, width) bytes
+ *   q        [seqs, q_heads, dim] of `type`; q_heads % kv.heads == 0
+ *   pages    int32 [seqs, kv.heads, top] out: logical pages in ascending order, then -1
+ *   counts   int32 [seqs, kv.heads] out: how many
+ *   workspace  wush_kv_select_workspace_bytes(seqs, heads, width) bytes, 16-byte aligned
  */
+typedef struct wush_kv_select_args {
+  wush_kv_pages kv;
+  wush_kv_table table;
+  wush_heads q;
+  const int32_t* seq_lens;
+  int32_t* pages;
+  int32_t* counts;
+  void* workspace;
+  uint64_t workspace_bytes;
+  int* status;
+  void* stream;
+  int32_t type, q_heads, top, sink, recent;
+} wush_kv_select_args;
 WUSH_API size_t wush_kv_select_workspace_bytes(int64_t seqs, int heads, int64_t width);
-WUSH_API int wush_kv_select_pages(const wush_kv_pages* kv, const wush_kv_table* table, int type, const wush_heads* q, int q_heads,
-                                  const int32_t* seq_lens, int top, int sink, int recent, int32_t* pages, int32_t* counts,
-                                  void* workspace, size_t workspace_bytes, int* status, void* stream);
+WUSH_API int wush_kv_select_pages(const wush_kv_select_args* args);
 
 /*
  * Attention of one new token per sequence over its pages: out = softmax(scale * q K^T) V over the tokens
  * [max(0, len - window), len) (window 0: all), or over the tokens of selected pages.
- *   q, out     [seqs, q_heads, dim] of `type`; query head h reads key head h / (q_heads / kv->heads)
+ *   q, out     [seqs, q_heads, dim] of `type`; query head h reads key head h / (q_heads / kv.heads); out may be q
  *   lse        null, or fp32 [seqs, q_heads] out: log of the sum of exponentials (-infinity for no tokens)
  *   seq_lens   int32 [seqs]; a sequence without tokens (len <= 0) gives zeros
  *   pages, counts  null (all pages), or what wush_kv_select_pages writes: for every sequence and key head the first
  *              counts[b, h] entries of pages[b, h, top] are attended to, each cut at len (window must be 0)
  * A length beyond the table, or an entry outside it, sets *status = 2; tokens on such pages are left out.
- *   workspace  wush_kv_attention_workspace_bytes(kv, q_heads) bytes
+ *   workspace  wush_kv_attention_workspace_bytes(kv, q_heads) bytes, 16-byte aligned
  */
+typedef struct wush_kv_attention_args {
+  wush_kv_pages kv;
+  wush_kv_table table;
+  wush_heads q, out;
+  float* lse;
+  const int32_t* seq_lens;
+  const int32_t* pages;
+  const int32_t* counts;
+  void* workspace;
+  uint64_t workspace_bytes;
+  int* status;
+  void* stream;
+  int64_t window;
+  int32_t type, q_heads, top;
+  float scale;
+} wush_kv_attention_args;
 WUSH_API size_t wush_kv_attention_workspace_bytes(const wush_kv_pages* kv, int q_heads);
-WUSH_API int wush_kv_attention(const wush_kv_pages* kv, const wush_kv_table* table, int type, const wush_heads* q, int q_heads,
-                               const wush_heads* out, float* lse, const int32_t* seq_lens, float scale, int64_t window,
-                               const int32_t* pages, const int32_t* counts, int top, void* workspace, size_t workspace_bytes,
-                               int* status, void* stream);
+WUSH_API int wush_kv_attention(const wush_kv_attention_args* args);
 
 #ifdef __cplusplus
 }

@@ -10,12 +10,63 @@ from wush_b200 import _lib, paged_kv
 BF, HF, F8 = torch.bfloat16, torch.float16, torch.float8_e4m3fn
 
 
+P, Q, I, F = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_float
+fields = lambda names, t: [(n, t) for n in names.split()]
+
+
+class Pages(ctypes.Structure):
+    _fields_ = fields("k v", P) + fields("k_page k_row k_head v_page v_row v_head", Q) + fields("k_scale v_scale bounds", P) \
+        + fields("num_pages", Q) + fields("page_size heads dim type bounds_type", I)
+
+
+class Table(ctypes.Structure):
+    _fields_ = fields("block_table", P) + fields("stride seqs width", Q)
+
+
+class Heads(ctypes.Structure):
+    _fields_ = fields("data", P) + fields("row head", Q)
+
+
+POOL = [("kv", Pages), ("table", Table)]
+
+
+class Append(ctypes.Structure):
+    _fields_ = POOL + fields("q q_out k v k_out", Heads) + fields("rope seq_ids positions status stream", P) \
+        + fields("rows rope_rows", Q) + fields("type q_heads rotary interleaved", I)
+
+
+class Bounds(ctypes.Structure):
+    _fields_ = POOL + fields("seq_lens status stream", P) + fields("new_tokens", Q)
+
+
+class Select(ctypes.Structure):
+    _fields_ = POOL + fields("q", Heads) + fields("seq_lens pages counts workspace", P) + fields("workspace_bytes", ctypes.c_uint64) \
+        + fields("status stream", P) + fields("type q_heads top sink recent", I)
+
+
+class Attention(ctypes.Structure):
+    _fields_ = POOL + fields("q out", Heads) + fields("lse seq_lens pages counts workspace", P) \
+        + fields("workspace_bytes", ctypes.c_uint64) + fields("status stream", P) + fields("window", Q) + fields("type q_heads top", I) \
+        + fields("scale", F)
+
+
+def test_packed_structs_have_the_layout_of_the_header():
+    for cls, packed in ((Append, paged_kv._APPEND), (Bounds, paged_kv._BOUNDS), (Select, paged_kv._SELECT), (Attention, paged_kv._ATTENTION)):
+        assert paged_kv._PAGES.size == ctypes.sizeof(Pages) and ctypes.sizeof(cls) == ctypes.sizeof(Pages) + packed.size
+        values = list(range(1, len(packed.unpack(bytes(packed.size))) + 1))
+        got, flat = cls.from_buffer_copy(bytes(ctypes.sizeof(Pages)) + packed.pack(*values)), []
+        for name, t in cls._fields_[1:]:
+            v = getattr(got, name)
+            flat += [getattr(v, n) for n, _ in t._fields_] if isinstance(v, ctypes.Structure) else [v]
+        assert flat == values
+
+
 def _pages(p, **kw):
     """A bf16 pool of 4 pages of 16 rows, 2 heads of 64 channels."""
     d = dict(k=p, v=p, k_page=2048, k_row=128, k_head=64, v_page=2048, v_row=128, v_head=64, k_scale=None, v_scale=None,
              bounds=p, num_pages=4, page_size=16, heads=2, dim=64, type=0, bounds_type=0)
     d.update(kw)
-    return _lib.KVPages(**d)
+    return Pages(**d)
 
 
 @pytest.fixture()
@@ -25,77 +76,58 @@ def ptr():
     del buf
 
 
-def _append(lib, pages, table, p, typ=0, q_heads=4, rotary=64, rope_rows=100, rows=1, k=None, q=None, q_out=None, ids=True):
-    h = lambda **kw: _lib.Heads(**{**dict(data=p, row=512, head=64), **kw})
-    k, q, q_out = k or h(), q or h(), q_out or h()
-    r = ctypes.byref
-    return lib.wush_kv_append(r(pages), r(table), typ, r(q), q_heads, r(q_out), r(k), r(h()), None, p, rope_rows, rotary, 0,
-                              p if ids else None, p, rows, None, None)
-
-
 def test_c_abi_refusals(ptr):
     lib, p = _lib.load(), ptr
-    table = _lib.KVTable(p, 8, 3, 8)
-    r = ctypes.byref
-    lens = p
-    assert _append(lib, _pages(p), table, p, rows=0) == 0
-    assert _append(lib, _pages(None), table, p) == -1
-    assert _append(lib, _pages(p), table, p, ids=False) == -1
-    assert _append(lib, _pages(p), table, p, q_out=_lib.Heads(None, 512, 64)) == -1
-    assert _append(lib, _pages(p), table, p, typ=2) == -4                 # queries have 16 bits
-    assert _append(lib, _pages(p), table, p, typ=1) == -4                 # fp16 queries, bf16 pages
-    assert _append(lib, _pages(p, type=3), table, p) == -4
-    assert _append(lib, _pages(p, dim=264), table, p) == -2               # more than 256 channels
-    assert _append(lib, _pages(p, dim=60), table, p) == -2                # no whole 16 bytes
-    assert _append(lib, _pages(p, type=2, dim=72, k_scale=p, v_scale=p), table, p) == -2
-    assert _append(lib, _pages(p, type=2), table, p) == -1                # 8-bit pages without scales
-    assert _append(lib, _pages(p, k_scale=p, v_scale=p), table, p) == -1  # scales without 8-bit pages
-    assert _append(lib, _pages(p, k_row=130), table, p) == -3
-    assert _append(lib, _pages(p, v_page=-2048), table, p) == -2
-    assert _append(lib, _pages(p + 8), table, p) == -3
-    assert _append(lib, _pages(p, page_size=0), table, p) == -2
-    assert _append(lib, _pages(p, num_pages=1 << 31), table, p) == -2
-    assert _append(lib, _pages(p), _lib.KVTable(p, 8, 3, 0), p) == -2
-    assert _append(lib, _pages(p), _lib.KVTable(p, 8, 3, 1 << 27), p) == -8   # 2^31 tokens
-    assert _append(lib, _pages(p), table, p, rotary=24) == -2
-    assert _append(lib, _pages(p), table, p, rotary=80) == -2             # more than the head
-    assert _append(lib, _pages(p), table, p, rope_rows=0) == -2
-    assert _append(lib, _pages(p), table, p, q_heads=0) == -2
-    assert _append(lib, _pages(p), table, p, k=_lib.Heads(p + 2, 512, 64)) == -3
-    assert _append(lib, _pages(p), table, p, k=_lib.Heads(p, 516, 64)) == -3
-    assert _append(lib, _pages(p), table, p, rows=-1) == -2
+    h = lambda **kw: Heads(**{**dict(data=p, row=512, head=64), **kw})
 
-    assert lib.wush_kv_bounds(r(_pages(p, bounds=None)), r(table), lens, 1, None, None) == -1
-    assert lib.wush_kv_bounds(r(_pages(p, bounds_type=1)), r(table), lens, 1, None, None) == -4
-    assert lib.wush_kv_bounds(r(_pages(p)), r(table), None, 1, None, None) == -1
-    assert lib.wush_kv_bounds(r(_pages(p)), r(table), lens, -1, None, None) == -2
-    assert lib.wush_kv_bounds(r(_pages(p)), r(table), lens, 0, None, None) == 0
+    def call(fn, cls, base, kw):
+        return getattr(lib, fn)(bytes(cls(**{**dict(kv=_pages(p), table=Table(p, 8, 3, 8)), **base, **kw})))
+    append = lambda **kw: call("wush_kv_append", Append, dict(q=h(), q_out=h(), k=h(), v=h(), rope=p, seq_ids=p, positions=p, rows=1,
+                                                             rope_rows=100, q_heads=4, rotary=64), kw)
+    assert append(rows=0) == 0
+    assert append(kv=_pages(None)) == -1 and append(seq_ids=None) == -1 and append(q_out=h(data=None)) == -1
+    assert append(type=2) == -4                                            # queries have 16 bits
+    assert append(type=1) == -4                                            # fp16 queries, bf16 pages
+    assert append(kv=_pages(p, type=3)) == -4
+    assert append(kv=_pages(p, dim=264)) == -2                             # more than 256 channels
+    assert append(kv=_pages(p, dim=60)) == -2                              # no whole 16 bytes
+    assert append(kv=_pages(p, type=2, dim=72, k_scale=p, v_scale=p)) == -2
+    assert append(kv=_pages(p, type=2)) == -1                              # 8-bit pages without scales
+    assert append(kv=_pages(p, k_scale=p, v_scale=p)) == -1                # scales without 8-bit pages
+    assert append(kv=_pages(p, k_row=130)) == -3 and append(kv=_pages(p + 8)) == -3
+    assert append(kv=_pages(p, v_page=-2048)) == -2 and append(kv=_pages(p, page_size=0)) == -2
+    assert append(kv=_pages(p, num_pages=1 << 31)) == -2
+    assert append(table=Table(p, 8, 3, 0)) == -2
+    assert append(table=Table(p, 8, 3, 1 << 27)) == -8                     # 2^31 tokens
+    assert append(rotary=24) == -2 and append(rotary=80) == -2 and append(rope_rows=0) == -2
+    assert append(q_heads=0) == -2 and append(rows=-1) == -2
+    assert append(k=h(data=p + 2)) == -3 and append(k=h(row=516)) == -3 and append(k_out=h(head=4)) == -3
 
-    h = _lib.Heads(p, 512, 64)
-    select = lambda pages=None, heads=4, top=4, sink=1, recent=1, work=p, nbytes=4096, q=h: lib.wush_kv_select_pages(
-        r(pages or _pages(p)), r(table), 0, r(q), heads, lens, top, sink, recent, p, p, work, nbytes, None, None)
+    bounds = lambda **kw: call("wush_kv_bounds", Bounds, dict(seq_lens=p, new_tokens=1), kw)
+    assert bounds(kv=_pages(p, bounds=None)) == -1 and bounds(kv=_pages(p, bounds_type=1)) == -4
+    assert bounds(seq_lens=None) == -1 and bounds(new_tokens=-1) == -2 and bounds(new_tokens=0) == 0
+
     need = lib.wush_kv_select_workspace_bytes(3, 2, 8)
     assert need >= 3 * 2 * 8 * 8
-    assert select(heads=3) == -2                                          # not a multiple of the key heads
+    select = lambda **kw: call("wush_kv_select_pages", Select, dict(q=h(), q_heads=4, seq_lens=p, top=4, sink=1, recent=1, pages=p,
+                                                                    counts=p, workspace=p, workspace_bytes=4096), kw)
+    assert select(q_heads=3) == -2                                         # not a multiple of the key heads
     assert select(top=0, sink=0, recent=0) == -2 and select(top=1) == -2 and select(sink=-1) == -2
-    assert select(pages=_pages(p, bounds=None)) == -1 and select(work=None) == -1
-    assert select(nbytes=need - 1) == -5
-    assert select(q=_lib.Heads(p, 512, 60)) == -3
+    assert select(kv=_pages(p, bounds=None)) == -1 and select(workspace=None) == -1 and select(counts=None) == -1
+    assert select(workspace_bytes=need - 1) == -5 and select(q=h(head=60)) == -3
 
-    nbytes = lib.wush_kv_attention_workspace_bytes(r(_pages(p)), 4)
-    attend = lambda heads=4, window=0, pages=None, counts=None, top=0, out=h, q=h, lens=p, work=p, nbytes=1 << 40: \
-        lib.wush_kv_attention(r(_pages(p)), r(table), 0, r(q), heads, r(out), None, lens, 0.125, window, pages, counts, top, work,
-                              nbytes, None, None)
-    assert attend(heads=5) == -2 and attend(window=-1) == -2
-    assert attend(pages=p) == -1 and attend(counts=p) == -1               # they go together
+    nbytes = lib.wush_kv_attention_workspace_bytes(bytes(_pages(p)), 4)
+    attend = lambda **kw: call("wush_kv_attention", Attention, dict(q=h(), out=h(), q_heads=4, seq_lens=p, scale=0.125, workspace=p,
+                                                                    workspace_bytes=1 << 40), kw)
+    assert attend(q_heads=5) == -2 and attend(window=-1) == -2
+    assert attend(pages=p) == -1 and attend(counts=p) == -1                # they go together
     assert attend(pages=p, counts=p, top=0) == -2 and attend(pages=p, counts=p, top=1 << 28) == -2
     assert attend(pages=p, counts=p, top=4, window=5) == -4
-    assert attend(out=_lib.Heads(None, 512, 64)) == -1 and attend(lens=None) == -1
-    assert attend(q=_lib.Heads(p + 4, 512, 64)) == -3
-    if nbytes:
-        assert attend(nbytes=nbytes - 1) == -5
-    empty = _lib.KVTable(None, 8, 0, 8)
-    assert lib.wush_kv_attention(r(_pages(p)), r(empty), 0, r(h), 4, r(h), None, None, 1.0, 0, None, None, 0, None, 0, None, None) == 0
+    assert attend(out=h(data=None)) == -1 and attend(seq_lens=None) == -1 and attend(workspace=None) == -1
+    assert attend(q=h(data=p + 4)) == -3 and attend(workspace=p + 4) == -3 and attend(workspace_bytes=nbytes - 1) == -5
+    assert attend(table=Table(None, 8, 0, 8)) == 0
+    for fn in ("wush_kv_append", "wush_kv_bounds", "wush_kv_select_pages", "wush_kv_attention"):
+        assert getattr(lib, fn)(None) == -1
 
 
 def test_cpu_tensors_are_refused():

@@ -37,24 +37,6 @@ class WushB200Error(RuntimeError):
     pass
 
 
-class KVPages(ctypes.Structure):
-    """wush_kv_pages"""
-    _fields_ = ([(n, ctypes.c_void_p) for n in ("k", "v")]
-                + [(n, ctypes.c_int64) for n in ("k_page", "k_row", "k_head", "v_page", "v_row", "v_head")]
-                + [(n, ctypes.c_void_p) for n in ("k_scale", "v_scale", "bounds")] + [("num_pages", ctypes.c_int64)]
-                + [(n, ctypes.c_int32) for n in ("page_size", "heads", "dim", "type", "bounds_type")])
-
-
-class KVTable(ctypes.Structure):
-    """wush_kv_table"""
-    _fields_ = [("block_table", ctypes.c_void_p), ("stride", ctypes.c_int64), ("seqs", ctypes.c_int64), ("width", ctypes.c_int64)]
-
-
-class Heads(ctypes.Structure):
-    """wush_heads"""
-    _fields_ = [("data", ctypes.c_void_p), ("row", ctypes.c_int64), ("head", ctypes.c_int64)]
-
-
 def declared_symbols(header: str = HEADER_PATH) -> list[str]:
     """Names of every function the public header declares."""
     text = open(header).read()
@@ -104,14 +86,8 @@ def load() -> ctypes.CDLL:
         "wush_gptq_block_step": [vp, vp, vp, vp, i32, i32, i64, i64, i32, i32, vp, vp, vp, vp, vp],
         "wush_gptq_block_prepare": [vp, vp, i64, i64, i32, i32, i32, i32, i64, vp, vp, vp, vp, vp],
     }
-    f32, size = ctypes.c_float, ctypes.c_size_t
-    pages, table, heads = ctypes.POINTER(KVPages), ctypes.POINTER(KVTable), ctypes.POINTER(Heads)
-    sigs |= {
-        "wush_kv_append": [pages, table, i32, heads, i32, heads, heads, heads, heads, vp, i64, i32, i32, vp, vp, i64, vp, vp],
-        "wush_kv_bounds": [pages, table, vp, i64, vp, vp],
-        "wush_kv_select_pages": [pages, table, i32, heads, i32, vp, i32, i32, i32, vp, vp, vp, size, vp, vp],
-        "wush_kv_attention": [pages, table, i32, heads, i32, heads, vp, vp, f32, i64, vp, vp, i32, vp, size, vp, vp],
-    }
+    # these take one struct, packed by the caller (wush_b200/paged_kv.py)
+    sigs |= {name: [ctypes.c_char_p] for name in ("wush_kv_append", "wush_kv_bounds", "wush_kv_select_pages", "wush_kv_attention")}
     for name, args in sigs.items():
         fn = getattr(lib, name)
         fn.argtypes = args
@@ -122,7 +98,7 @@ def load() -> ctypes.CDLL:
     lib.wush_gemm_workspace_bytes.restype = ctypes.c_size_t
     lib.wush_kv_select_workspace_bytes.argtypes = [i64, i32, i64]
     lib.wush_kv_select_workspace_bytes.restype = ctypes.c_size_t
-    lib.wush_kv_attention_workspace_bytes.argtypes = [pages, i32]
+    lib.wush_kv_attention_workspace_bytes.argtypes = [ctypes.c_char_p, i32]
     lib.wush_kv_attention_workspace_bytes.restype = ctypes.c_size_t
     lib.wush_hessian_tile_count.argtypes = [i64]
     lib.wush_hessian_tile_count.restype = ctypes.c_int64
@@ -186,4 +162,16 @@ def gemm_workspace(device, nbytes: int):
     w = _workspaces.get(key)
     if w is None or w.numel() < nbytes:
         w = _workspaces[key] = torch.empty(max(nbytes, 1 << 22), dtype=torch.uint8, device=device)
+    return w
+
+
+def stream_workspace(index: int, stream: int, nbytes: int):
+    """gemm_workspace for callers that have the device's index (the current device) and the raw stream at hand: the same
+    scratch per stream, or the graph's own while the stream is being captured."""
+    import torch
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
+    w = _workspaces.get((index, stream))
+    if w is None or w.numel() < nbytes:
+        w = _workspaces[(index, stream)] = torch.empty(max(nbytes, 1 << 22), dtype=torch.uint8, device=torch.device("cuda", index))
     return w

@@ -880,49 +880,50 @@ extern "C" size_t wush_kv_attention_workspace_bytes(const wush_kv_pages* kv, int
   return (size_t)2 * grid_blocks(dp, element_bytes(kv->type), nt) * (nt * 8 * (dp + 2) * sizeof(float) + sizeof(int4));
 }
 
-extern "C" int wush_kv_attention(const wush_kv_pages* kv, const wush_kv_table* table, int type, const wush_heads* q, int q_heads,
-                                 const wush_heads* out, float* lse, const int32_t* seq_lens, float scale, int64_t window,
-                                 const int32_t* pages, const int32_t* counts, int top, void* workspace, size_t workspace_bytes,
-                                 int* status, void* stream) {
-  int rc = check_pages(kv, table, type);
+extern "C" int wush_kv_attention(const wush_kv_attention_args* args) {
+  if (!args) return WUSH_ERR_NULL_POINTER;
+  const wush_kv_attention_args& a = *args;
+  const wush_kv_pages& kv = a.kv;
+  const wush_kv_table& table = a.table;
+  int rc = check_pages(&kv, &table, a.type);
   if (rc != 0) return rc;
-  if (q_heads <= 0 || q_heads % kv->heads || window < 0) return WUSH_ERR_BAD_SHAPE;
-  if ((pages == nullptr) != (counts == nullptr)) return WUSH_ERR_NULL_POINTER;
-  if (pages && (top <= 0 || (int64_t)top * kv->page_size > MAX_TOKENS)) return WUSH_ERR_BAD_SHAPE;
-  if (pages && window != 0) return WUSH_ERR_BAD_FLAG;
-  if (table->seqs == 0) return WUSH_OK;
-  if ((rc = check_heads(q, 2)) != 0 || (rc = check_heads(out, 2)) != 0) return rc;
-  if (!seq_lens || !workspace) return WUSH_ERR_NULL_POINTER;
-  if (!aligned16(workspace)) return WUSH_ERR_BAD_ALIGNMENT;
-  if (workspace_bytes < wush_kv_attention_workspace_bytes(kv, q_heads)) return WUSH_ERR_WORKSPACE_TOO_SMALL;
-  if (table->seqs * q_heads > INT32_MAX) return WUSH_ERR_TOO_LARGE;
+  if (a.q_heads <= 0 || a.q_heads % kv.heads || a.window < 0) return WUSH_ERR_BAD_SHAPE;
+  if ((a.pages == nullptr) != (a.counts == nullptr)) return WUSH_ERR_NULL_POINTER;
+  if (a.pages && (a.top <= 0 || (int64_t)a.top * kv.page_size > MAX_TOKENS)) return WUSH_ERR_BAD_SHAPE;
+  if (a.pages && a.window != 0) return WUSH_ERR_BAD_FLAG;
+  if (table.seqs == 0) return WUSH_OK;
+  if ((rc = check_heads(&a.q, 2)) != 0 || (rc = check_heads(&a.out, 2)) != 0) return rc;
+  if (!a.seq_lens || !a.workspace) return WUSH_ERR_NULL_POINTER;
+  if (!aligned16(a.workspace)) return WUSH_ERR_BAD_ALIGNMENT;
+  if (a.workspace_bytes < wush_kv_attention_workspace_bytes(&kv, a.q_heads)) return WUSH_ERR_WORKSPACE_TOO_SMALL;
+  if (table.seqs * a.q_heads > INT32_MAX) return WUSH_ERR_TOO_LARGE;
   if ((rc = require_sm100()) != 0) return rc;
   AttentionParams p{};
-  p.kv = *kv;
-  p.table = *table;
-  p.q = *q;
-  p.out = *out;
-  p.lse = lse;
-  p.seq_lens = seq_lens;
-  p.pages = pages;
-  p.counts = counts;
-  p.status = status;
-  p.scale = scale;
-  p.window = window;
-  p.q_heads = q_heads;
-  p.group = q_heads / kv->heads;
-  p.top = top;
-  const int dp = pad_dim(kv->dim), nt = head_tiles(dp, p.group), heads = nt * 8;
+  p.kv = kv;
+  p.table = table;
+  p.q = a.q;
+  p.out = a.out;
+  p.lse = a.lse;
+  p.seq_lens = a.seq_lens;
+  p.pages = a.pages;
+  p.counts = a.counts;
+  p.status = a.status;
+  p.scale = a.scale;
+  p.window = a.window;
+  p.q_heads = a.q_heads;
+  p.group = a.q_heads / kv.heads;
+  p.top = a.top;
+  const int dp = pad_dim(kv.dim), nt = head_tiles(dp, p.group), heads = nt * 8;
   p.chunks = (p.group + heads - 1) / heads;
-  p.entries = pages ? table->seqs * kv->heads : table->seqs;
-  p.part_o = reinterpret_cast<float*>(workspace);
-  const size_t slots = (size_t)2 * grid_blocks(dp, element_bytes(kv->type), nt);
+  p.entries = a.pages ? table.seqs * kv.heads : table.seqs;
+  p.part_o = reinterpret_cast<float*>(a.workspace);
+  const size_t slots = (size_t)2 * grid_blocks(dp, element_bytes(kv.type), nt);
   p.part_ml = p.part_o + slots * heads * dp;
   p.splits = reinterpret_cast<int4*>(p.part_ml + slots * heads * 2);
-  int64_t most = pages ? (int64_t)top * kv->page_size : table->width * kv->page_size;   // tokens an item can have
-  if (window > 0 && window < most) most = window;
-  cudaStream_t s = (cudaStream_t)stream;
-  if (type == WUSH_TYPE_BF16)
-    return kv->type == WUSH_TYPE_E4M3 ? dispatch<__nv_bfloat16, __nv_fp8_e4m3>(p, most, s) : dispatch<__nv_bfloat16, __nv_bfloat16>(p, most, s);
-  return kv->type == WUSH_TYPE_E4M3 ? dispatch<__half, __nv_fp8_e4m3>(p, most, s) : dispatch<__half, __half>(p, most, s);
+  int64_t most = a.pages ? (int64_t)a.top * kv.page_size : table.width * kv.page_size;   // tokens an item can have
+  if (a.window > 0 && a.window + 15 < most) most = a.window + 15;                        // (from a multiple of 16 on)
+  cudaStream_t s = (cudaStream_t)a.stream;
+  if (a.type == WUSH_TYPE_BF16)
+    return kv.type == WUSH_TYPE_E4M3 ? dispatch<__nv_bfloat16, __nv_fp8_e4m3>(p, most, s) : dispatch<__nv_bfloat16, __nv_bfloat16>(p, most, s);
+  return kv.type == WUSH_TYPE_E4M3 ? dispatch<__half, __nv_fp8_e4m3>(p, most, s) : dispatch<__half, __half>(p, most, s);
 }

@@ -5,17 +5,7 @@ namespace wush {
 namespace kv {
 
 // ---- append --------------------------------------------------------------------------------------------------------
-struct AppendParams {
-  wush_kv_pages kv;
-  wush_kv_table table;
-  wush_heads q, q_out, k, v, k_out;
-  const float* rope;
-  const int32_t* seq_ids;
-  const int32_t* positions;
-  int* status;
-  int64_t rows, rope_rows;
-  int q_heads, rotary, interleaved;
-};
+using AppendParams = wush_kv_append_args;
 
 // One thread per unit of 16 channels of a head (two chunks of 8 that are rotated against each other, or two chunks that
 // are only copied).
@@ -271,95 +261,96 @@ __global__ void __launch_bounds__(1024) select_kernel(int page_size, int64_t wid
 using namespace wush;
 using namespace wush::kv;
 
-extern "C" int wush_kv_append(const wush_kv_pages* kv, const wush_kv_table* table, int type, const wush_heads* q, int q_heads,
-                              const wush_heads* q_out, const wush_heads* k, const wush_heads* v, const wush_heads* k_out,
-                              const float* rope, int64_t rope_rows, int rotary, int interleaved, const int32_t* seq_ids,
-                              const int32_t* positions, int64_t rows, int* status, void* stream) {
-  int rc = check_pages(kv, table, type);
-  if (rc == 0) rc = check_heads(k, 2);
-  if (rc == 0) rc = check_heads(v, 2);
-  const bool with_q = q && q->data;
-  if (rc == 0 && with_q) rc = check_heads(q, 2);
-  if (rc == 0 && with_q) rc = check_heads(q_out, 2);
-  if (rc == 0 && k_out && k_out->data) rc = check_heads(k_out, 2);
+extern "C" int wush_kv_append(const wush_kv_append_args* args) {
+  if (!args) return WUSH_ERR_NULL_POINTER;
+  AppendParams p = *args;
+  int rc = check_pages(&p.kv, &p.table, p.type);
+  if (rc == 0) rc = check_heads(&p.k, 2);
+  if (rc == 0) rc = check_heads(&p.v, 2);
+  if (rc == 0 && p.q.data) rc = check_heads(&p.q, 2);
+  if (rc == 0 && p.q.data) rc = check_heads(&p.q_out, 2);
+  if (rc == 0 && p.k_out.data) rc = check_heads(&p.k_out, 2);
   if (rc != 0) return rc;
-  if (rows < 0 || (with_q && (q_heads <= 0 || q_heads > 65535))) return WUSH_ERR_BAD_SHAPE;
-  if (rope) {
-    if (rope_rows <= 0 || rotary <= 0 || rotary % 16 || rotary > kv->dim) return WUSH_ERR_BAD_SHAPE;
-    if (!aligned16(rope)) return WUSH_ERR_BAD_ALIGNMENT;
+  if (p.rows < 0 || (p.q.data && (p.q_heads <= 0 || p.q_heads > 65535))) return WUSH_ERR_BAD_SHAPE;
+  if (p.rope) {
+    if (p.rope_rows <= 0 || p.rotary <= 0 || p.rotary % 16 || p.rotary > p.kv.dim) return WUSH_ERR_BAD_SHAPE;
+    if (!aligned16(p.rope)) return WUSH_ERR_BAD_ALIGNMENT;
+  } else {
+    p.rotary = 0;
   }
-  if (rows == 0) return WUSH_OK;
-  if (!seq_ids || !positions) return WUSH_ERR_NULL_POINTER;
+  if (!p.q.data) p.q_heads = 0;
+  if (p.rows == 0) return WUSH_OK;
+  if (!p.seq_ids || !p.positions) return WUSH_ERR_NULL_POINTER;
   if ((rc = require_sm100()) != 0) return rc;
-  const wush_heads none = {nullptr, 0, 0};
-  AppendParams p{*kv, *table, with_q ? *q : none, with_q ? *q_out : none, *k, *v, k_out ? *k_out : none, rope, seq_ids,
-                 positions, status, rows, rope_rows, with_q ? q_heads : 0, rope ? rotary : 0, interleaved != 0};
-  const int64_t units = rows * (int64_t)(p.q_heads + 2 * kv->heads) * ((kv->dim + 15) / 16 + 1);
+  const int64_t units = p.rows * (int64_t)(p.q_heads + 2 * p.kv.heads) * ((p.kv.dim + 15) / 16 + 1);
   const unsigned grid = (unsigned)min((units + 255) / 256, (int64_t)sm_count() * 32);
   auto go = [&](auto kern) {
-    kern<<<grid, 256, 0, (cudaStream_t)stream>>>(p);
+    kern<<<grid, 256, 0, (cudaStream_t)p.stream>>>(p);
     return (int)cudaGetLastError();
   };
-  if (type == WUSH_TYPE_BF16)
-    return kv->type == WUSH_TYPE_E4M3 ? go(append_kernel<__nv_bfloat16, __nv_fp8_e4m3>) : go(append_kernel<__nv_bfloat16, __nv_bfloat16>);
-  return kv->type == WUSH_TYPE_E4M3 ? go(append_kernel<__half, __nv_fp8_e4m3>) : go(append_kernel<__half, __half>);
+  if (p.type == WUSH_TYPE_BF16)
+    return p.kv.type == WUSH_TYPE_E4M3 ? go(append_kernel<__nv_bfloat16, __nv_fp8_e4m3>) : go(append_kernel<__nv_bfloat16, __nv_bfloat16>);
+  return p.kv.type == WUSH_TYPE_E4M3 ? go(append_kernel<__half, __nv_fp8_e4m3>) : go(append_kernel<__half, __half>);
 }
 
-extern "C" int wush_kv_bounds(const wush_kv_pages* kv, const wush_kv_table* table, const int32_t* seq_lens, int64_t new_tokens,
-                              int* status, void* stream) {
-  int rc = check_pages(kv, table, kv && kv->type == WUSH_TYPE_FP16 ? WUSH_TYPE_FP16 : WUSH_TYPE_BF16);
+extern "C" int wush_kv_bounds(const wush_kv_bounds_args* args) {
+  if (!args) return WUSH_ERR_NULL_POINTER;
+  const wush_kv_pages& kv = args->kv;
+  const wush_kv_table& table = args->table;
+  int rc = check_pages(&kv, &table, kv.type == WUSH_TYPE_FP16 ? WUSH_TYPE_FP16 : WUSH_TYPE_BF16);
   if (rc != 0) return rc;
-  if (!kv->bounds) return WUSH_ERR_NULL_POINTER;
-  if (new_tokens < 0) return WUSH_ERR_BAD_SHAPE;
+  if (!kv.bounds) return WUSH_ERR_NULL_POINTER;
+  if (args->new_tokens < 0) return WUSH_ERR_BAD_SHAPE;
   // the bounds hold stored keys exactly: their type is the cache's, or either 16-bit type for E4M3
-  if (kv->type != WUSH_TYPE_E4M3 && kv->bounds_type != kv->type) return WUSH_ERR_BAD_FLAG;
-  if (table->seqs == 0 || new_tokens == 0) return WUSH_OK;
-  if (!seq_lens) return WUSH_ERR_NULL_POINTER;
+  if (kv.type != WUSH_TYPE_E4M3 && kv.bounds_type != kv.type) return WUSH_ERR_BAD_FLAG;
+  if (table.seqs == 0 || args->new_tokens == 0) return WUSH_OK;
+  if (!args->seq_lens) return WUSH_ERR_NULL_POINTER;
   if ((rc = require_sm100()) != 0) return rc;
-  const int64_t most = min(table->width, (new_tokens - 1) / kv->page_size + 2);   // pages that the last tokens can touch
-  const int64_t warps = table->seqs * most * kv->heads;
+  const int64_t most = min(table.width, (args->new_tokens - 1) / kv.page_size + 2);   // pages that the last tokens can touch
+  const int64_t warps = table.seqs * most * kv.heads;
   const unsigned grid = (unsigned)min((warps + 7) / 8, (int64_t)sm_count() * 32);
   auto go = [&](auto kern) {
-    kern<<<grid, 256, 0, (cudaStream_t)stream>>>(*kv, *table, seq_lens, new_tokens, most, status);
+    kern<<<grid, 256, 0, (cudaStream_t)args->stream>>>(kv, table, args->seq_lens, args->new_tokens, most, args->status);
     return (int)cudaGetLastError();
   };
-  if (kv->type == WUSH_TYPE_BF16) return go(bounds_kernel<__nv_bfloat16, __nv_bfloat16>);
-  if (kv->type == WUSH_TYPE_FP16) return go(bounds_kernel<__half, __half>);
-  return kv->bounds_type == WUSH_TYPE_BF16 ? go(bounds_kernel<__nv_fp8_e4m3, __nv_bfloat16>) : go(bounds_kernel<__nv_fp8_e4m3, __half>);
+  if (kv.type == WUSH_TYPE_BF16) return go(bounds_kernel<__nv_bfloat16, __nv_bfloat16>);
+  if (kv.type == WUSH_TYPE_FP16) return go(bounds_kernel<__half, __half>);
+  return kv.bounds_type == WUSH_TYPE_BF16 ? go(bounds_kernel<__nv_fp8_e4m3, __nv_bfloat16>) : go(bounds_kernel<__nv_fp8_e4m3, __half>);
 }
 
 extern "C" size_t wush_kv_select_workspace_bytes(int64_t seqs, int heads, int64_t width) {
   return seqs > 0 && heads > 0 && width > 0 ? (size_t)seqs * heads * width * 8 : 0;
 }
 
-extern "C" int wush_kv_select_pages(const wush_kv_pages* kv, const wush_kv_table* table, int type, const wush_heads* q, int q_heads,
-                                    const int32_t* seq_lens, int top, int sink, int recent, int32_t* pages, int32_t* counts,
-                                    void* workspace, size_t workspace_bytes, int* status, void* stream) {
-  int rc = check_pages(kv, table, type);
+extern "C" int wush_kv_select_pages(const wush_kv_select_args* args) {
+  if (!args) return WUSH_ERR_NULL_POINTER;
+  const wush_kv_select_args& a = *args;
+  int rc = check_pages(&a.kv, &a.table, a.type);
   if (rc != 0) return rc;
-  if (!kv->bounds) return WUSH_ERR_NULL_POINTER;
-  if (q_heads <= 0 || q_heads % kv->heads || top <= 0 || sink < 0 || recent < 0 || sink > top || recent > top - sink)
+  if (!a.kv.bounds) return WUSH_ERR_NULL_POINTER;
+  if (a.q_heads <= 0 || a.q_heads % a.kv.heads || a.top <= 0 || a.sink < 0 || a.recent < 0 || a.sink > a.top || a.recent > a.top - a.sink)
     return WUSH_ERR_BAD_SHAPE;
-  if (table->seqs == 0) return WUSH_OK;
-  if ((rc = check_heads(q, 2)) != 0) return rc;
-  if (!seq_lens || !pages || !counts || !workspace) return WUSH_ERR_NULL_POINTER;
-  if (!aligned16(workspace)) return WUSH_ERR_BAD_ALIGNMENT;
-  if (workspace_bytes < wush_kv_select_workspace_bytes(table->seqs, kv->heads, table->width)) return WUSH_ERR_WORKSPACE_TOO_SMALL;
-  if (table->seqs * kv->heads > INT32_MAX) return WUSH_ERR_TOO_LARGE;
+  if (a.table.seqs == 0) return WUSH_OK;
+  if ((rc = check_heads(&a.q, 2)) != 0) return rc;
+  if (!a.seq_lens || !a.pages || !a.counts || !a.workspace) return WUSH_ERR_NULL_POINTER;
+  if (!aligned16(a.workspace)) return WUSH_ERR_BAD_ALIGNMENT;
+  if (a.workspace_bytes < wush_kv_select_workspace_bytes(a.table.seqs, a.kv.heads, a.table.width)) return WUSH_ERR_WORKSPACE_TOO_SMALL;
+  if (a.table.seqs * a.kv.heads > INT32_MAX) return WUSH_ERR_TOO_LARGE;
   if ((rc = require_sm100()) != 0) return rc;
-  unsigned long long* keys = reinterpret_cast<unsigned long long*>(workspace);
-  const int64_t warps = table->seqs * kv->heads * table->width;
+  unsigned long long* keys = reinterpret_cast<unsigned long long*>(a.workspace);
+  const int64_t warps = a.table.seqs * a.kv.heads * a.table.width;
   const unsigned grid = (unsigned)min((warps + 7) / 8, (int64_t)sm_count() * 32);
+  cudaStream_t stream = (cudaStream_t)a.stream;
   auto go = [&](auto kern) {
-    kern<<<grid, 256, 0, (cudaStream_t)stream>>>(*kv, *table, *q, q_heads / kv->heads, seq_lens, top, keys, status);
+    kern<<<grid, 256, 0, stream>>>(a.kv, a.table, a.q, a.q_heads / a.kv.heads, a.seq_lens, a.top, keys, a.status);
     return (int)cudaGetLastError();
   };
-  if (type == WUSH_TYPE_BF16)
-    rc = kv->bounds_type == WUSH_TYPE_BF16 ? go(score_kernel<__nv_bfloat16, __nv_bfloat16>) : go(score_kernel<__nv_bfloat16, __half>);
+  if (a.type == WUSH_TYPE_BF16)
+    rc = a.kv.bounds_type == WUSH_TYPE_BF16 ? go(score_kernel<__nv_bfloat16, __nv_bfloat16>) : go(score_kernel<__nv_bfloat16, __half>);
   else
-    rc = kv->bounds_type == WUSH_TYPE_BF16 ? go(score_kernel<__half, __nv_bfloat16>) : go(score_kernel<__half, __half>);
+    rc = a.kv.bounds_type == WUSH_TYPE_BF16 ? go(score_kernel<__half, __nv_bfloat16>) : go(score_kernel<__half, __half>);
   if (rc != 0) return rc;
-  select_kernel<<<(unsigned)(table->seqs * kv->heads), 1024, 0, (cudaStream_t)stream>>>(
-      kv->page_size, table->width, kv->heads, seq_lens, keys, top, sink, recent, pages, counts);
+  select_kernel<<<(unsigned)(a.table.seqs * a.kv.heads), 1024, 0, stream>>>(
+      a.kv.page_size, a.table.width, a.kv.heads, a.seq_lens, keys, a.top, a.sink, a.recent, a.pages, a.counts);
   return (int)cudaGetLastError();
 }

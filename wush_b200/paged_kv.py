@@ -21,12 +21,22 @@ reported by ``_lib.check_status(device)``.
 """
 from __future__ import annotations
 
-import ctypes
+import functools
+from struct import Struct
 from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
+
+# The structs of include/wush_b200.h: wush_kv_pages comes packed from the cache, the rest of a call's arguments follow it.
+# (Packing one struct costs a tenth of converting as many arguments, and a small call is bound by its host time.)
+_PAGES = Struct("@2P6q3Pq5i4x")
+_APPEND = Struct("@P3q" + 5 * "P2q" + "5P2q4i")
+_BOUNDS = Struct("@P3q3Pq")
+_SELECT = Struct("@P3qP2q4PQ2P5i4x")
+_ATTENTION = Struct("@P3q" + 2 * "P2q" + "5PQ2Pq3if")
+_NO_HEADS = (0, 0, 0)
 
 TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float8_e4m3fn: 2}
 MAX_DIM = 256
@@ -62,12 +72,14 @@ class PagedKVCache:
         self.k, self.v, self.k_scale, self.v_scale, self.bounds = k, v, k_scale, v_scale, bounds
         self.num_pages, self.page_size, self.n_kv_heads, self.head_dim = k.shape
         self.dtype, self.device = k.dtype, k.device
-        ptr = lambda t: t.data_ptr() if t is not None else None
-        self._desc = _lib.KVPages(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), v.stride(0), v.stride(1),
-                                  v.stride(2), ptr(k_scale), ptr(v_scale), ptr(bounds), *k.shape, TYPES[k.dtype],
-                                  TYPES[bounds.dtype] if bounds is not None else 0)
-        self._ref = ctypes.byref(self._desc)
+        ptr = lambda t: t.data_ptr() if t is not None else 0
+        self._packed = _PAGES.pack(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), v.stride(0), v.stride(1),
+                                   v.stride(2), ptr(k_scale), ptr(v_scale), ptr(bounds), *k.shape, TYPES[k.dtype],
+                                   TYPES[bounds.dtype] if bounds is not None else 0)
+        self._index = k.get_device()
         self._status = _lib.status_word(self.device).data_ptr()
+        self._query_types = (torch.bfloat16, torch.float16) if k.dtype == torch.float8_e4m3fn else (k.dtype,)
+        self._attention_scratch = {}                          # bytes by number of query heads
 
     @classmethod
     def allocate(cls, num_pages: int, page_size: int, n_kv_heads: int, head_dim: int, dtype=torch.bfloat16, device=None,
@@ -116,42 +128,47 @@ def _check_pool(k, v, k_scale, v_scale, bounds) -> None:
         raise ValueError("the tensors of a cache must be on one device")
 
 
-def _int32(t: torch.Tensor, shape, what: str, device) -> int:
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"{what} must be a contiguous int32 tensor of shape {shape} on {device}")
+def _int32(t: torch.Tensor, shape, what: str, index: int) -> int:
+    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous() or t.get_device() != index:
+        raise ValueError(f"{what} must be a contiguous int32 tensor of shape {shape} on cuda:{index}")
     return t.data_ptr()
 
 
-def _table(cache: PagedKVCache, block_table: torch.Tensor) -> "_lib.KVTable":
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.device != cache.device \
-            or block_table.shape[1] < 1 or (block_table.stride(1) != 1 and block_table.shape[1] > 1):
-        raise ValueError(f"block_table must be an int32 [sequences, pages] tensor on {cache.device} with unit column stride")
-    seqs, width = block_table.shape
+def _table(cache: PagedKVCache, block_table: torch.Tensor):
+    """(pointer, row stride, sequences, pages a sequence)"""
+    shape = block_table.shape
+    if block_table.dtype is not torch.int32 or len(shape) != 2 or block_table.get_device() != cache._index or shape[1] < 1:
+        raise ValueError(f"block_table must be an int32 [sequences, pages] tensor on {cache.device}")
+    seqs, width = shape
+    row, col = block_table.stride()
+    if (col != 1 and width > 1) or row < 0:
+        raise ValueError("block_table must have a unit column stride")
     if width * cache.page_size > MAX_TOKENS:
         raise ValueError(f"a block table can hold at most {MAX_TOKENS} tokens per sequence")
-    return _lib.KVTable(block_table.data_ptr(), block_table.stride(0), seqs, width)
+    return block_table.data_ptr(), row, seqs, width
 
 
-def _heads(cache: PagedKVCache, t: torch.Tensor, rows: int, heads: Optional[int], dtype, what: str) -> "_lib.Heads":
-    if t.dim() != 3 or t.shape[0] != rows or t.shape[2] != cache.head_dim or (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{what} must be a [{rows}, {'heads' if heads is None else heads}, {cache.head_dim}] tensor")
-    if t.device != cache.device:
+def _heads(cache: PagedKVCache, t: torch.Tensor, rows: int, heads: int, dtype, what: str):
+    """(pointer, row stride, head stride) of a [rows, heads, head_dim] tensor"""
+    if t.shape != (rows, heads, cache.head_dim):
+        raise ValueError(f"{what} must be a [{rows}, {heads}, {cache.head_dim}] tensor")
+    if t.get_device() != cache._index:
         if not t.is_cuda:
             raise _lib.WushB200Error("wush_b200 ops need CUDA tensors; there is no CPU fallback")
         raise ValueError(f"{what} is on {t.device}, the cache on {cache.device}")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise ValueError(f"{what} must be {dtype}")
-    s = t.stride()
+    row, head, channel = t.stride()
     p = t.data_ptr()
-    if s[2] != 1 or p & 15 or s[0] & 7 or s[1] & 7:
+    if channel != 1 or p & 15 or row & 7 or head & 7:
         raise ValueError(f"{what}: channels must be contiguous, and rows and heads start on 16-byte boundaries")
-    return _lib.Heads(p, s[0], s[1])
+    return p, row, head
 
 
 def _query_type(cache: PagedKVCache, t: torch.Tensor, what: str):
     """Element type of a call's queries, keys and values: that of 16-bit pages, either 16-bit type for 8-bit pages."""
-    if t.dtype not in (torch.bfloat16, torch.float16) or (cache.dtype != torch.float8_e4m3fn and t.dtype != cache.dtype):
-        raise ValueError(f"{what} must be {'bfloat16 or float16' if cache.dtype == torch.float8_e4m3fn else cache.dtype}")
+    if t.dtype not in cache._query_types:
+        raise ValueError(f"{what} must be " + " or ".join(str(x) for x in cache._query_types))
     return t.dtype
 
 
@@ -161,12 +178,33 @@ def _q_heads(cache: PagedKVCache, q: torch.Tensor) -> int:
     return q.shape[1]
 
 
+def _on_its_device(op):
+    """Run an operator with the cache's device as the current one (switching costs more than a small call, so only when
+    it is another)."""
+    @functools.wraps(op)
+    def run(*args, **kwargs):
+        cache = kwargs.get("cache")
+        if cache is None:
+            cache = next(a for a in args if isinstance(a, PagedKVCache))
+        if torch.cuda.current_device() == cache._index:
+            return op(*args, **kwargs)
+        with torch.cuda.device(cache._index):
+            return op(*args, **kwargs)
+    return run
+
+
+def _stream(cache: PagedKVCache) -> int:
+    # torch.cuda.current_stream(...).cuda_stream without the two objects in between
+    return torch._C._cuda_getCurrentRawStream(cache._index)
+
+
 def _finish(cache: PagedKVCache, rc: int, what: str) -> None:
     _lib.check(rc, what)
     if _lib.CHECK_EVERY_OP:
         _lib.check_status(cache.device, what)
 
 
+@_on_its_device
 def paged_kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, seq_ids: torch.Tensor,
                     positions: torch.Tensor, q: Optional[torch.Tensor] = None, rope: Optional[torch.Tensor] = None,
                     interleaved: bool = False, q_out: Optional[torch.Tensor] = None,
@@ -185,13 +223,13 @@ def paged_kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, block
                the rotated keys and may be ``k``.  Otherwise outputs must not overlap inputs.
     """
     typ = _query_type(cache, k, "k")
-    rows = k.shape[0] if k.dim() == 3 else -1
-    hk = _heads(cache, k, rows, cache.n_kv_heads, typ, "k")
-    hv = _heads(cache, v, rows, cache.n_kv_heads, typ, "v")
+    rows, kv_heads = k.shape[0], cache.n_kv_heads
+    hk = _heads(cache, k, rows, kv_heads, typ, "k")
+    hv = _heads(cache, v, rows, kv_heads, typ, "v")
     table = _table(cache, block_table)
-    ids = _int32(seq_ids, (rows,), "seq_ids", cache.device)
-    pos = _int32(positions, (rows,), "positions", cache.device)
-    hq = hqo = hko = None
+    ids = _int32(seq_ids, (rows,), "seq_ids", cache._index)
+    pos = _int32(positions, (rows,), "positions", cache._index)
+    hq = hqo = hko = _NO_HEADS
     n_heads = 0
     if q is not None:
         n_heads = _q_heads(cache, q)
@@ -202,10 +240,10 @@ def paged_kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, block
     elif q_out is not None:
         raise ValueError("q_out goes with q")
     if k_out is not None:
-        hko = _heads(cache, k_out, rows, cache.n_kv_heads, typ, "k_out")
-    rope_ptr, rope_rows, rotary = None, 0, 0
+        hko = _heads(cache, k_out, rows, kv_heads, typ, "k_out")
+    rope_ptr, rope_rows, rotary = 0, 0, 0
     if rope is not None:
-        if rope.dim() != 2 or rope.dtype != torch.float32 or not rope.is_contiguous() or rope.device != cache.device \
+        if rope.dim() != 2 or rope.dtype is not torch.float32 or not rope.is_contiguous() or rope.get_device() != cache._index \
                 or rope.data_ptr() % 16:
             raise ValueError(f"rope must be a contiguous float32 [positions, rotary_dim] tensor on {cache.device}")
         rope_rows, rotary = rope.shape
@@ -214,16 +252,14 @@ def paged_kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, block
         rope_ptr = rope.data_ptr()
     if rows == 0:
         return q_out
-    ref = ctypes.byref
-    with torch.cuda.device(cache.device):
-        rc = _lib.load().wush_kv_append(
-            cache._ref, ref(table), TYPES[typ], ref(hq) if hq is not None else None, n_heads,
-            ref(hqo) if hqo is not None else None, ref(hk), ref(hv), ref(hko) if hko is not None else None, rope_ptr, rope_rows,
-            rotary, int(interleaved), ids, pos, rows, cache._status, torch.cuda.current_stream().cuda_stream)
+    rc = _lib.load().wush_kv_append(cache._packed + _APPEND.pack(
+        *table, *hq, *hqo, *hk, *hv, *hko, rope_ptr, ids, pos, cache._status, _stream(cache), rows, rope_rows, TYPES[typ], n_heads,
+        rotary, interleaved))
     _finish(cache, rc, "wush_kv_append")
     return q_out
 
 
+@_on_its_device
 def paged_kv_bounds(cache: PagedKVCache, block_table: torch.Tensor, seq_lens: torch.Tensor, new_tokens: int = 1) -> None:
     """Recompute ``cache.bounds`` for the pages that hold the last ``new_tokens`` of the ``seq_lens`` tokens of every
     sequence: the smallest and the largest stored key of every channel over the page's filled rows (NaN if one is).
@@ -233,13 +269,12 @@ def paged_kv_bounds(cache: PagedKVCache, block_table: torch.Tensor, seq_lens: to
     if new_tokens < 0:
         raise ValueError("new_tokens must not be negative")
     table = _table(cache, block_table)
-    lens = _int32(seq_lens, (table.seqs,), "seq_lens", cache.device)
-    with torch.cuda.device(cache.device):
-        rc = _lib.load().wush_kv_bounds(cache._ref, ctypes.byref(table), lens, new_tokens, cache._status,
-                                        torch.cuda.current_stream().cuda_stream)
+    lens = _int32(seq_lens, (table[2],), "seq_lens", cache._index)
+    rc = _lib.load().wush_kv_bounds(cache._packed + _BOUNDS.pack(*table, lens, cache._status, _stream(cache), new_tokens))
     _finish(cache, rc, "wush_kv_bounds")
 
 
+@_on_its_device
 def paged_select_pages(q: torch.Tensor, cache: PagedKVCache, block_table: torch.Tensor, seq_lens: torch.Tensor, top: int,
                        sink: int = 1, recent: int = 1) -> Tuple[torch.Tensor, torch.Tensor]:
     """The pages worth attending to: (pages int32 [sequences, n_kv_heads, top], counts int32 [sequences, n_kv_heads]).
@@ -256,24 +291,24 @@ def paged_select_pages(q: torch.Tensor, cache: PagedKVCache, block_table: torch.
         raise ValueError("top must be at least 1 and at least sink + recent, which must not be negative")
     typ = _query_type(cache, q, "q")
     table = _table(cache, block_table)
+    _, _, seqs, width = table
     n_heads = _q_heads(cache, q)
-    hq = _heads(cache, q, table.seqs, n_heads, typ, "q")
-    lens = _int32(seq_lens, (table.seqs,), "seq_lens", cache.device)
-    pages = torch.empty(table.seqs, cache.n_kv_heads, top, dtype=torch.int32, device=cache.device)
-    counts = torch.empty(table.seqs, cache.n_kv_heads, dtype=torch.int32, device=cache.device)
-    if table.seqs == 0:
+    hq = _heads(cache, q, seqs, n_heads, typ, "q")
+    lens = _int32(seq_lens, (seqs,), "seq_lens", cache._index)
+    pages = torch.empty((seqs, cache.n_kv_heads, top), dtype=torch.int32, device=cache.device)
+    counts = torch.empty((seqs, cache.n_kv_heads), dtype=torch.int32, device=cache.device)
+    if seqs == 0:
         return pages, counts
-    lib = _lib.load()
-    with torch.cuda.device(cache.device):
-        nbytes = lib.wush_kv_select_workspace_bytes(table.seqs, cache.n_kv_heads, table.width)
-        work = _lib.gemm_workspace(cache.device, nbytes)
-        rc = lib.wush_kv_select_pages(cache._ref, ctypes.byref(table), TYPES[typ], ctypes.byref(hq), n_heads, lens, top, sink,
-                                      recent, pages.data_ptr(), counts.data_ptr(), work.data_ptr(), work.numel(), cache._status,
-                                      torch.cuda.current_stream().cuda_stream)
+    lib, stream = _lib.load(), _stream(cache)
+    work = _lib.stream_workspace(cache._index, stream, lib.wush_kv_select_workspace_bytes(seqs, cache.n_kv_heads, width))
+    rc = lib.wush_kv_select_pages(cache._packed + _SELECT.pack(
+        *table, *hq, lens, pages.data_ptr(), counts.data_ptr(), work.data_ptr(), work.numel(), cache._status, stream, TYPES[typ],
+        n_heads, top, sink, recent))
     _finish(cache, rc, "wush_kv_select_pages")
     return pages, counts
 
 
+@_on_its_device
 def paged_decode_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.Tensor, seq_lens: torch.Tensor,
                            scale: Optional[float] = None, window: int = 0, pages: Optional[torch.Tensor] = None,
                            counts: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
@@ -292,12 +327,13 @@ def paged_decode_attention(q: torch.Tensor, cache: PagedKVCache, block_table: to
     """
     typ = _query_type(cache, q, "q")
     table = _table(cache, block_table)
+    seqs = table[2]
     n_heads = _q_heads(cache, q)
-    hq = _heads(cache, q, table.seqs, n_heads, typ, "q")
-    lens = _int32(seq_lens, (table.seqs,), "seq_lens", cache.device)
+    hq = _heads(cache, q, seqs, n_heads, typ, "q")
+    lens = _int32(seq_lens, (seqs,), "seq_lens", cache._index)
     if window < 0:
         raise ValueError("window must not be negative")
-    top, pages_ptr, counts_ptr = 0, None, None
+    top, pages_ptr, counts_ptr = 0, 0, 0
     if (pages is None) != (counts is None):
         raise ValueError("pages and counts go together")
     if pages is not None:
@@ -306,21 +342,20 @@ def paged_decode_attention(q: torch.Tensor, cache: PagedKVCache, block_table: to
         if pages.dim() != 3 or pages.shape[2] < 1 or pages.shape[2] * cache.page_size > MAX_TOKENS:
             raise ValueError(f"pages must be [sequences, n_kv_heads, top] and hold at most {MAX_TOKENS} tokens")
         top = pages.shape[2]
-        pages_ptr = _int32(pages, (table.seqs, cache.n_kv_heads, top), "pages", cache.device)
-        counts_ptr = _int32(counts, (table.seqs, cache.n_kv_heads), "counts", cache.device)
+        pages_ptr = _int32(pages, (seqs, cache.n_kv_heads, top), "pages", cache._index)
+        counts_ptr = _int32(counts, (seqs, cache.n_kv_heads), "counts", cache._index)
     if out is None:
-        out = torch.empty(q.shape, dtype=typ, device=cache.device)
-    ho = _heads(cache, out, table.seqs, n_heads, typ, "out")
-    lse = torch.empty(table.seqs, n_heads, dtype=torch.float32, device=cache.device) if return_lse else None
-    if table.seqs > 0:
-        lib = _lib.load()
-        with torch.cuda.device(cache.device):
-            nbytes = lib.wush_kv_attention_workspace_bytes(cache._ref, n_heads)
-            work = _lib.gemm_workspace(cache.device, nbytes) if nbytes else None
-            rc = lib.wush_kv_attention(
-                cache._ref, ctypes.byref(table), TYPES[typ], ctypes.byref(hq), n_heads, ctypes.byref(ho),
-                lse.data_ptr() if return_lse else None, lens, cache.head_dim ** -0.5 if scale is None else scale, window,
-                pages_ptr, counts_ptr, top, work.data_ptr() if work is not None else None,
-                work.numel() if work is not None else 0, cache._status, torch.cuda.current_stream().cuda_stream)
+        out = torch.empty((seqs, n_heads, cache.head_dim), dtype=typ, device=cache.device)
+    ho = _heads(cache, out, seqs, n_heads, typ, "out")
+    lse = torch.empty((seqs, n_heads), dtype=torch.float32, device=cache.device) if return_lse else None
+    if seqs > 0:
+        lib, stream = _lib.load(), _stream(cache)
+        nbytes = cache._attention_scratch.get(n_heads)
+        if nbytes is None:
+            nbytes = cache._attention_scratch[n_heads] = lib.wush_kv_attention_workspace_bytes(cache._packed, n_heads)
+        work = _lib.stream_workspace(cache._index, stream, nbytes)
+        rc = lib.wush_kv_attention(cache._packed + _ATTENTION.pack(
+            *table, *hq, *ho, lse.data_ptr() if return_lse else 0, lens, pages_ptr, counts_ptr, work.data_ptr(), work.numel(),
+            cache._status, stream, window, TYPES[typ], n_heads, top, cache.head_dim ** -0.5 if scale is None else scale))
         _finish(cache, rc, "wush_kv_attention")
     return (out, lse) if return_lse else out
