@@ -60,8 +60,10 @@ def lse_tolerance(lse, n, d, mass):
 
 def scores(q, low, high):
     """float64 score of one page for one key head: q [g, d], low and high [d]."""
+    if not bool((low.isfinite() & high.isfinite()).all()):
+        return math.inf
     s = torch.maximum(q * low, q * high).sum(1)
-    return float(torch.where(s.isnan(), torch.full_like(s, math.inf), s).max())
+    return float(torch.where(s.isfinite(), s, torch.full_like(s, math.inf)).max())
 
 
 def select(score, top, sink, recent):

@@ -404,16 +404,39 @@ def test_selection_takes_the_lowest_page_among_equals_and_nan_first():
     for lp, x in ((1500, 2.0), (700, 2.0), (1999, -5.0), (1998, math.nan)):
         s.cache.bounds[int(s.table[0, lp])] = x
     s.cache.bounds[int(s.table[0, 3])] = -0.0
+    s.cache.bounds[int(s.table[0, 1997]), 0, 0, 5] = -math.inf      # only the lower bound, which a positive query does not use
     pages, counts = paged_kv.paged_select_pages(q, s.cache, s.table, s.seq_lens, 6, sink=0, recent=0)
-    assert pages[0, 0].tolist() == [0, 1, 2, 700, 1500, 1998] and int(counts[0, 0]) == 6
+    assert pages[0, 0].tolist() == [0, 1, 700, 1500, 1997, 1998] and int(counts[0, 0]) == 6
     pages, _ = paged_kv.paged_select_pages(q, s.cache, s.table, s.seq_lens, 6, sink=2, recent=1)
-    assert pages[0, 0].tolist() == [0, 1, 700, 1500, 1998, 1999]
+    assert pages[0, 0].tolist() == [0, 1, 700, 1997, 1998, 1999]
     pages, _ = paged_kv.paged_select_pages(q, s.cache, s.table, s.seq_lens, 5, sink=2, recent=3)
     assert pages[0, 0].tolist() == [0, 1, 1997, 1998, 1999]
     pages, _ = paged_kv.paged_select_pages(q, s.cache, s.table, s.seq_lens, 1999, sink=0, recent=0)
     assert pages[0, 0].tolist() == list(range(1999))
     pages, counts = paged_kv.paged_select_pages(q, s.cache, s.table, s.seq_lens, 2100)
     assert pages[0, 0].tolist() == list(range(2000)) + [-1] * 100 and int(counts[0, 0]) == 2000
+
+
+@pytest.mark.parametrize("width", [1000, 1025, 3000, 8192, 8193, 20000])
+def test_selection_over_many_pages(width):
+    """Widths around the sizes at which the kernel changes its block, with many equal scores across the border."""
+    from wush_b200 import paged_kv
+    from wush_b200.paged_kv import PagedKVCache
+    g, dev = _gen(width), _dev()
+    lens = [width, width - 7, width // 2]
+    pool = PagedKVCache.allocate(width, 1, 1, 8, device=dev, bounds=True)
+    pool.bounds.copy_(torch.randint(-3, 4, pool.bounds.shape, generator=g, device=dev).sort(dim=2).values.to(BF))
+    table = torch.stack([torch.randperm(width, generator=g, device=dev) for _ in lens]).to(torch.int32)
+    q = torch.randint(-2, 3, (3, 2, 8), generator=g, device=dev).to(BF)
+    seq_lens = torch.tensor(lens, dtype=torch.int32, device=dev)
+    for top, sink, recent in ((1, 0, 0), (77, 1, 1), (width // 3, 5, 0)):
+        pages, counts = paged_kv.paged_select_pages(q, pool, table, seq_lens, top, sink=sink, recent=recent)
+        for b, n in enumerate(lens):
+            bound = pool.bounds[table[b, :n].long(), 0].double()
+            score = torch.maximum(q[b].double()[:, None] * bound[:, 0], q[b].double()[:, None] * bound[:, 1]).sum(2).amax(0)
+            want = ref.select(score.tolist(), top, sink, recent)
+            assert int(counts[b, 0]) == len(want) and pages[b, 0, : len(want)].tolist() == want, (b, top)
+    _status_clear()
 
 
 def test_selection_close_scores_do_not_depend_on_the_order_of_the_sum():

@@ -138,119 +138,293 @@ __global__ void __launch_bounds__(256) bounds_kernel(const wush_kv_pages kv, con
 }
 
 // ---- selection -----------------------------------------------------------------------------------------------------
-// A score as a 64-bit key with the same order; NaN counts as +infinity.
+// A score as a 64-bit key with the same order; one that is not finite counts as +infinity.
 __device__ __forceinline__ unsigned long long score_key(double s) {
-  if (s != s) s = __longlong_as_double(0x7ff0000000000000ll);
+  if (!(fabs(s) <= 1.7976931348623157e308)) return ~0ull;
   const long long b = __double_as_longlong(s + 0.0);       // -0 + 0 = +0: equal numbers, equal keys
   return b < 0 ? ~(unsigned long long)b : (unsigned long long)b | 0x8000000000000000ull;
 }
 
-// One warp per (sequence, head, page): keys of the scores.
-template <typename T, typename B>
-__global__ void __launch_bounds__(256) score_kernel(const wush_kv_pages kv, const wush_kv_table table, const wush_heads q,
-                                                    int group, const int32_t* seq_lens, int top, unsigned long long* keys,
-                                                    int* status) {
-  const int lane = threadIdx.x & 31;
-  const int64_t warps = (int64_t)gridDim.x * (blockDim.x >> 5), total = table.seqs * kv.heads * table.width;
-  for (int64_t w = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); w < total; w += warps) {
-    const int lp = (int)(w % table.width), head = (int)(w / table.width % kv.heads);
-    const int64_t seq = w / table.width / kv.heads;
-    const int len = clamp_length(seq_lens[seq], table.width * kv.page_size, status);
-    const int n = (len + kv.page_size - 1) / kv.page_size;
-    if (lp >= n || n <= top) continue;
-    const int page = lookup_page(table, seq, lp, kv.num_pages, status);
-    unsigned long long best = 0;
-    if (page >= 0) {
-      const B* bound = reinterpret_cast<const B*>(kv.bounds) + ((int64_t)page * kv.heads + head) * 2 * kv.dim;
-      for (int g = 0; g < group; ++g) {
-        const T* row = reinterpret_cast<const T*>(q.data) + seq * q.row + (int64_t)(head * group + g) * q.head;
-        double s = 0.0;
-        for (int c = lane * 8; c < kv.dim; c += 256) {
-          float x[8], lo[8], hi[8];
-          load8(row + c, x);
-          load8(bound + c, lo);
-          load8(bound + kv.dim + c, hi);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) s += (double)max_nan(x[j] * lo[j], x[j] * hi[j]);   // 16-bit factors: exact products
-        }
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        const unsigned long long key = score_key(s);
-        best = best < key ? key : best;
-      }
-    }
-    if (lane == 0) keys[w] = best;
-  }
+__device__ __forceinline__ void mma_f64(double (&d)[2], double a, double b) {
+  asm("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0,%1}, {%2}, {%3}, {%0,%1};\n" : "+d"(d[0]), "+d"(d[1]) : "d"(a), "d"(b));
 }
 
-// One block per (sequence, head).  The threshold key is built bit by bit from the top (the largest key that at least
-// `want` pages reach), then the pages above it and the first ones equal to it are written in order.
-__global__ void __launch_bounds__(1024) select_kernel(int page_size, int64_t width, int heads, const int32_t* seq_lens,
-                                                      const unsigned long long* keys, int top, int sink, int recent,
-                                                      int32_t* pages, int32_t* counts) {
-  __shared__ int warp_sum[32];
-  const int tid = threadIdx.x, lane = tid & 31;
+// Keys of the scores: sum_d max(q_d lower_d, q_d upper_d) = sum_d q+_d upper_d + q-_d lower_d, with q+ and q- the positive and
+// negative parts: products [8 queries x 4 channels] . [4 channels x 8 pages] in 64 bits.  (A bound that is not finite makes
+// one of its two terms infinite or NaN whatever the query is.)  As in the attention, a product does not care which channel
+// is which, so a lane takes 8 neighbouring channels of a page with one load and feeds them to 8 products; the queries are
+// laid out to match in shared memory.  A block works on 64 pages of one (sequence, key head), 16 a warp.
+constexpr int SCORE_WARPS = 4, SCORE_PAGES = 16 * SCORE_WARPS;
+template <typename T, typename B>
+__global__ void __launch_bounds__(SCORE_WARPS * 32) score_kernel(const wush_kv_select_args a, int group, unsigned long long* keys) {
+  extern __shared__ double sm_q[];                           // [parts][channels / 32][8][8 queries][4]
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
+  const int d = a.kv.dim, steps = (d + 31) / 32;
+  const int blocks = (int)((a.table.width + SCORE_PAGES - 1) / SCORE_PAGES);
+  const int64_t entry = blockIdx.x / blocks, seq = entry / a.kv.heads;
+  const int head = (int)(entry % a.kv.heads), page0 = (int)(blockIdx.x % blocks) * SCORE_PAGES;
+  const int len = clamp_length(a.seq_lens[seq], a.table.width * a.kv.page_size, a.status);
+  const int n = (len + a.kv.page_size - 1) / a.kv.page_size;
+  if (page0 >= n || n <= a.top) return;
+  const B* bound[2];                                         // of the lane's two pages
+  bool known[2];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int lp = page0 + warp * 16 + x * 8 + r;
+    const int page = lp < n ? lookup_page(a.table, seq, lp, a.kv.num_pages, a.status) : -1;
+    known[x] = page >= 0;
+    bound[x] = reinterpret_cast<const B*>(a.kv.bounds) + ((int64_t)max(page, 0) * a.kv.heads + head) * 2 * d;
+  }
+  double best[2][2] = {{-INFINITY, -INFINITY}, {-INFINITY, -INFINITY}};
+  bool bad[2][2] = {{false, false}, {false, false}};         // a score that is not finite
+  for (int g0 = 0; g0 < group; g0 += 8) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < steps * 32; i += SCORE_WARPS * 32) {   // 8 channels of one query
+      const int row = i / (steps * 4), piece = i % (steps * 4);
+      float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (g0 + row < group && piece * 8 < d)
+        load8(reinterpret_cast<const T*>(a.q.data) + seq * a.q.row + (int64_t)(head * group + g0 + row) * a.q.head + piece * 8, x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        double* at = sm_q + ((piece >> 2) * 8 + e) * 32 + row * 4 + (piece & 3);
+        at[0] = x[e] > 0.0f ? (double)x[e] : 0.0;
+        at[steps * 256] = x[e] > 0.0f ? 0.0 : (double)x[e];  // (a NaN query lands here)
+      }
+    }
+    __syncthreads();
+    double s[2][2] = {{0.0, 0.0}, {0.0, 0.0}};
+    for (int j = 0; j < steps; ++j) {
+      const int ch = (j * 4 + c) * 8;
+      float lo[2][8], hi[2][8];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        if (known[x] && ch < d) {
+          load8(bound[x] + ch, lo[x]);
+          load8(bound[x] + d + ch, hi[x]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) lo[x][e] = hi[x][e] = 0.0f;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const double plus = sm_q[(j * 8 + e) * 32 + lane], minus = sm_q[steps * 256 + (j * 8 + e) * 32 + lane];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          mma_f64(s[x], plus, (double)hi[x][e]);
+          mma_f64(s[x], minus, (double)lo[x][e]);
+        }
+      }
+    }
+    // the lane has query g0 + r and pages 2c, 2c + 1 of each 8
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        if (g0 + r >= group) continue;
+        bad[x][y] |= !(fabs(s[x][y]) <= 1.7976931348623157e308);
+        best[x][y] = fmax(best[x][y], s[x][y]);
+      }
+  }
+#pragma unroll
+  for (int x = 0; x < 2; ++x)
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      double top = best[x][y];
+      unsigned any = bad[x][y];
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) {
+        top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
+        any |= __shfl_xor_sync(0xffffffffu, any, o);
+      }
+      const bool known_page = __shfl_sync(0xffffffffu, known[x], (2 * c + y) * 4);
+      const int lp = page0 + warp * 16 + x * 8 + 2 * c + y;
+      // a page outside the pool comes last: the attention would leave it out
+      if (r == 0 && lp < n) keys[entry * a.table.width + lp] = !known_page ? 0 : (any ? ~0ull : score_key(top));
+    }
+}
+
+// Exclusive sums over `count` <= 256 numbers in shared memory, by one warp; returns the total.
+__device__ __forceinline__ int scan256(int* x, int count) {
+  const int lane = threadIdx.x & 31;
+  int mine[8], sum = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    mine[i] = sum;
+    sum += lane * 8 + i < count ? x[lane * 8 + i] : 0;
+  }
+  int before = sum;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += y;
+  }
+  const int total = __shfl_sync(0xffffffffu, before, 31);
+  before -= sum;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (lane * 8 + i < count) x[lane * 8 + i] = before + mine[i];
+  return total;
+}
+
+// One block per (sequence, key head).  A radix selection from the first bit in which the keys differ: 8 bits at a time the
+// keys that share the threshold's leading bits are counted by their next digit, until all of them are wanted or all bits are
+// known; the last of them are then taken in the order of their pages.  A thread holds every blockDim-th key, up to ROWS of
+// them (ROWS is 8, or 0 for more pages than that: then they are read again for every pass).
+template <int ROWS>
+__global__ void __launch_bounds__(1024) select_kernel(const wush_kv_select_args a, const unsigned long long* keys) {
+  __shared__ int hist[256];
+  __shared__ unsigned long long sm_low[32], sm_high[32];
+  __shared__ int sm_digit, sm_need, sm_count;
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5;
   const int64_t item = blockIdx.x;
-  const int len = (int)max((int64_t)0, min((int64_t)seq_lens[item / heads], width * page_size));
-  const int n = (len + page_size - 1) / page_size;
-  const unsigned long long* key = keys + item * width;
-  int32_t* out = pages + item * top;
+  const int len = (int)max((int64_t)0, min((int64_t)a.seq_lens[item / a.kv.heads], a.table.width * a.kv.page_size));
+  const int n = (len + a.kv.page_size - 1) / a.kv.page_size, top = a.top;
+  int32_t* out = a.pages + item * top;
   const int count = min(n, top);
-  if (tid == 0) counts[item] = count;
-  for (int i = count + tid; i < top; i += blockDim.x) out[i] = -1;
+  if (tid == 0) a.counts[item] = count;
+  for (int i = count + tid; i < top; i += threads) out[i] = -1;
   if (n <= top) {
-    for (int i = tid; i < n; i += blockDim.x) out[i] = i;
+    for (int i = tid; i < n; i += threads) out[i] = i;
     return;
   }
-  const int begin = sink, end = n - recent, want = top - sink - recent;
-  unsigned long long threshold = 0;
-  for (int bit = 63; bit >= 0; --bit) {
-    const unsigned long long trial = threshold | 1ull << bit;
-    int mine = 0;
-    for (int i = begin + tid; i < end; i += blockDim.x) mine += key[i] >= trial;
-    // every thread gets the sum
-    mine = __reduce_add_sync(0xffffffffu, mine);
-    if (lane == 0) warp_sum[tid >> 5] = mine;
-    __syncthreads();
-    const int sum = __reduce_add_sync(0xffffffffu, warp_sum[lane]);
-    __syncthreads();
-    if (sum >= want) threshold = trial;
+  const int begin = a.sink, end = n - a.recent;              // pages that compete
+  const unsigned long long* from = keys + item * a.table.width;
+  unsigned long long held[ROWS > 0 ? ROWS : 1];
+#pragma unroll
+  for (int j = 0; j < ROWS; ++j) {
+    const int i = j * threads + tid;
+    held[j] = i >= begin && i < end ? from[i] : 0;
   }
-  // pages in ascending order: those above the threshold, and the first of those equal to it that are still wanted
-  int above = 0;
-  for (int i = begin + tid; i < end; i += blockDim.x) above += key[i] > threshold;
-  above = __reduce_add_sync(0xffffffffu, above);
-  if (lane == 0) warp_sum[tid >> 5] = above;
-  __syncthreads();
-  const int ties = want - __reduce_add_sync(0xffffffffu, warp_sum[lane]);
-  __syncthreads();
-  __shared__ int taken_sum[32], equal_sum[32];
-  int taken = 0, equals = 0;                               // running totals over the pages before this round
-  for (int base = 0; base < n; base += blockDim.x) {
-    const int i = base + tid;
-    const bool forced = i < n && (i < begin || i >= end);
-    const unsigned long long x = i >= begin && i < end && want > 0 ? key[i] : 0;
-    const bool middle = i >= begin && i < end && want > 0;
-    const bool over = middle && x > threshold, equal = middle && x == threshold;
-    const unsigned em = __ballot_sync(0xffffffffu, equal);
-    if (lane == 0) equal_sum[tid >> 5] = __popc(em);
-    __syncthreads();
-    int before = equals, all_equal = 0;
-    for (int j = 0; j < 32; ++j) {
-      before += j < (tid >> 5) ? equal_sum[j] : 0;
-      all_equal += equal_sum[j];
+  const int rounds = ROWS > 0 ? ROWS : (n + threads - 1) / threads;
+  auto key_of = [&](int j) { return ROWS > 0 ? held[ROWS > 0 ? j : 0] : from[j * threads + tid]; };
+  auto competes = [&](int j) {
+    const int i = j * threads + tid;
+    return i >= begin && i < end;
+  };
+
+  // smallest and largest key: the bits before the first in which they differ need no passes
+  unsigned long long low = ~0ull, high = 0;
+#pragma unroll
+  for (int j = 0; j < rounds; ++j)
+    if (competes(j)) {
+      const unsigned long long k = key_of(j);
+      low = k < low ? k : low;
+      high = k > high ? k : high;
     }
-    const bool take = forced || over || (equal && before + __popc(em & ((1u << lane) - 1)) < ties);
-    const unsigned tm = __ballot_sync(0xffffffffu, take);
-    if (lane == 0) taken_sum[tid >> 5] = __popc(tm);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const unsigned long long x = __shfl_xor_sync(0xffffffffu, low, o), y = __shfl_xor_sync(0xffffffffu, high, o);
+    low = x < low ? x : low;
+    high = y > high ? y : high;
+  }
+  if (lane == 0) {
+    sm_low[warp] = low;
+    sm_high[warp] = high;
+  }
+  __syncthreads();
+  for (int w = 0; w < warps; ++w) {
+    low = sm_low[w] < low ? sm_low[w] : low;
+    high = sm_high[w] > high ? sm_high[w] : high;
+  }
+  int need = top - a.sink - a.recent, among = end - begin;   // wanted among the keys that match the prefix
+  int shift = low == high ? 0 : 64 - __clzll(low ^ high);    // bits of a key that are not known
+  unsigned long long prefix = shift == 64 ? 0 : high >> shift;
+  auto matches = [&](unsigned long long k) { return shift == 64 || k >> shift == prefix; };
+  while (need > 0 && need < among && shift > 0) {
+    const int bits = min(8, shift), next = shift - bits;
+    for (int i = tid; i < 256; i += threads) hist[i] = 0;
     __syncthreads();
-    int slot = taken, all_taken = 0;
-    for (int j = 0; j < 32; ++j) {
-      slot += j < (tid >> 5) ? taken_sum[j] : 0;
-      all_taken += taken_sum[j];
+#pragma unroll
+    for (int j = 0; j < rounds; ++j)
+      if (competes(j)) {
+        const unsigned long long k = key_of(j);
+        if (matches(k)) atomicAdd(&hist[(int)(k >> next) & ((1 << bits) - 1)], 1);
+      }
+    __syncthreads();
+    if (warp == 0) {                                         // the digit that the need-th largest key has
+      int mine[8], sum = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += mine[i] = hist[255 - (lane * 8 + i)];
+      int before = sum;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += y;
+      }
+      before -= sum;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (before < need && need <= before + mine[i]) {
+          sm_digit = 255 - (lane * 8 + i);
+          sm_need = need - before;
+          sm_count = mine[i];
+        }
+        before += mine[i];
+      }
     }
-    if (take) out[slot + __popc(tm & ((1u << lane) - 1))] = i;
-    taken += all_taken;
-    equals += all_equal;
+    __syncthreads();
+    prefix = (shift == 64 ? 0 : prefix << bits) | (unsigned)sm_digit;
+    need = sm_need;
+    among = sm_count;
+    shift = next;
+  }
+
+  // Take the keys above the prefix and the first `need` of those that match it; place them in the order of the pages, 8 rounds
+  // at a time.  hist holds the counts of (round, warp): 8 * 32 at most.
+  int taken_before = 0, equal_before = 0;
+  for (int j0 = 0; j0 < rounds; j0 += 8) {
+    unsigned equal = 0, take = 0;                            // one bit a round
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const int j = j0 + x, i = j * threads + tid;
+      const bool in = need > 0 && competes(j);
+      const unsigned long long k = in ? key_of(ROWS > 0 ? x : j) : 0;
+      equal |= (unsigned)(in && matches(k)) << x;
+      take |= (unsigned)((i < n && (i < begin || i >= end)) || (in && shift < 64 && k >> shift > prefix)) << x;
+    }
+    if (need < among) {                                      // not all that match: by rank
+      __syncthreads();
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const unsigned m = __ballot_sync(0xffffffffu, equal >> x & 1);
+        if (lane == 0) hist[x * warps + warp] = __popc(m);
+      }
+      __syncthreads();
+      if (warp == 0) {
+        const int total = scan256(hist, 8 * warps);
+        if (lane == 0) sm_count = total;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const unsigned m = __ballot_sync(0xffffffffu, equal >> x & 1);
+        if ((equal >> x & 1) && equal_before + hist[x * warps + warp] + __popc(m & ((1u << lane) - 1)) < need) take |= 1u << x;
+      }
+      equal_before += sm_count;
+    } else {
+      take |= equal;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const unsigned m = __ballot_sync(0xffffffffu, take >> x & 1);
+      if (lane == 0) hist[x * warps + warp] = __popc(m);
+    }
+    __syncthreads();
+    if (warp == 0) {
+      const int total = scan256(hist, 8 * warps);
+      if (lane == 0) sm_count = total;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const unsigned m = __ballot_sync(0xffffffffu, take >> x & 1);
+      if (take >> x & 1) out[taken_before + hist[x * warps + warp] + __popc(m & ((1u << lane) - 1))] = (j0 + x) * threads + tid;
+    }
+    taken_before += sm_count;
     __syncthreads();
   }
 }
@@ -338,19 +512,31 @@ extern "C" int wush_kv_select_pages(const wush_kv_select_args* args) {
   if (a.table.seqs * a.kv.heads > INT32_MAX) return WUSH_ERR_TOO_LARGE;
   if ((rc = require_sm100()) != 0) return rc;
   unsigned long long* keys = reinterpret_cast<unsigned long long*>(a.workspace);
-  const int64_t warps = a.table.seqs * a.kv.heads * a.table.width;
-  const unsigned grid = (unsigned)min((warps + 7) / 8, (int64_t)sm_count() * 32);
-  cudaStream_t stream = (cudaStream_t)a.stream;
-  auto go = [&](auto kern) {
-    kern<<<grid, 256, 0, stream>>>(a.kv, a.table, a.q, a.q_heads / a.kv.heads, a.seq_lens, a.top, keys, a.status);
-    return (int)cudaGetLastError();
-  };
+  const int64_t blocks = a.table.seqs * a.kv.heads * ((a.table.width + SCORE_PAGES - 1) / SCORE_PAGES);
+  if (blocks > INT32_MAX) return WUSH_ERR_TOO_LARGE;
+  // the kernels may be launched while the one before still runs, and wait for it before they read anything
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.stream = (cudaStream_t)a.stream;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(SCORE_WARPS * 32);
+  cfg.dynamicSmemBytes = (size_t)((a.kv.dim + 31) / 32) * 512 * sizeof(double);
+  auto go = [&](auto kern) { return (int)cudaLaunchKernelEx(&cfg, kern, a, a.q_heads / a.kv.heads, keys); };
   if (a.type == WUSH_TYPE_BF16)
     rc = a.kv.bounds_type == WUSH_TYPE_BF16 ? go(score_kernel<__nv_bfloat16, __nv_bfloat16>) : go(score_kernel<__nv_bfloat16, __half>);
   else
     rc = a.kv.bounds_type == WUSH_TYPE_BF16 ? go(score_kernel<__half, __nv_bfloat16>) : go(score_kernel<__half, __half>);
   if (rc != 0) return rc;
-  select_kernel<<<(unsigned)(a.table.seqs * a.kv.heads), 1024, 0, stream>>>(
-      a.kv.page_size, a.table.width, a.kv.heads, a.seq_lens, keys, a.top, a.sink, a.recent, a.pages, a.counts);
-  return (int)cudaGetLastError();
+  // 8 keys a thread in registers while that is enough
+  int threads = 128;
+  while (threads < 1024 && threads * 8 < a.table.width) threads *= 2;
+  cfg.gridDim = dim3((unsigned)(a.table.seqs * a.kv.heads));
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = 0;
+  if (threads * 8 >= a.table.width) return (int)cudaLaunchKernelEx(&cfg, select_kernel<8>, a, (const unsigned long long*)keys);
+  return (int)cudaLaunchKernelEx(&cfg, select_kernel<0>, a, (const unsigned long long*)keys);
 }
