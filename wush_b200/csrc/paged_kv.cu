@@ -1,4 +1,6 @@
 // Paged key-value cache: append with rotation, per-page bounds of the keys, selection of pages.
+#include <type_traits>
+
 #include "paged_kv.cuh"
 
 namespace wush {
@@ -7,133 +9,206 @@ namespace kv {
 // ---- append --------------------------------------------------------------------------------------------------------
 using AppendParams = wush_kv_append_args;
 
-// One thread per unit of 16 channels of a head (two chunks of 8 that are rotated against each other, or two chunks that
-// are only copied).
+// 16 bytes that are read once, past the L1 (not through the read-only path: the outputs may be the inputs)
+template <typename T>
+__device__ __forceinline__ uint4 load_once(const T* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void widen8(uint4 v, float (&x)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = to_float2<T>(w[i]);
+    x[2 * i] = f.x;
+    x[2 * i + 1] = f.y;
+  }
+}
+
+// One block per row.  A thread has one unit of 16 channels (two chunks of 8 that are turned against each other, or two that
+// are only copied) of every `lanes`-th head, so that the angles of its unit are loaded once for all of them; BATCH heads are
+// loaded before the first is turned.  A pure pass over memory: q, k and v once in, once out.
+constexpr int APPEND_BATCH = 5, APPEND_THREADS = 128;
 template <typename T, typename C>
-__global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
-  const int d = p.kv.dim, turned = p.rotary >> 4;
-  const int per_head = turned + ((d - p.rotary + 15) >> 4), per_value = (d + 15) >> 4;
-  const int rotated_heads = p.q_heads + p.kv.heads;
-  const int64_t per_row = (int64_t)rotated_heads * per_head + (int64_t)p.kv.heads * per_value;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < p.rows * per_row; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t row = i / per_row;
-    int u = (int)(i - row * per_row);
+__global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendParams p) {
+  const int d = p.kv.dim, units = (d + 15) >> 4, lanes = APPEND_THREADS / units, turned = p.rotary >> 4;
+  const int u = threadIdx.x % units, lane = threadIdx.x / units;
+  if (lane >= lanes) return;
+  const bool turn = u < turned;                              // (of q and k; the rotary channels are whole units)
+  const int ca = !turn ? u * 16 : (p.interleaved ? u * 16 : u * 8), cb = !turn || p.interleaved ? ca + 8 : ca + p.rotary / 2;
+  const int q_heads = p.q_heads, all_heads = q_heads + 2 * p.kv.heads;
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const int seq = p.seq_ids[row], pos = p.positions[row];
     if (seq < 0 || pos < 0) continue;
     if (seq >= p.table.seqs || pos >= p.table.width * p.kv.page_size || (p.rope && pos >= p.rope_rows)) {
       report_index(p.status);
       continue;
     }
-    const int lp = pos / p.kv.page_size;
+    const int lp = pos / p.kv.page_size, at = pos - lp * p.kv.page_size;
     const int page = lookup_page(p.table, seq, lp, p.kv.num_pages, p.status);
     if (page < 0) continue;
-    const int at = pos - lp * p.kv.page_size;
-    const bool value = u >= rotated_heads * per_head;
-    if (value) u -= rotated_heads * per_head;
-    int head = u / (value ? per_value : per_head);
-    u -= head * (value ? per_value : per_head);
-    const bool query = !value && head < p.q_heads;
-    if (!value && !query) head -= p.q_heads;
-    int ca, cb;                                             // first channels of the two chunks
-    const bool turn = !value && u < turned;
+    float cosine[8], sine[8];
     if (turn) {
-      ca = p.interleaved ? u * 16 : u * 8;
-      cb = p.interleaved ? ca + 8 : ca + p.rotary / 2;
-    } else {
-      ca = value ? u * 16 : p.rotary + (u - turned) * 16;
-      cb = ca + 8;
-    }
-    const wush_heads& src = value ? p.v : (query ? p.q : p.k);
-    const T* in = reinterpret_cast<const T*>(src.data) + row * src.row + head * src.head;
-    const bool two = cb < d;
-    float a[8], b[8];
-    load8(in + ca, a);
-    if (two) load8(in + cb, b);
-    if (turn) {
-      const float* c = p.rope + (int64_t)pos * p.rotary + u * 8;
-      const float* s = c + p.rotary / 2;
+      const float4* c = reinterpret_cast<const float4*>(p.rope + (int64_t)pos * p.rotary + u * 8);
+      const float4* s = c + p.rotary / 8;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float cj = c[j], sj = s[j];
-        float& x = p.interleaved ? (j < 4 ? a[2 * j] : b[2 * j - 8]) : a[j];
-        float& y = p.interleaved ? (j < 4 ? a[2 * j + 1] : b[2 * j - 7]) : b[j];
-        const float nx = __fsub_rn(__fmul_rn(x, cj), __fmul_rn(y, sj));
-        const float ny = __fadd_rn(__fmul_rn(y, cj), __fmul_rn(x, sj));
-        x = nx;
-        y = ny;
+      for (int i = 0; i < 2; ++i) {
+        const float4 x = __ldg(c + i), y = __ldg(s + i);
+        cosine[4 * i] = x.x, cosine[4 * i + 1] = x.y, cosine[4 * i + 2] = x.z, cosine[4 * i + 3] = x.w;
+        sine[4 * i] = y.x, sine[4 * i + 1] = y.y, sine[4 * i + 2] = y.z, sine[4 * i + 3] = y.w;
       }
     }
-    if (query) {
-      T* o = reinterpret_cast<T*>(p.q_out.data) + row * p.q_out.row + head * p.q_out.head;
-      store8(o + ca, a);
-      if (two) store8(o + cb, b);
-      continue;
-    }
-    if (!value && p.k_out.data) {
-      T* o = reinterpret_cast<T*>(p.k_out.data) + row * p.k_out.row + head * p.k_out.head;
-      store8(o + ca, a);
-      if (two) store8(o + cb, b);
-    }
-    C* o = value ? reinterpret_cast<C*>(p.kv.v) + page * p.kv.v_page + at * p.kv.v_row + head * p.kv.v_head
-                 : reinterpret_cast<C*>(p.kv.k) + page * p.kv.k_page + at * p.kv.k_row + head * p.kv.k_head;
-    if (sizeof(C) == 1) {
-      const float scale = value ? p.kv.v_scale[head] : p.kv.k_scale[head];
+    for (int h0 = lane; h0 < all_heads; h0 += lanes * APPEND_BATCH) {
+      uint4 in[APPEND_BATCH][2];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        a[j] = __fdiv_rn(a[j], scale);
-        b[j] = __fdiv_rn(b[j], scale);
+      for (int i = 0; i < APPEND_BATCH; ++i) {
+        const int h = h0 + i * lanes;
+        if (h >= all_heads) continue;
+        const bool value = h >= q_heads + p.kv.heads;
+        const wush_heads& src = h < q_heads ? p.q : (value ? p.v : p.k);
+        const int head = h < q_heads ? h : (h - q_heads) % p.kv.heads;
+        const T* from = reinterpret_cast<const T*>(src.data) + row * src.row + head * src.head;
+        const int a = value ? u * 16 : ca, b = value ? u * 16 + 8 : cb;
+        in[i][0] = load_once(from + a);
+        in[i][1] = b < d ? load_once(from + b) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < APPEND_BATCH; ++i) {
+        const int h = h0 + i * lanes;
+        if (h >= all_heads) continue;
+        const bool query = h < q_heads, value = h >= q_heads + p.kv.heads;
+        const int head = query ? h : (h - q_heads) % p.kv.heads;
+        const int ac = value ? u * 16 : ca, bc = value ? u * 16 + 8 : cb;
+        const bool two = bc < d;
+        float a[8], b[8];
+        widen8<T>(in[i][0], a);
+        widen8<T>(in[i][1], b);
+        if (turn && !value) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            float& x = p.interleaved ? (j < 4 ? a[2 * j] : b[2 * j - 8]) : a[j];
+            float& y = p.interleaved ? (j < 4 ? a[2 * j + 1] : b[2 * j - 7]) : b[j];
+            const float nx = __fsub_rn(__fmul_rn(x, cosine[j]), __fmul_rn(y, sine[j]));
+            const float ny = __fadd_rn(__fmul_rn(y, cosine[j]), __fmul_rn(x, sine[j]));
+            x = nx;
+            y = ny;
+          }
+        }
+        if (query || (!value && p.k_out.data)) {
+          const wush_heads& dst = query ? p.q_out : p.k_out;
+          T* o = reinterpret_cast<T*>(dst.data) + row * dst.row + head * dst.head;
+          store8(o + ac, a);
+          if (two) store8(o + bc, b);
+        }
+        if (query) continue;
+        C* o = value ? reinterpret_cast<C*>(p.kv.v) + page * p.kv.v_page + at * p.kv.v_row + head * p.kv.v_head
+                     : reinterpret_cast<C*>(p.kv.k) + page * p.kv.k_page + at * p.kv.k_row + head * p.kv.k_head;
+        if (sizeof(C) == 1) {
+          const float scale = value ? p.kv.v_scale[head] : p.kv.k_scale[head];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            a[j] = __fdiv_rn(a[j], scale);
+            b[j] = __fdiv_rn(b[j], scale);
+          }
+        }
+        store8(o + ac, a);
+        if (two) store8(o + bc, b);
       }
     }
-    store8(o + ca, a);
-    if (two) store8(o + cb, b);
   }
 }
 
 // ---- bounds --------------------------------------------------------------------------------------------------------
-// minimum / maximum that keep a NaN
-__device__ __forceinline__ float min_nan(float a, float b) {
-  float r;
-  asm("min.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b));
+// Packed minimum and maximum that keep a NaN, of bf16 pairs (bf16 pages) or fp16 pairs (fp16 pages, and E4M3 values widened).
+template <typename C>
+__device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if (std::is_same<C, __nv_bfloat16>::value) asm("min.NaN.bf16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
+  else asm("min.NaN.f16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b));
+template <typename C>
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if (std::is_same<C, __nv_bfloat16>::value) asm("max.NaN.bf16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
+  else asm("max.NaN.f16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
 
-// One warp per (sequence, page, head), lanes over the chunks of 8 channels.
+// One warp per (sequence, page, head); a lane takes 16 bytes of every n-th row, 8 rows under way at a time.
+constexpr int BOUNDS_ROWS = 8;
 template <typename C, typename B>
 __global__ void __launch_bounds__(256) bounds_kernel(const wush_kv_pages kv, const wush_kv_table table, const int32_t* seq_lens,
                                                      int64_t new_tokens, int64_t most, int* status) {
+  constexpr int CH = 16 / (int)sizeof(C), PAIRS = CH / 2;    // channels of a lane
   const int lane = threadIdx.x & 31;
+  const int across = (kv.dim + CH - 1) / CH, down = 32 / across;   // lanes of a row, rows of a warp
+  const int piece = lane % across, row0 = lane / across;
   const int64_t warps = (int64_t)gridDim.x * (blockDim.x >> 5), total = table.seqs * most * kv.heads;
   for (int64_t w = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); w < total; w += warps) {
-    const int head = (int)(w % kv.heads);
-    const int64_t seq = w / kv.heads / most;
+    const int64_t slot = w / kv.heads, seq = slot / most;
+    const int head = (int)(w - slot * kv.heads);
     const int len = clamp_length(seq_lens[seq], table.width * kv.page_size, status);
     const int64_t first = len > new_tokens ? len - new_tokens : 0;
-    const int64_t lp = first / kv.page_size + w / kv.heads % most;
+    const int64_t lp = first / kv.page_size + (slot - seq * most);
     if (lp * kv.page_size >= len) continue;
     const int page = lookup_page(table, seq, (int)lp, kv.num_pages, status);
     if (page < 0) continue;
     const int rows = (int)min((int64_t)kv.page_size, len - lp * kv.page_size);
-    if (lane * 8 >= kv.dim) continue;
-    const C* k = reinterpret_cast<const C*>(kv.k) + page * kv.k_page + head * kv.k_head + lane * 8;
-    float lo[8], hi[8], x[8];
-    load8(k, lo);
-    load8(k, hi);
-    for (int r = 1; r < rows; ++r) {
-      load8(k + r * kv.k_row, x);
+    const C* k = reinterpret_cast<const C*>(kv.k) + page * kv.k_page + head * kv.k_head + piece * CH;
+    uint32_t lo[PAIRS], hi[PAIRS];
+    for (int r0 = row0; r0 - row0 < rows; r0 += down * BOUNDS_ROWS) {
+      uint4 v[BOUNDS_ROWS];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        lo[j] = min_nan(lo[j], x[j]);
-        hi[j] = max_nan(hi[j], x[j]);
+      for (int i = 0; i < BOUNDS_ROWS; ++i) {                // rows past the last repeat it; lanes past the last row repeat row 0
+        const int r = min(row0 < down ? r0 + i * down : 0, rows - 1);
+        v[i] = ld_nc_v4(k + r * kv.k_row);
+      }
+#pragma unroll
+      for (int i = 0; i < BOUNDS_ROWS; ++i) {
+        const uint32_t word[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+        uint32_t pair[PAIRS];
+        if constexpr (sizeof(C) == 1) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) e4m3x4_to_f16x4(word[x], pair[2 * x], pair[2 * x + 1]);
+        } else {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) pair[x] = word[x];
+        }
+        const bool start = r0 == row0 && i == 0;
+#pragma unroll
+        for (int x = 0; x < PAIRS; ++x) {
+          lo[x] = start ? pair[x] : min2<C>(lo[x], pair[x]);
+          hi[x] = start ? pair[x] : max2<C>(hi[x], pair[x]);
+        }
       }
     }
-    B* out = reinterpret_cast<B*>(kv.bounds) + ((int64_t)page * kv.heads + head) * 2 * kv.dim + lane * 8;
-    store8(out, lo);
-    store8(out + kv.dim, hi);
+    for (int g = 1; g < down; ++g) {                         // the other rows' lanes
+#pragma unroll
+      for (int x = 0; x < PAIRS; ++x) {
+        lo[x] = min2<C>(lo[x], __shfl_sync(0xffffffffu, lo[x], g * across + piece));
+        hi[x] = max2<C>(hi[x], __shfl_sync(0xffffffffu, hi[x], g * across + piece));
+      }
+    }
+    if (row0 != 0) continue;
+    using P = typename std::conditional<std::is_same<C, __nv_bfloat16>::value, __nv_bfloat16, __half>::type;
+    B* out = reinterpret_cast<B*>(kv.bounds) + ((int64_t)page * kv.heads + head) * 2 * kv.dim + piece * CH;
+#pragma unroll
+    for (int x = 0; x < PAIRS; x += 4) {
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 t = to_float2<P>(y ? hi[x + i] : lo[x + i]);
+          f[2 * i] = t.x;
+          f[2 * i + 1] = t.y;
+        }
+        store8(out + y * kv.dim + x * 2, f);
+      }
+    }
   }
 }
 
@@ -153,97 +228,166 @@ __device__ __forceinline__ void mma_f64(double (&d)[2], double a, double b) {
 // negative parts: products [8 queries x 4 channels] . [4 channels x 8 pages] in 64 bits.  (A bound that is not finite makes
 // one of its two terms infinite or NaN whatever the query is.)  As in the attention, a product does not care which channel
 // is which, so a lane takes 8 neighbouring channels of a page with one load and feeds them to 8 products; the queries are
-// laid out to match in shared memory.  A block works on 64 pages of one (sequence, key head), 16 a warp.
+// laid out to match in shared memory.  A unit of work is 64 pages of one (sequence, key head), 16 a warp; the units of all
+// sequences that have more than `top` pages are numbered through, and every block takes an equal run of them.
+// The bounds are asked for before the queries are laid out (J: steps of 32 channels; 2 of them at a time).
 constexpr int SCORE_WARPS = 4, SCORE_PAGES = 16 * SCORE_WARPS;
-template <typename T, typename B>
-__global__ void __launch_bounds__(SCORE_WARPS * 32) score_kernel(const wush_kv_select_args a, int group, unsigned long long* keys) {
+template <typename T, typename B, int J>
+__global__ void __launch_bounds__(SCORE_WARPS * 32, J <= 4 ? 4 : 3) score_kernel(const wush_kv_select_args a, int group, unsigned long long* keys) {
   extern __shared__ double sm_q[];                           // [parts][channels / 32][8][8 queries][4]
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
-  const int d = a.kv.dim, steps = (d + 31) / 32;
-  const int blocks = (int)((a.table.width + SCORE_PAGES - 1) / SCORE_PAGES);
-  const int64_t entry = blockIdx.x / blocks, seq = entry / a.kv.heads;
-  const int head = (int)(entry % a.kv.heads), page0 = (int)(blockIdx.x % blocks) * SCORE_PAGES;
-  const int len = clamp_length(a.seq_lens[seq], a.table.width * a.kv.page_size, a.status);
-  const int n = (len + a.kv.page_size - 1) / a.kv.page_size;
-  if (page0 >= n || n <= a.top) return;
-  const B* bound[2];                                         // of the lane's two pages
-  bool known[2];
-#pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    const int lp = page0 + warp * 16 + x * 8 + r;
-    const int page = lp < n ? lookup_page(a.table, seq, lp, a.kv.num_pages, a.status) : -1;
-    known[x] = page >= 0;
-    bound[x] = reinterpret_cast<const B*>(a.kv.bounds) + ((int64_t)max(page, 0) * a.kv.heads + head) * 2 * d;
+  const int d = a.kv.dim, heads = a.kv.heads;
+  auto pages_of = [&](int64_t seq) {
+    const int len = clamp_length(a.seq_lens[seq], a.table.width * a.kv.page_size, a.status);
+    return (len + a.kv.page_size - 1) / a.kv.page_size;
+  };
+  auto units_of = [&](int64_t seq) -> int64_t {              // of one key head
+    if (seq >= a.table.seqs) return 0;
+    const int n = pages_of(seq);
+    return n > a.top ? (n + SCORE_PAGES - 1) / SCORE_PAGES : 0;
+  };
+  int64_t total = 0;
+  for (int64_t s0 = lane; s0 < a.table.seqs; s0 += 32) total += units_of(s0);
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  total *= heads;
+  const int64_t per = (total + gridDim.x - 1) / gridDim.x, unit_end = min(total, (blockIdx.x + 1) * per);
+  int64_t unit = blockIdx.x * per;
+  if (unit >= unit_end) return;
+  int64_t seq = 0, base = 0, units = 0;                      // the sequence the unit lies in, and its first unit
+  for (int64_t s0 = 0;; s0 += 32) {
+    units = units_of(s0 + lane);
+    int64_t sum = units * heads;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += x;
+    }
+    const unsigned beyond = __ballot_sync(0xffffffffu, base + sum > unit);
+    if (beyond) {
+      const int at = __ffs(beyond) - 1;
+      seq = s0 + at;
+      units = __shfl_sync(0xffffffffu, units, at);
+      base += __shfl_sync(0xffffffffu, sum, at) - units * heads;
+      break;
+    }
+    base += __shfl_sync(0xffffffffu, sum, 31);
   }
-  double best[2][2] = {{-INFINITY, -INFINITY}, {-INFINITY, -INFINITY}};
-  bool bad[2][2] = {{false, false}, {false, false}};         // a score that is not finite
-  for (int g0 = 0; g0 < group; g0 += 8) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < steps * 32; i += SCORE_WARPS * 32) {   // 8 channels of one query
-      const int row = i / (steps * 4), piece = i % (steps * 4);
-      float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-      if (g0 + row < group && piece * 8 < d)
-        load8(reinterpret_cast<const T*>(a.q.data) + seq * a.q.row + (int64_t)(head * group + g0 + row) * a.q.head + piece * 8, x);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        double* at = sm_q + ((piece >> 2) * 8 + e) * 32 + row * 4 + (piece & 3);
-        at[0] = x[e] > 0.0f ? (double)x[e] : 0.0;
-        at[steps * 256] = x[e] > 0.0f ? 0.0 : (double)x[e];  // (a NaN query lands here)
-      }
+  int laid_out = -1;                                         // key head whose queries are in shared memory
+  for (; unit < unit_end; ++unit) {
+    while (unit >= base + units * heads) {
+      base += units * heads;
+      units = units_of(++seq);
+      laid_out = -1;
     }
-    __syncthreads();
-    double s[2][2] = {{0.0, 0.0}, {0.0, 0.0}};
-    for (int j = 0; j < steps; ++j) {
-      const int ch = (j * 4 + c) * 8;
-      float lo[2][8], hi[2][8];
+    const int n = pages_of(seq), head = (int)((unit - base) / units), page0 = (int)((unit - base) % units) * SCORE_PAGES;
+    const int64_t entry = seq * heads + head;
+    const B* bound[2];                                         // of the lane's two pages
+    bool known[2];
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        if (known[x] && ch < d) {
-          load8(bound[x] + ch, lo[x]);
-          load8(bound[x] + d + ch, hi[x]);
-        } else {
+    for (int x = 0; x < 2; ++x) {
+      const int lp = page0 + warp * 16 + x * 8 + r;
+      const int page = lp < n ? lookup_page(a.table, seq, lp, a.kv.num_pages, a.status) : -1;
+      known[x] = page >= 0;
+      bound[x] = reinterpret_cast<const B*>(a.kv.bounds) + ((int64_t)max(page, 0) * heads + head) * 2 * d;
+    }
+    constexpr int HELD = 2;
+    uint4 raw[HELD][2][2];                                     // [step][page][lower, upper]
+    auto ask = [&](int j0) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) lo[x][e] = hi[x][e] = 0.0f;
+      for (int j = 0; j < HELD; ++j) {
+        const int ch = ((j0 + j) * 4 + c) * 8;
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            raw[j][x][y] = make_uint4(0, 0, 0, 0);
+            if (known[x] && ch < d) raw[j][x][y] = __ldg(reinterpret_cast<const uint4*>(bound[x] + y * d + ch));
+          }
+      }
+    };
+    ask(0);
+    double best[2][2] = {{-INFINITY, -INFINITY}, {-INFINITY, -INFINITY}};
+    bool bad[2][2] = {{false, false}, {false, false}};         // a score that is not finite
+    for (int g0 = 0; g0 < group; g0 += 8) {
+      if (group > 8 || laid_out != head) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < J * 32; i += SCORE_WARPS * 32) {   // 8 channels of one query
+          const int row = i / (J * 4), piece = i % (J * 4);
+        float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (g0 + row < group && piece * 8 < d)
+          load8(reinterpret_cast<const T*>(a.q.data) + seq * a.q.row + (int64_t)(head * group + g0 + row) * a.q.head + piece * 8, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          double* at = sm_q + ((piece >> 2) * 8 + e) * 32 + row * 4 + (piece & 3);
+          at[0] = x[e] > 0.0f ? (double)x[e] : 0.0;
+          at[J * 256] = x[e] > 0.0f ? 0.0 : (double)x[e];      // (a NaN query lands here)
         }
       }
+      laid_out = head;
+      __syncthreads();
+      }
+      // eight chains: a 64-bit product takes about 200 cycles to come back
+      double part[2][2][2][2] = {};                            // [page][sign][channel parity][element]
+      for (int j0 = 0; j0 < J; j0 += HELD) {
+        if (j0 > 0 || g0 > 0) ask(j0);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const double plus = sm_q[(j * 8 + e) * 32 + lane], minus = sm_q[steps * 256 + (j * 8 + e) * 32 + lane];
+        for (int j = 0; j < HELD; ++j) {
+          const double* plus = sm_q + (j0 + j) * 256 + lane;
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          mma_f64(s[x], plus, (double)hi[x][e]);
-          mma_f64(s[x], minus, (double)lo[x][e]);
+          for (int e2 = 0; e2 < 4; ++e2) {
+            float2 lo[2], hi[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const uint32_t l[4] = {raw[j][x][0].x, raw[j][x][0].y, raw[j][x][0].z, raw[j][x][0].w};
+              const uint32_t h[4] = {raw[j][x][1].x, raw[j][x][1].y, raw[j][x][1].z, raw[j][x][1].w};
+              lo[x] = to_float2<B>(l[e2]);
+              hi[x] = to_float2<B>(h[e2]);
+            }
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const double qp = plus[(2 * e2 + y) * 32], qm = plus[J * 256 + (2 * e2 + y) * 32];
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                mma_f64(part[x][0][y], qp, (double)(y ? hi[x].y : hi[x].x));
+                mma_f64(part[x][1][y], qm, (double)(y ? lo[x].y : lo[x].x));
+              }
+            }
+          }
         }
       }
+      double s[2][2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) s[x][y] = (part[x][0][0][y] + part[x][0][1][y]) + (part[x][1][0][y] + part[x][1][1][y]);
+      // the lane has query g0 + r and pages 2c, 2c + 1 of each 8
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          if (g0 + r >= group) continue;
+          bad[x][y] |= !(fabs(s[x][y]) <= 1.7976931348623157e308);
+          best[x][y] = fmax(best[x][y], s[x][y]);
+        }
     }
-    // the lane has query g0 + r and pages 2c, 2c + 1 of each 8
 #pragma unroll
     for (int x = 0; x < 2; ++x)
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
-        if (g0 + r >= group) continue;
-        bad[x][y] |= !(fabs(s[x][y]) <= 1.7976931348623157e308);
-        best[x][y] = fmax(best[x][y], s[x][y]);
+        double top = best[x][y];
+        unsigned any = bad[x][y];
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+          top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
+          any |= __shfl_xor_sync(0xffffffffu, any, o);
+        }
+        const bool known_page = __shfl_sync(0xffffffffu, known[x], (2 * c + y) * 4);
+        const int lp = page0 + warp * 16 + x * 8 + 2 * c + y;
+        // a page outside the pool comes last: the attention would leave it out
+        if (r == 0 && lp < n) keys[entry * a.table.width + lp] = !known_page ? 0 : (any ? ~0ull : score_key(top));
       }
   }
-#pragma unroll
-  for (int x = 0; x < 2; ++x)
-#pragma unroll
-    for (int y = 0; y < 2; ++y) {
-      double top = best[x][y];
-      unsigned any = bad[x][y];
-#pragma unroll
-      for (int o = 4; o < 32; o <<= 1) {
-        top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
-        any |= __shfl_xor_sync(0xffffffffu, any, o);
-      }
-      const bool known_page = __shfl_sync(0xffffffffu, known[x], (2 * c + y) * 4);
-      const int lp = page0 + warp * 16 + x * 8 + 2 * c + y;
-      // a page outside the pool comes last: the attention would leave it out
-      if (r == 0 && lp < n) keys[entry * a.table.width + lp] = !known_page ? 0 : (any ? ~0ull : score_key(top));
-    }
 }
 
 // Exclusive sums over `count` <= 256 numbers in shared memory, by one warp; returns the total.
@@ -456,10 +600,9 @@ extern "C" int wush_kv_append(const wush_kv_append_args* args) {
   if (p.rows == 0) return WUSH_OK;
   if (!p.seq_ids || !p.positions) return WUSH_ERR_NULL_POINTER;
   if ((rc = require_sm100()) != 0) return rc;
-  const int64_t units = p.rows * (int64_t)(p.q_heads + 2 * p.kv.heads) * ((p.kv.dim + 15) / 16 + 1);
-  const unsigned grid = (unsigned)min((units + 255) / 256, (int64_t)sm_count() * 32);
+  const unsigned grid = (unsigned)min(p.rows, (int64_t)INT32_MAX);
   auto go = [&](auto kern) {
-    kern<<<grid, 256, 0, (cudaStream_t)p.stream>>>(p);
+    kern<<<grid, APPEND_THREADS, 0, (cudaStream_t)p.stream>>>(p);
     return (int)cudaGetLastError();
   };
   if (p.type == WUSH_TYPE_BF16)
@@ -512,8 +655,7 @@ extern "C" int wush_kv_select_pages(const wush_kv_select_args* args) {
   if (a.table.seqs * a.kv.heads > INT32_MAX) return WUSH_ERR_TOO_LARGE;
   if ((rc = require_sm100()) != 0) return rc;
   unsigned long long* keys = reinterpret_cast<unsigned long long*>(a.workspace);
-  const int64_t blocks = a.table.seqs * a.kv.heads * ((a.table.width + SCORE_PAGES - 1) / SCORE_PAGES);
-  if (blocks > INT32_MAX) return WUSH_ERR_TOO_LARGE;
+  const int64_t units = a.table.seqs * a.kv.heads * ((a.table.width + SCORE_PAGES - 1) / SCORE_PAGES);
   // the kernels may be launched while the one before still runs, and wait for it before they read anything
   cudaLaunchAttribute early;
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -522,14 +664,21 @@ extern "C" int wush_kv_select_pages(const wush_kv_select_args* args) {
   cfg.stream = (cudaStream_t)a.stream;
   cfg.attrs = &early;
   cfg.numAttrs = 1;
-  cfg.gridDim = dim3((unsigned)blocks);
   cfg.blockDim = dim3(SCORE_WARPS * 32);
-  cfg.dynamicSmemBytes = (size_t)((a.kv.dim + 31) / 32) * 512 * sizeof(double);
-  auto go = [&](auto kern) { return (int)cudaLaunchKernelEx(&cfg, kern, a, a.q_heads / a.kv.heads, keys); };
-  if (a.type == WUSH_TYPE_BF16)
-    rc = a.kv.bounds_type == WUSH_TYPE_BF16 ? go(score_kernel<__nv_bfloat16, __nv_bfloat16>) : go(score_kernel<__nv_bfloat16, __half>);
-  else
-    rc = a.kv.bounds_type == WUSH_TYPE_BF16 ? go(score_kernel<__half, __nv_bfloat16>) : go(score_kernel<__half, __half>);
+  auto go = [&](auto kern, int steps) {
+    cfg.gridDim = dim3((unsigned)min(units, (int64_t)sm_count() * (steps <= 4 ? 4 : 3)));
+    cfg.dynamicSmemBytes = (size_t)steps * 512 * sizeof(double);
+    return (int)cudaLaunchKernelEx(&cfg, kern, a, a.q_heads / a.kv.heads, keys);
+  };
+  auto by_dim = [&](auto t, auto b) {
+    using T = decltype(t);
+    using B = decltype(b);
+    return a.kv.dim <= 64 ? go(score_kernel<T, B, 2>, 2) : (a.kv.dim <= 128 ? go(score_kernel<T, B, 4>, 4) : go(score_kernel<T, B, 8>, 8));
+  };
+  const __nv_bfloat16 bf = {};
+  const __half hf = {};
+  if (a.type == WUSH_TYPE_BF16) rc = a.kv.bounds_type == WUSH_TYPE_BF16 ? by_dim(bf, bf) : by_dim(bf, hf);
+  else rc = a.kv.bounds_type == WUSH_TYPE_BF16 ? by_dim(hf, bf) : by_dim(hf, hf);
   if (rc != 0) return rc;
   // 8 keys a thread in registers while that is enough
   int threads = 128;
