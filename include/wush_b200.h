@@ -542,8 +542,8 @@ typedef struct wush_heads {
  *   rope        fp32 [rope_rows, rotary]: cosines of the rotary/2 angles of a position, then sines; null: no rotation.
  *               rotary % 16 == 0, rotary <= dim; the channels behind it are copied.
  *   interleaved 0: channel i turns with i + rotary/2; 1: channel 2i with 2i + 1
- *   seq_ids, positions  int32 [rows].  A row with a negative id or position is padding: nothing of it is read or
- *               written.  An id, position or page outside its table sets *status = 2 and the row is skipped.
+ *   seq_ids, positions  int32 [rows].  A row with a negative id or position is padding: nothing is written for
+ *               it.  An id, position or page outside its table sets *status = 2 and the row is skipped.
  * No two rows may name the same token.  Arithmetic: products and their sum each rounded to fp32, stored rounded once
  * to the cache's type (E4M3: divided by the head's scale, saturated at +-448).
  */

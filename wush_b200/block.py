@@ -21,6 +21,10 @@ activations as a stack of K shards (`rows=` of qutlass_ops.matmul_fp4_blocked). 
 whole rows: the per-rank partial sums (4 bytes per token) travel the same way, and the normalisation itself is folded
 into the quantize kernel (its row_scale / col_scale prologue), as SwiGLU is a single pass.
 
+Decoding.  ``prefill`` is ``forward`` with a paged key-value cache of this rank's key heads (wush_b200/paged_kv.py) that is
+filled on the way; ``decode`` then runs one new token per sequence: rotation and append, attention over the pages, and
+the same linear layers.
+
 Overlap.  The tokens are cut into micro-batches that run on separate streams: while one micro-batch multiplies, the
 codes of the other are in flight.  Buffers live in torch symmetric memory; a stage's exchange ends with one
 cross-rank barrier on its stream.  No collective library call and no multicast is involved.
@@ -33,6 +37,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib
+from . import paged_kv
 from . import qutlass_ops as ops
 
 
@@ -234,8 +239,19 @@ class ShardedDecoderBlock:
         total = sums.total(ops.row_sumsq(h))
         return torch.rsqrt(total / self.cfg.hidden + self.cfg.rms_eps)
 
-    def _attention(self, qkv: torch.Tensor) -> torch.Tensor:
+    def _heads(self, qkv: torch.Tensor):
+        """(q, k, v) views [tokens, heads, head_dim] of the fused projection's output."""
+        t = qkv.view(qkv.shape[0], self.hq + 2 * self.hkv, self.cfg.head_dim)
+        return t[:, : self.hq], t[:, self.hq: self.hq + self.hkv], t[:, self.hq + self.hkv:]
+
+    def _attention(self, qkv: torch.Tensor, prompt=None) -> torch.Tensor:
+        """prompt: (cache, block table, sequence ids, positions, rotation table, interleaved) when the keys and values are
+        kept; q and k are then rotated in place first."""
         d, s = self.cfg.head_dim, self.seq_len
+        if prompt is not None:
+            cache, table, ids, positions, rope, interleaved = prompt
+            q, k, v = self._heads(qkv)
+            paged_kv.paged_kv_append(cache, k, v, table, ids, positions, q=q, rope=rope, interleaved=interleaved, q_out=q, k_out=k)
         b = qkv.shape[0] // s
         t = qkv.view(b, s, self.hq + 2 * self.hkv, d)
         q = t[:, :, : self.hq].transpose(1, 2)
@@ -244,13 +260,14 @@ class ShardedDecoderBlock:
         o = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=self.hq != self.hkv)
         return o.transpose(1, 2).reshape(qkv.shape[0], self.hq * d)
 
-    def _micro_batch(self, h: torch.Tensor, slot: dict) -> None:
+    def _micro_batch(self, h: torch.Tensor, slot: dict, attention=None) -> None:
         cfg, fmt, m = self.cfg, self.cfg.fmt, h.shape[0]
+        attention = attention or self._attention
         a, b = slot["h"]
         # attention half
         a.put(h, self.t["attn_in"], fmt, self.gs, row_scale=self._rstd(h, slot["ssq"][0]), col_scale=self.gamma[0])
         qkv = a.gemm(m, *self.w["qkv"], self.alpha, fmt)
-        b.put(self._attention(qkv), self.t["o"], fmt, self.gs)
+        b.put(attention(qkv), self.t["o"], fmt, self.gs)
         b.gemm(m, *self.w["o"], self.alpha, fmt, residual=h, out=h)            # h += o_proj(...) in the epilogue
         # MLP half
         a.put(h, self.t["mlp_in"], fmt, self.gs, row_scale=self._rstd(h, slot["ssq"][1]), col_scale=self.gamma[1])
@@ -260,6 +277,48 @@ class ShardedDecoderBlock:
         del cfg
 
     def forward(self, h_local: torch.Tensor) -> torch.Tensor:
+        return self._forward(h_local, None)
+
+    def prefill(self, h_local: torch.Tensor, cache: "paged_kv.PagedKVCache", block_table: torch.Tensor, lengths: torch.Tensor,
+                rope=None, interleaved: bool = False) -> torch.Tensor:
+        """``forward`` of prompts whose keys (rotated by ``rope``, see ``paged_kv.rope_table``; None: not at all) and values
+        go into this rank's ``cache``.  h_local: sequences of ``seq_len`` rows each, the first lengths[b] of them real; rows
+        behind a sequence's length are computed but not kept (causal attention keeps them from the rows before).
+        lengths: int32 [sequences]; block_table: int32 [sequences, pages]."""
+        seqs = h_local.shape[0] // self.seq_len
+        if cache.dtype not in (torch.bfloat16, torch.float8_e4m3fn) or cache.n_kv_heads != self.hkv or cache.head_dim != self.cfg.head_dim:
+            raise ValueError(f"the cache must hold bfloat16 or 8-bit pages of {self.hkv} heads of {self.cfg.head_dim} channels")
+        if lengths.dtype != torch.int32 or tuple(lengths.shape) != (seqs,) or block_table.shape[0] != seqs:
+            raise ValueError(f"lengths must be int32 [{seqs}], block_table int32 [{seqs}, pages]")
+        at = torch.arange(self.seq_len, dtype=torch.int32, device=self.dev)
+        positions = torch.where(at < lengths[:, None], at, torch.full_like(at, -1)).view(-1)   # -1: padding
+        ids = torch.arange(seqs, dtype=torch.int32, device=self.dev).repeat_interleave(self.seq_len)
+        out = self._forward(h_local, lambda lo, hi: lambda qkv: self._attention(
+            qkv, (cache, block_table, ids[lo:hi], positions[lo:hi], rope, interleaved)))
+        if cache.bounds is not None:
+            paged_kv.paged_kv_bounds(cache, block_table, lengths, self.seq_len)
+        return out
+
+    def decode(self, h_local: torch.Tensor, cache: "paged_kv.PagedKVCache", step: "paged_kv.DecodeStep") -> torch.Tensor:
+        """One new token per sequence: h_local is this rank's column shard [sequences, hidden / world] of the residual
+        stream, updated in place; ``step`` (shared by all layers) says where the tokens stand.  Rows of sequences with
+        length 0 are padding: nothing of them enters the cache, and they attend to nothing.  Runs on the current stream; like
+        ``forward`` it uses the block's buffers, so one call of a block at a time."""
+        if h_local.dtype != torch.bfloat16 or h_local.dim() != 2 or h_local.shape[1] != self.hs or not h_local.is_contiguous():
+            raise ValueError(f"h_local must be a contiguous bfloat16 [sequences, {self.hs}] tensor")
+        m = h_local.shape[0]
+        if m != step.seq_lens.shape[0] or m > self.mb_rows:
+            raise ValueError(f"one row per sequence, and at most {self.mb_rows}")
+        if m == 0:
+            return h_local
+
+        def attention(qkv):
+            q, k, v = self._heads(qkv)
+            return step.attend(cache, q, k, v).view(m, self.hq * self.cfg.head_dim)
+        self._micro_batch(h_local, self.slots[0], attention)
+        return h_local
+
+    def _forward(self, h_local: torch.Tensor, attention_of) -> torch.Tensor:
         if h_local.dtype != torch.bfloat16 or h_local.shape[1] != self.hs or not h_local.is_contiguous():
             raise ValueError(f"h_local must be a contiguous bfloat16 [tokens, {self.hs}] tensor")
         tokens = h_local.shape[0]
@@ -276,7 +335,7 @@ class ShardedDecoderBlock:
                 continue
             st.wait_stream(main)
             with torch.cuda.stream(st):
-                self._micro_batch(h_local[lo:hi], self.slots[j])
+                self._micro_batch(h_local[lo:hi], self.slots[j], attention_of(lo, hi) if attention_of else None)
         for st in self.streams:
             main.wait_stream(st)
         return h_local

@@ -100,6 +100,48 @@ class PagedKVCache:
         return cls(pool(), pool(), k_scale=k_scale, v_scale=v_scale, bounds=b)
 
 
+class DecodeStep:
+    """What the layers of a model share in one decoding step (or the prompt pass before it): lengths, tables, rotation and
+    the form of the attention.  ``wush_b200.block.ShardedDecoderBlock.decode`` takes it.
+
+    block_table  int32 [sequences, pages]
+    seq_lens     int32 [sequences]: tokens of every sequence, the new one included; 0 for a padded row
+    rope         fp32 table for ``paged_kv_append`` (None: no rotation), interleaved its pairing
+    scale, window  of ``paged_decode_attention``
+    top_pages    attend to this many selected pages per key head (0: all); needs caches with bounds
+    """
+
+    def __init__(self, block_table: torch.Tensor, seq_lens: torch.Tensor, rope: Optional[torch.Tensor] = None,
+                 interleaved: bool = False, scale: Optional[float] = None, window: int = 0, top_pages: int = 0):
+        if top_pages < 0 or (top_pages and window):
+            raise ValueError("top_pages must not be negative; a window and selected pages exclude each other")
+        if seq_lens.dim() != 1 or seq_lens.dtype != torch.int32:
+            raise ValueError("seq_lens must be an int32 [sequences] tensor")
+        self.block_table, self.seq_lens, self.rope, self.interleaved = block_table, seq_lens, rope, interleaved
+        self.scale, self.window, self.top_pages = scale, window, top_pages
+        self.seq_ids = torch.arange(seq_lens.shape[0], dtype=torch.int32, device=seq_lens.device)
+        self.positions = seq_lens - 1                         # of the new tokens; -1 in a padded row
+
+    def advance(self) -> None:
+        """The next token of every sequence (padded rows stay padding); in place, so that captured steps see it."""
+        self.seq_lens += self.seq_lens > 0
+        torch.sub(self.seq_lens, 1, out=self.positions)
+
+    def attend(self, cache: PagedKVCache, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
+        """Append the new tokens' keys and values ([sequences, heads, head_dim]) to a layer's cache and attend.  ``q`` is
+        overwritten, first by the rotated queries, then by the result, and returned."""
+        paged_kv_append(cache, k, v, self.block_table, self.seq_ids, self.positions, q=q, rope=self.rope,
+                        interleaved=self.interleaved, q_out=q)
+        if cache.bounds is not None:
+            paged_kv_bounds(cache, self.block_table, self.seq_lens)
+        pages = counts = None
+        if self.top_pages:
+            pages, counts = paged_select_pages(q, cache, self.block_table, self.seq_lens, self.top_pages,
+                                               sink=min(1, self.top_pages - 1))
+        return paged_decode_attention(q, cache, self.block_table, self.seq_lens, scale=self.scale, window=self.window,
+                                      pages=pages, counts=counts, out=q)
+
+
 def _check_pool(k, v, k_scale, v_scale, bounds) -> None:
     if k.dim() != 4 or k.shape != v.shape or min(k.shape) < 1:
         raise ValueError("k and v must be [num_pages, page_size, n_kv_heads, head_dim] tensors of one shape")
@@ -215,7 +257,7 @@ def paged_kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, block
     k, v       [rows, n_kv_heads, head_dim], q [rows, heads, head_dim]: slices of one fused projection will do
     seq_ids    int32 [rows]: row of ``block_table`` (int32 [sequences, pages]) the token belongs to
     positions  int32 [rows]: its position in that sequence.  A row with a negative id or position is padding: nothing is
-               read from it or written for it.  No two rows may name the same token.
+               written for it.  No two rows may name the same token.
     rope       fp32 [positions, rotary_dim] (see ``rope_table``), rotary_dim a multiple of 16; None: no rotation.
                Channels behind rotary_dim are copied.  ``interleaved`` False: channel i turns with i + rotary_dim/2,
                True: channel 2i with 2i + 1.
