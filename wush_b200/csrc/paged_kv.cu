@@ -149,38 +149,51 @@ __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
   return r;
 }
 
-// One warp per (sequence, page, head); a lane takes 16 bytes of every n-th row, 8 rows under way at a time.
-constexpr int BOUNDS_ROWS = 8;
+// A warp works on `span` consecutive pages of one (sequence, head), whose places its lanes look up together; a lane takes 16
+// bytes of every n-th row, and the next BOUNDS_ROWS rows, of this page or the next, are under way while it compares those it
+// has.  (A page a warp without that: 3.9 TB/s whatever the batch, every warp waiting for length, page and rows in turn.)
+constexpr int BOUNDS_ROWS = 8, BOUNDS_SPAN = 8;
 template <typename C, typename B>
-__global__ void __launch_bounds__(256) bounds_kernel(const wush_kv_pages kv, const wush_kv_table table, const int32_t* seq_lens,
-                                                     int64_t new_tokens, int64_t most, int* status) {
+__global__ void __launch_bounds__(128) bounds_kernel(const wush_kv_pages kv, const wush_kv_table table, const int32_t* seq_lens,
+                                                     int64_t new_tokens, int64_t most, int span, int* status) {
   constexpr int CH = 16 / (int)sizeof(C), PAIRS = CH / 2;    // channels of a lane
+  using P = typename std::conditional<std::is_same<C, __nv_bfloat16>::value, __nv_bfloat16, __half>::type;
   const int lane = threadIdx.x & 31;
   const int across = (kv.dim + CH - 1) / CH, down = 32 / across;   // lanes of a row, rows of a warp
   const int piece = lane % across, row0 = lane / across;
-  const int64_t warps = (int64_t)gridDim.x * (blockDim.x >> 5), total = table.seqs * most * kv.heads;
+  const int64_t groups = (most + span - 1) / span, total = table.seqs * groups * kv.heads;
+  const int64_t warps = (int64_t)gridDim.x * (blockDim.x >> 5);
   for (int64_t w = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); w < total; w += warps) {
-    const int64_t slot = w / kv.heads, seq = slot / most;
+    const int64_t slot = w / kv.heads, seq = slot / groups;
     const int head = (int)(w - slot * kv.heads);
     const int len = clamp_length(seq_lens[seq], table.width * kv.page_size, status);
-    const int64_t first = len > new_tokens ? len - new_tokens : 0;
-    const int64_t lp = first / kv.page_size + (slot - seq * most);
-    if (lp * kv.page_size >= len) continue;
-    const int page = lookup_page(table, seq, (int)lp, kv.num_pages, status);
-    if (page < 0) continue;
-    const int rows = (int)min((int64_t)kv.page_size, len - lp * kv.page_size);
-    const C* k = reinterpret_cast<const C*>(kv.k) + page * kv.k_page + head * kv.k_head + piece * CH;
+    const int64_t first = (len > new_tokens ? len - new_tokens : 0) / kv.page_size + (slot - seq * groups) * span;
+    const int64_t behind = min((int64_t)(len + kv.page_size - 1) / kv.page_size, first + span);   // one past the last page
+    if (first >= behind) continue;
+    const int pages = (int)(behind - first);
+    const int my_page = lane < pages ? lookup_page(table, seq, (int)first + lane, kv.num_pages, status) : -1;
+    const C* base = reinterpret_cast<const C*>(kv.k) + head * kv.k_head + piece * CH;
+    auto rows_of = [&](int i) { return (int)min((int64_t)kv.page_size, len - (first + i) * kv.page_size); };
+    uint4 v[BOUNDS_ROWS], ahead[BOUNDS_ROWS];
+    auto load = [&](int i, int r0) {                         // rows r0, r0 + down, ... of page i; past the last: that again
+      const int page = max(0, __shfl_sync(0xffffffffu, my_page, i)), rows = rows_of(i);
+      const C* k = base + page * kv.k_page;
+#pragma unroll
+      for (int x = 0; x < BOUNDS_ROWS; ++x) ahead[x] = ld_nc_v4(k + min(row0 < down ? r0 + row0 + x * down : 0, rows - 1) * kv.k_row);
+    };
     uint32_t lo[PAIRS], hi[PAIRS];
-    for (int r0 = row0; r0 - row0 < rows; r0 += down * BOUNDS_ROWS) {
-      uint4 v[BOUNDS_ROWS];
+    load(0, 0);
+    for (int i = 0, r0 = 0; i < pages;) {
+      const int rows = rows_of(i), next_r = r0 + down * BOUNDS_ROWS;
+      const bool start = r0 == 0, ends = next_r >= rows;
+      const int page = __shfl_sync(0xffffffffu, my_page, i);
 #pragma unroll
-      for (int i = 0; i < BOUNDS_ROWS; ++i) {                // rows past the last repeat it; lanes past the last row repeat row 0
-        const int r = min(row0 < down ? r0 + i * down : 0, rows - 1);
-        v[i] = ld_nc_v4(k + r * kv.k_row);
-      }
+      for (int x = 0; x < BOUNDS_ROWS; ++x) v[x] = ahead[x];
+      if (!ends) load(i, next_r);
+      else if (i + 1 < pages) load(i + 1, 0);
 #pragma unroll
-      for (int i = 0; i < BOUNDS_ROWS; ++i) {
-        const uint32_t word[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+      for (int y = 0; y < BOUNDS_ROWS; ++y) {
+        const uint32_t word[4] = {v[y].x, v[y].y, v[y].z, v[y].w};
         uint32_t pair[PAIRS];
         if constexpr (sizeof(C) == 1) {
 #pragma unroll
@@ -189,36 +202,68 @@ __global__ void __launch_bounds__(256) bounds_kernel(const wush_kv_pages kv, con
 #pragma unroll
           for (int x = 0; x < 4; ++x) pair[x] = word[x];
         }
-        const bool start = r0 == row0 && i == 0;
 #pragma unroll
         for (int x = 0; x < PAIRS; ++x) {
-          lo[x] = start ? pair[x] : min2<C>(lo[x], pair[x]);
-          hi[x] = start ? pair[x] : max2<C>(hi[x], pair[x]);
+          lo[x] = start && y == 0 ? pair[x] : min2<C>(lo[x], pair[x]);
+          hi[x] = start && y == 0 ? pair[x] : max2<C>(hi[x], pair[x]);
         }
       }
-    }
-    for (int g = 1; g < down; ++g) {                         // the other rows' lanes
-#pragma unroll
-      for (int x = 0; x < PAIRS; ++x) {
-        lo[x] = min2<C>(lo[x], __shfl_sync(0xffffffffu, lo[x], g * across + piece));
-        hi[x] = max2<C>(hi[x], __shfl_sync(0xffffffffu, hi[x], g * across + piece));
-      }
-    }
-    if (row0 != 0) continue;
-    using P = typename std::conditional<std::is_same<C, __nv_bfloat16>::value, __nv_bfloat16, __half>::type;
-    B* out = reinterpret_cast<B*>(kv.bounds) + ((int64_t)page * kv.heads + head) * 2 * kv.dim + piece * CH;
-#pragma unroll
-    for (int x = 0; x < PAIRS; x += 4) {
-#pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        float f[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 t = to_float2<P>(y ? hi[x + i] : lo[x + i]);
-          f[2 * i] = t.x;
-          f[2 * i + 1] = t.y;
+      i += ends;
+      r0 = ends ? 0 : next_r;
+      if (!ends) continue;
+      uint32_t* out = reinterpret_cast<uint32_t*>(reinterpret_cast<B*>(kv.bounds) + ((int64_t)max(page, 0) * kv.heads + head) * 2 * kv.dim + piece * CH);
+      auto store = [&](int x, uint32_t l, uint32_t h) {        // pair x of the lane's piece
+        if constexpr (std::is_same<P, B>::value) {
+          out[x] = l;
+          out[kv.dim / 2 + x] = h;
+        } else {                                               // E4M3 values: exact in either type
+          const float2 fl = to_float2<P>(l), fh = to_float2<P>(h);
+          out[x] = pack2<B>(fl.x, fl.y);
+          out[kv.dim / 2 + x] = pack2<B>(fh.x, fh.y);
         }
-        store8(out + y * kv.dim + x * 2, f);
+      };
+      if ((across & (across - 1)) == 0) {
+        // lanes of the same channels exchange halves of what they hold: 12 shuffles for 4 rows of 16 channels instead of 96
+        int offset = 0, held = PAIRS;
+        bool writes = true;
+#pragma unroll
+        for (int s = 0; s < 5; ++s) {
+          if (1 << s >= down) break;
+          const int half = PAIRS >> (s + 1), partner = across << s;
+          const bool upper = lane & partner;
+          if (half > 0) {
+#pragma unroll
+            for (int x = 0; x < half; ++x) {
+              const uint32_t kl = upper ? lo[x + half] : lo[x], sl = upper ? lo[x] : lo[x + half];
+              const uint32_t kh = upper ? hi[x + half] : hi[x], sh = upper ? hi[x] : hi[x + half];
+              lo[x] = min2<C>(kl, __shfl_xor_sync(0xffffffffu, sl, partner));
+              hi[x] = max2<C>(kh, __shfl_xor_sync(0xffffffffu, sh, partner));
+            }
+            offset += upper ? half : 0;
+            held = half;
+          } else {
+            lo[0] = min2<C>(lo[0], __shfl_xor_sync(0xffffffffu, lo[0], partner));
+            hi[0] = max2<C>(hi[0], __shfl_xor_sync(0xffffffffu, hi[0], partner));
+            writes = writes && !upper;
+          }
+        }
+        if (writes && page >= 0) {
+#pragma unroll
+          for (int x = 0; x < PAIRS; ++x)
+            if (x < held) store(offset + x, lo[x], hi[x]);
+        }
+      } else {
+        for (int g = 1; g < down; ++g) {                       // the other rows' lanes, one after another
+#pragma unroll
+          for (int x = 0; x < PAIRS; ++x) {
+            lo[x] = min2<C>(lo[x], __shfl_sync(0xffffffffu, lo[x], g * across + piece));
+            hi[x] = max2<C>(hi[x], __shfl_sync(0xffffffffu, hi[x], g * across + piece));
+          }
+        }
+        if (row0 == 0 && page >= 0) {
+#pragma unroll
+          for (int x = 0; x < PAIRS; ++x) store(x, lo[x], hi[x]);
+        }
       }
     }
   }
@@ -640,10 +685,13 @@ extern "C" int wush_kv_bounds(const wush_kv_bounds_args* args) {
   if (!args->seq_lens) return WUSH_ERR_NULL_POINTER;
   if ((rc = require_sm100()) != 0) return rc;
   const int64_t most = min(table.width, (args->new_tokens - 1) / kv.page_size + 2);   // pages that the last tokens can touch
-  const int64_t warps = table.seqs * most * kv.heads;
-  const unsigned grid = (unsigned)min((warps + 7) / 8, (int64_t)sm_count() * 32);
+  // one page a warp until every SM has 16 warps
+  const int sms = sm_count();
+  const int span = (int)min((int64_t)BOUNDS_SPAN, max((int64_t)1, table.seqs * most * kv.heads / (16 * sms)));
+  const int64_t warps = table.seqs * ((most + span - 1) / span) * kv.heads;
+  const unsigned grid = (unsigned)min((warps + 3) / 4, (int64_t)sms * 64);
   auto go = [&](auto kern) {
-    kern<<<grid, 256, 0, (cudaStream_t)args->stream>>>(kv, table, args->seq_lens, args->new_tokens, most, args->status);
+    kern<<<grid, 128, 0, (cudaStream_t)args->stream>>>(kv, table, args->seq_lens, args->new_tokens, most, span, args->status);
     return (int)cudaGetLastError();
   };
   if (kv.type == WUSH_TYPE_BF16) return go(bounds_kernel<__nv_bfloat16, __nv_bfloat16>);
