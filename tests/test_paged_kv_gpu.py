@@ -439,6 +439,45 @@ def test_selection_over_many_pages(width):
     _status_clear()
 
 
+@pytest.mark.parametrize("typ,bounds", [(BF, BF), (HF, HF), (HF, BF), (BF, HF)])
+@pytest.mark.parametrize("crowd,width", [(3, 900), (200, 900), (900, 900), (900, 9000)])
+def test_selection_where_fp32_scores_cannot_decide(typ, bounds, crowd, width):
+    """`crowd` pages of `width` are equal but for terms of 2^12 and -2^12 in other channels and one of -2^-14 to 2^-14: fp32
+    sums lose it.  The border runs through them; bounds of the other 16-bit type than the queries' go with 8-bit pages."""
+    from wush_b200 import paged_kv
+    from wush_b200.paged_kv import PagedKVCache
+    g, dev = _gen(crowd + width), _dev()
+    one = torch.ones(2, device=dev)
+    cache = F8 if typ != bounds else typ
+    data = torch.zeros(width, 16, 2, 128, dtype=cache, device=dev)
+    pool = PagedKVCache(data, data, k_scale=one if cache == F8 else None, v_scale=one if cache == F8 else None,
+                        bounds=torch.zeros(width, 2, 2, 128, dtype=bounds, device=dev))
+    low = torch.randn(width, 2, 128, generator=g, device=dev) - 4
+    who = torch.randperm(width, generator=g, device=dev)[:crowd]
+    low[who] = 0.0
+    for h in range(2):
+        at = torch.randint(0, 63, (crowd,), generator=g, device=dev)
+        low[who, h, at], low[who, h, at + 64] = 2.0 ** 12, -2.0 ** 12
+        low[who, h, 63] = 2.0 ** -14 * torch.randint(-1, 2, (crowd,), generator=g, device=dev).float()
+    pool.bounds[:, :, 0] = low.to(bounds)
+    pool.bounds[:, :, 1] = pool.bounds[:, :, 0]
+    q = torch.ones(1, 6, 128, dtype=typ, device=dev)
+    q[0, 4] = 0.5
+    table = torch.randperm(width, generator=g, device=dev).to(torch.int32)[None]
+    lens = torch.tensor([16 * width], dtype=torch.int32, device=dev)
+    for top, sink, recent in ((max(2, crowd // 2), 0, 0), (crowd // 3 + 3, 1, 1), (1, 0, 0)):
+        pages, counts = paged_kv.paged_select_pages(q, pool, table, lens, top, sink=sink, recent=recent)
+        for h in range(2):
+            b = pool.bounds[table[0].long(), h].double()
+            score = torch.stack([torch.maximum(q[0, x].double() * b[:, 0], q[0, x].double() * b[:, 1]).sum(1) for x in range(3 * h, 3 * h + 3)])
+            assert pages[0, h].tolist() == ref.select(score.amax(0).tolist(), top, sink, recent), (top, h)
+    # one page that is not finite: every score is computed again
+    pool.bounds[int(table[0, width // 2]), 0, 1, 7] = math.inf
+    pages, _ = paged_kv.paged_select_pages(q, pool, table, lens, 2, sink=0, recent=0)
+    assert width // 2 in pages[0, 0].tolist()
+    _status_clear()
+
+
 def test_selection_close_scores_do_not_depend_on_the_order_of_the_sum():
     """Pages whose scores differ only in the 40th bit: terms of 2^20 and -2^20 around one of 2^-20."""
     from wush_b200 import paged_kv

@@ -1,4 +1,5 @@
 // Paged key-value cache: append with rotation, per-page bounds of the keys, selection of pages.
+#include <cfloat>
 #include <type_traits>
 
 #include "paged_kv.cuh"
@@ -270,31 +271,73 @@ __global__ void __launch_bounds__(128) bounds_kernel(const wush_kv_pages kv, con
 }
 
 // ---- selection -----------------------------------------------------------------------------------------------------
-// A score as a 64-bit key with the same order; one that is not finite counts as +infinity.
+// The score of a page for a key head is max over its queries of sum_d max(q_d lower_d, q_d upper_d), and the choice has to be
+// the one that exact scores give.  64-bit sums of all of them cost 35 us where their bounds can be read in 6 (64-bit products,
+// on either pipe, were the limit), so the work is divided:
+//   1. score_kernel computes every score on the tensor cores in fp32, with the sum of the terms' magnitudes;
+//   2. select_kernel finds the k-th largest of them, and from the magnitudes an eps by which no score is off.  What is more
+//      than 2 eps above the k-th largest is among the k best, what is more than 2 eps below it is not; the few pages between
+//      are scored again in 64 bits and ranked.
+// Error of an fp32 score: an m16n8k16 product of its own (nothing to add to) adds 16 exact products; if each addend and the
+// result is cut to 24 bits at the scale of the largest, it is off by at most 17 * 2^-23 of its terms' magnitude.  The
+// 2 * ceil(dim / 16) products of a score are added in fp32, 2^-24 of the magnitude each.  (Chained through the product's
+// accumulator every product would add 18 * 2^-23 of the whole magnitude: 16 times as many pages lay between, and scoring them
+// again took 5 to 10 us.)
+struct Score {
+  float value, magnitude;               // magnitude: infinity when the score has to be computed again in any case
+};
+
+__device__ __forceinline__ uint32_t float_key(float x) {     // same order; equal numbers, equal keys
+  const uint32_t b = __float_as_uint(x + 0.0f);
+  return b >> 31 ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float key_float(uint32_t k) { return __uint_as_float(k >> 31 ? k & 0x7fffffffu : ~k); }
+
+// A 64-bit score as a key with the same order; one that is not finite counts as +infinity.
 __device__ __forceinline__ unsigned long long score_key(double s) {
   if (!(fabs(s) <= 1.7976931348623157e308)) return ~0ull;
-  const long long b = __double_as_longlong(s + 0.0);       // -0 + 0 = +0: equal numbers, equal keys
+  const long long b = __double_as_longlong(s + 0.0);         // -0 + 0 = +0: equal numbers, equal keys
   return b < 0 ? ~(unsigned long long)b : (unsigned long long)b | 0x8000000000000000ull;
 }
 
-__device__ __forceinline__ void mma_f64(double (&d)[2], double a, double b) {
-  asm("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0,%1}, {%2}, {%3}, {%0,%1};\n" : "+d"(d[0]), "+d"(d[1]) : "d"(a), "d"(b));
+template <typename T>
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (std::is_same<T, __half>::value)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Keys of the scores: sum_d max(q_d lower_d, q_d upper_d) = sum_d q+_d upper_d + q-_d lower_d, with q+ and q- the positive and
-// negative parts: products [8 queries x 4 channels] . [4 channels x 8 pages] in 64 bits.  (A bound that is not finite makes
-// one of its two terms infinite or NaN whatever the query is.)  As in the attention, a product does not care which channel
-// is which, so a lane takes 8 neighbouring channels of a page with one load and feeds them to 8 products; the queries are
-// laid out to match in shared memory.  A unit of work is 64 pages of one (sequence, key head), 16 a warp; the units of all
-// sequences that have more than `top` pages are numbered through, and every block takes an equal run of them.
-// The bounds are asked for before the queries are laid out (J: steps of 32 channels; 2 of them at a time).
-constexpr int SCORE_WARPS = 4, SCORE_PAGES = 16 * SCORE_WARPS;
+// A pair of bounds in the queries' type; NaN where that is not exact (E4M3 keys are exact in both).
+template <typename T, typename B>
+__device__ __forceinline__ uint32_t as_query_type(uint32_t pair) {
+  if constexpr (std::is_same<T, B>::value) {
+    return pair;
+  } else {
+    const float2 f = to_float2<B>(pair);
+    const uint32_t p = pack2<T>(f.x, f.y);
+    const float2 back = to_float2<T>(p);
+    return (p & (back.x == f.x ? 0xffffu : 0u)) | (back.x == f.x ? 0u : 0x7fffu) | (p & (back.y == f.y ? 0xffff0000u : 0u)) |
+           (back.y == f.y ? 0u : 0x7fff0000u);
+  }
+}
+
+// fp32 scores: products [16 pages x 16 channels] . [16 channels x 8 queries] of the upper bounds with the queries' positive
+// parts, the lower bounds with their negative parts, and the larger magnitudes with their magnitudes.  As in the attention,
+// a product does not care which channel is which: a lane takes 8 neighbouring channels of two pages with one load each.
+// (A bound that is not finite makes one of its terms infinite or NaN whatever the query is.)  A unit of work is 16 pages of
+// one (sequence, key head); the units of all sequences that have more than `top` pages are numbered through, and every warp
+// takes an equal run of them.  J: steps of 32 channels.
+constexpr int SCORE_WARPS = 4, SCORE_PAGES = 16, SCORE_BLOCKS = 3;
 template <typename T, typename B, int J>
-__global__ void __launch_bounds__(SCORE_WARPS * 32, J <= 4 ? 4 : 3) score_kernel(const wush_kv_select_args a, int group, unsigned long long* keys) {
-  extern __shared__ double sm_q[];                           // [parts][channels / 32][8][8 queries][4]
+__global__ void __launch_bounds__(SCORE_WARPS * 32, J <= 4 ? SCORE_BLOCKS : 2) score_kernel(const wush_kv_select_args a, int group, Score* scores) {
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
+  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   const int d = a.kv.dim, heads = a.kv.heads;
   auto pages_of = [&](int64_t seq) {
     const int len = clamp_length(a.seq_lens[seq], a.table.width * a.kv.page_size, a.status);
@@ -309,8 +352,9 @@ __global__ void __launch_bounds__(SCORE_WARPS * 32, J <= 4 ? 4 : 3) score_kernel
   for (int64_t s0 = lane; s0 < a.table.seqs; s0 += 32) total += units_of(s0);
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   total *= heads;
-  const int64_t per = (total + gridDim.x - 1) / gridDim.x, unit_end = min(total, (blockIdx.x + 1) * per);
-  int64_t unit = blockIdx.x * per;
+  const int64_t warps = (int64_t)gridDim.x * SCORE_WARPS, per = (total + warps - 1) / warps;
+  int64_t unit = ((int64_t)blockIdx.x * SCORE_WARPS + (threadIdx.x >> 5)) * per;
+  const int64_t unit_end = min(total, unit + per);
   if (unit >= unit_end) return;
   int64_t seq = 0, base = 0, units = 0;                      // the sequence the unit lies in, and its first unit
   for (int64_t s0 = 0;; s0 += 32) {
@@ -330,121 +374,141 @@ __global__ void __launch_bounds__(SCORE_WARPS * 32, J <= 4 ? 4 : 3) score_kernel
     }
     base += __shfl_sync(0xffffffffu, sum, 31);
   }
-  int laid_out = -1;                                         // key head whose queries are in shared memory
-  for (; unit < unit_end; ++unit) {
-    while (unit >= base + units * heads) {
+  // the pages of a unit are looked up one unit ahead
+  struct Unit { int64_t seq; int head, page0, n, my_page; };
+  auto find = [&](int64_t t) -> Unit {
+    while (t >= base + units * heads) {
       base += units * heads;
       units = units_of(++seq);
-      laid_out = -1;
     }
-    const int n = pages_of(seq), head = (int)((unit - base) / units), page0 = (int)((unit - base) % units) * SCORE_PAGES;
-    const int64_t entry = seq * heads + head;
-    const B* bound[2];                                         // of the lane's two pages
-    bool known[2];
+    Unit u{seq, (int)((uint64_t)(t - base) / (uint64_t)units), 0, pages_of(seq), -1};
+    u.page0 = (int)(t - base - u.head * units) * SCORE_PAGES;
+    const int lp = u.page0 + (lane & 15);
+    if (lp < u.n) u.my_page = lookup_page(a.table, seq, lp, a.kv.num_pages, a.status);
+    return u;
+  };
+  uint4 q[J];                                                // of the lane's query
+  auto ask_queries = [&](const Unit& u, int g0) {
+    const T* row = reinterpret_cast<const T*>(a.q.data) + u.seq * a.q.row + (int64_t)(u.head * group + min(g0 + r, group - 1)) * a.q.head;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int ch = (j * 4 + c) * 8;
+      q[j] = ch < d ? *reinterpret_cast<const uint4*>(row + ch) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  Unit then = find(unit);
+  int64_t held_seq = -1;
+  int held_head = -1;
+  for (; unit < unit_end; ++unit) {
+    const Unit now = then;
+    const int head = now.head;
+    uint4 raw[J][2][2];                                      // [step][page r, r + 8][lower, upper]
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      const int lp = page0 + warp * 16 + x * 8 + r;
-      const int page = lp < n ? lookup_page(a.table, seq, lp, a.kv.num_pages, a.status) : -1;
-      known[x] = page >= 0;
-      bound[x] = reinterpret_cast<const B*>(a.kv.bounds) + ((int64_t)max(page, 0) * heads + head) * 2 * d;
+      // (a page that is not there reads the first page of the pool, whose scores are not kept)
+      const int page = max(0, __shfl_sync(0xffffffffu, now.my_page, x * 8 + r));
+      const B* bound = reinterpret_cast<const B*>(a.kv.bounds) + ((int64_t)page * heads + head) * 2 * d;
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int ch = (j * 4 + c) * 8;
+#pragma unroll
+        for (int y = 0; y < 2; ++y) raw[j][x][y] = ld_nc_v4(bound + y * d + (ch < d ? ch : 0));
+      }
     }
-    constexpr int HELD = 2;
-    uint4 raw[HELD][2][2];                                     // [step][page][lower, upper]
-    auto ask = [&](int j0) {
+    if (group > 8 || held_head != head || held_seq != now.seq) {
+      ask_queries(now, 0);
+      held_head = head;
+      held_seq = now.seq;
+    }
+    if (unit + 1 < unit_end) then = find(unit + 1);
 #pragma unroll
-      for (int j = 0; j < HELD; ++j) {
-        const int ch = ((j0 + j) * 4 + c) * 8;
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            raw[j][x][y] = make_uint4(0, 0, 0, 0);
-            if (known[x] && ch < d) raw[j][x][y] = __ldg(reinterpret_cast<const uint4*>(bound[x] + y * d + ch));
-          }
-      }
-    };
-    ask(0);
-    double best[2][2] = {{-INFINITY, -INFINITY}, {-INFINITY, -INFINITY}};
-    bool bad[2][2] = {{false, false}, {false, false}};         // a score that is not finite
-    for (int g0 = 0; g0 < group; g0 += 8) {
-      if (group > 8 || laid_out != head) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < J * 32; i += SCORE_WARPS * 32) {   // 8 channels of one query
-          const int row = i / (J * 4), piece = i % (J * 4);
-        float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (g0 + row < group && piece * 8 < d)
-          load8(reinterpret_cast<const T*>(a.q.data) + seq * a.q.row + (int64_t)(head * group + g0 + row) * a.q.head + piece * 8, x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          double* at = sm_q + ((piece >> 2) * 8 + e) * 32 + row * 4 + (piece & 3);
-          at[0] = x[e] > 0.0f ? (double)x[e] : 0.0;
-          at[J * 256] = x[e] > 0.0f ? 0.0 : (double)x[e];      // (a NaN query lands here)
-        }
-      }
-      laid_out = head;
-      __syncthreads();
-      }
-      // eight chains: a 64-bit product takes about 200 cycles to come back
-      double part[2][2][2][2] = {};                            // [page][sign][channel parity][element]
-      for (int j0 = 0; j0 < J; j0 += HELD) {
-        if (j0 > 0 || g0 > 0) ask(j0);
-#pragma unroll
-        for (int j = 0; j < HELD; ++j) {
-          const double* plus = sm_q + (j0 + j) * 256 + lane;
-#pragma unroll
-          for (int e2 = 0; e2 < 4; ++e2) {
-            float2 lo[2], hi[2];
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const uint32_t l[4] = {raw[j][x][0].x, raw[j][x][0].y, raw[j][x][0].z, raw[j][x][0].w};
-              const uint32_t h[4] = {raw[j][x][1].x, raw[j][x][1].y, raw[j][x][1].z, raw[j][x][1].w};
-              lo[x] = to_float2<B>(l[e2]);
-              hi[x] = to_float2<B>(h[e2]);
-            }
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              const double qp = plus[(2 * e2 + y) * 32], qm = plus[J * 256 + (2 * e2 + y) * 32];
-#pragma unroll
-              for (int x = 0; x < 2; ++x) {
-                mma_f64(part[x][0][y], qp, (double)(y ? hi[x].y : hi[x].x));
-                mma_f64(part[x][1][y], qm, (double)(y ? lo[x].y : lo[x].x));
-              }
-            }
-          }
-        }
-      }
-      double s[2][2];
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int y = 0; y < 2; ++y) s[x][y] = (part[x][0][0][y] + part[x][0][1][y]) + (part[x][1][0][y] + part[x][1][1][y]);
-      // the lane has query g0 + r and pages 2c, 2c + 1 of each 8
+    for (int j = 0; j < J; ++j)
 #pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
-          if (g0 + r >= group) continue;
-          bad[x][y] |= !(fabs(s[x][y]) <= 1.7976931348623157e308);
-          best[x][y] = fmax(best[x][y], s[x][y]);
+          const bool in = (j * 4 + c) * 8 < d;
+          uint4& v = raw[j][x][y];
+          v = make_uint4(in ? as_query_type<T, B>(v.x) : 0, in ? as_query_type<T, B>(v.y) : 0, in ? as_query_type<T, B>(v.z) : 0,
+                         in ? as_query_type<T, B>(v.w) : 0);
+        }
+    float best[2] = {-INFINITY, -INFINITY}, magnitude[2] = {0.0f, 0.0f};
+    for (int g0 = 0; g0 < group; g0 += 8) {
+      if (g0 > 0) ask_queries(now, g0);
+      float s[4] = {}, m[4] = {};
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const uint32_t qw[4] = {q[j].x, q[j].y, q[j].z, q[j].w};
+        uint32_t lo[2][4], hi[2][4], big[2][4];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const uint32_t l[4] = {raw[j][x][0].x, raw[j][x][0].y, raw[j][x][0].z, raw[j][x][0].w};
+          const uint32_t h[4] = {raw[j][x][1].x, raw[j][x][1].y, raw[j][x][1].z, raw[j][x][1].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            lo[x][i] = l[i];
+            hi[x][i] = h[i];
+            big[x][i] = max2<T>(lo[x][i] & 0x7fff7fffu, hi[x][i] & 0x7fff7fffu);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          const uint32_t al[4] = {lo[0][i], lo[1][i], lo[0][i + 1], lo[1][i + 1]}, ah[4] = {hi[0][i], hi[1][i], hi[0][i + 1], hi[1][i + 1]};
+          const uint32_t ab[4] = {big[0][i], big[1][i], big[0][i + 1], big[1][i + 1]};
+          float plus[4] = {}, minus[4] = {};
+          mma_16816<T>(plus, ah, max2<T>(qw[i], 0), max2<T>(qw[i + 1], 0));
+          mma_16816<T>(minus, al, min2<T>(qw[i], 0), min2<T>(qw[i + 1], 0));
+#pragma unroll
+          for (int x = 0; x < 4; ++x) s[x] += plus[x];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) s[x] += minus[x];
+          mma_16816<T>(m, ab, qw[i] & 0x7fff7fffu, qw[i + 1] & 0x7fff7fffu);
+        }
+      }
+      // the lane has pages r and r + 8, and queries g0 + 2c and g0 + 2c + 1
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          if (g0 + 2 * c + y >= group) continue;
+          const float v = s[2 * x + y], w = m[2 * x + y];
+          best[x] = fmaxf(best[x], v);
+          magnitude[x] = fabsf(v) <= FLT_MAX && w <= FLT_MAX ? fmaxf(magnitude[x], w) : INFINITY;
         }
     }
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
+    for (int x = 0; x < 2; ++x) {
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        double top = best[x][y];
-        unsigned any = bad[x][y];
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) {
-          top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
-          any |= __shfl_xor_sync(0xffffffffu, any, o);
-        }
-        const bool known_page = __shfl_sync(0xffffffffu, known[x], (2 * c + y) * 4);
-        const int lp = page0 + warp * 16 + x * 8 + 2 * c + y;
-        // a page outside the pool comes last: the attention would leave it out
-        if (r == 0 && lp < n) keys[entry * a.table.width + lp] = !known_page ? 0 : (any ? ~0ull : score_key(top));
+      for (int o = 1; o < 4; o <<= 1) {
+        best[x] = fmaxf(best[x], __shfl_xor_sync(0xffffffffu, best[x], o));
+        magnitude[x] = fmaxf(magnitude[x], __shfl_xor_sync(0xffffffffu, magnitude[x], o));
       }
+      const int lp = now.page0 + x * 8 + r;
+      const bool known = __shfl_sync(0xffffffffu, now.my_page, x * 8 + r) >= 0;
+      // a page outside the pool comes last (-infinity): the attention would leave it out
+      if (c == 0 && lp < now.n)
+        *reinterpret_cast<float2*>(scores + (now.seq * heads + head) * a.table.width + lp) =
+            known ? make_float2(magnitude[x] <= FLT_MAX ? best[x] : 0.0f, magnitude[x]) : make_float2(-INFINITY, 0.0f);
+    }
   }
+}
+
+// Exact key of a page (`lower`: its bounds) for one query, by one warp.
+template <typename T, typename B>
+__device__ __noinline__ unsigned long long exact_key(const T* q, const B* lower, int d) {
+  double s = 0.0;
+#pragma unroll 2
+  for (int i = (threadIdx.x & 31) * 2; i < d; i += 64) {
+    const float2 x = to_float2<T>(*reinterpret_cast<const uint32_t*>(q + i));
+    const float2 l = to_float2<B>(*reinterpret_cast<const uint32_t*>(lower + i)), h = to_float2<B>(*reinterpret_cast<const uint32_t*>(lower + d + i));
+    // (as two terms, one of them 0 times a bound: NaN when that is not finite)
+    s = fma((double)fmaxf(x.x, 0.0f), (double)h.x, fma((double)fminf(x.x, 0.0f), (double)l.x, s));
+    s = fma((double)fmaxf(x.y, 0.0f), (double)h.y, fma((double)fminf(x.y, 0.0f), (double)l.y, s));
+    if (x.x != x.x || x.y != x.y) s = INFINITY;
+  }
+#pragma unroll 1
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return score_key(s);
 }
 
 // Exclusive sums over `count` <= 256 numbers in shared memory, by one warp; returns the total.
@@ -469,15 +533,181 @@ __device__ __forceinline__ int scan256(int* x, int count) {
   return total;
 }
 
-// One block per (sequence, key head).  A radix selection from the first bit in which the keys differ: 8 bits at a time the
-// keys that share the threshold's leading bits are counted by their next digit, until all of them are wanted or all bits are
-// known; the last of them are then taken in the order of their pages.  A thread holds every blockDim-th key, up to ROWS of
-// them (ROWS is 8, or 0 for more pages than that: then they are read again for every pass).
-template <int ROWS>
-__global__ void __launch_bounds__(1024) select_kernel(const wush_kv_select_args a, const unsigned long long* keys) {
-  __shared__ int hist[256];
-  __shared__ unsigned long long sm_low[32], sm_high[32];
-  __shared__ int sm_digit, sm_need, sm_count;
+constexpr int BORDER = 256;                                  // pages between that are ranked in shared memory
+
+struct SelectShared {
+  int hist[256];
+  unsigned long long low[32], high[32];
+  int digit, need, count;
+  int sums[2][32];
+  int border[BORDER];
+  unsigned long long border_key[BORDER];
+};
+
+// What a radix selection found: the `need` first of the `among` keys that match the prefix, and all above it, are taken.
+template <typename K>
+struct Chosen {
+  K prefix;
+  int shift, need, among;
+  __device__ bool matches(K k) const { return shift == (int)sizeof(K) * 8 || k >> shift == prefix; }
+  __device__ bool above(K k) const { return shift < (int)sizeof(K) * 8 && k >> shift > prefix; }
+};
+
+// The `need` largest of `among` keys, from the first bit in which they differ: 8 bits at a time the keys that share the
+// threshold's leading bits are counted by their next digit, until all of them are wanted or all bits are known.
+// key(j) is the thread's j-th key, valid(j) whether it has one; ROWS rounds, or `rounds` where that is 0.
+template <typename K, int ROWS, class Key, class Valid>
+__device__ Chosen<K> radix_select(SelectShared& sm, int rounds, int need, int among, Key key, Valid valid) {
+  constexpr int BITS = (int)sizeof(K) * 8;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5;
+  const int end = ROWS > 0 ? ROWS : rounds;
+  K low = ~(K)0, high = 0;
+#pragma unroll
+  for (int j = 0; j < end; ++j)
+    if (valid(j)) {
+      const K k = key(j);
+      low = k < low ? k : low;
+      high = k > high ? k : high;
+    }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const K x = __shfl_xor_sync(0xffffffffu, low, o), y = __shfl_xor_sync(0xffffffffu, high, o);
+    low = x < low ? x : low;
+    high = y > high ? y : high;
+  }
+  __syncthreads();
+  if (lane == 0) {
+    sm.low[warp] = low;
+    sm.high[warp] = high;
+  }
+  __syncthreads();
+  for (int w = 0; w < warps; ++w) {
+    low = (K)sm.low[w] < low ? (K)sm.low[w] : low;
+    high = (K)sm.high[w] > high ? (K)sm.high[w] : high;
+  }
+  Chosen<K> c;
+  c.need = need;
+  c.among = among;
+  c.shift = low >= high ? 0 : 64 - __clzll((unsigned long long)low ^ (unsigned long long)high);   // bits that are not known
+  c.prefix = c.shift == BITS ? 0 : high >> c.shift;
+  while (c.need > 0 && c.need < c.among && c.shift > 0) {
+    const int bits = min(8, c.shift), next = c.shift - bits;
+    for (int i = tid; i < 256; i += threads) sm.hist[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < end; ++j)
+      if (valid(j)) {
+        const K k = key(j);
+        if (c.matches(k)) atomicAdd(&sm.hist[(int)(k >> next) & ((1 << bits) - 1)], 1);
+      }
+    __syncthreads();
+    if (warp == 0) {                                         // the digit that the need-th largest key has
+      int mine[8], sum = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += mine[i] = sm.hist[255 - (lane * 8 + i)];
+      int before = sum;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += y;
+      }
+      before -= sum;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (before < c.need && c.need <= before + mine[i]) {
+          sm.digit = 255 - (lane * 8 + i);
+          sm.need = c.need - before;
+          sm.count = mine[i];
+        }
+        before += mine[i];
+      }
+    }
+    __syncthreads();
+    c.prefix = (c.shift == BITS ? 0 : c.prefix << bits) | (K)sm.digit;
+    c.need = sm.need;
+    c.among = sm.count;
+    c.shift = next;
+    __syncthreads();
+  }
+  return c;
+}
+
+// Sums of two numbers over the block, for every thread.
+__device__ __forceinline__ int2 block_sums(SelectShared& sm, int x, int y) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  x = __reduce_add_sync(0xffffffffu, x);
+  y = __reduce_add_sync(0xffffffffu, y);
+  __syncthreads();
+  if (lane == 0) {
+    sm.sums[0][warp] = x;
+    sm.sums[1][warp] = y;
+  }
+  __syncthreads();
+  return make_int2(__reduce_add_sync(0xffffffffu, lane < warps ? sm.sums[0][lane] : 0),
+                   __reduce_add_sync(0xffffffffu, lane < warps ? sm.sums[1][lane] : 0));
+}
+
+// Writes the taken pages in ascending order: those with take(j), and the first `need` of the `among` with equal(j).  8 rounds
+// at a time; hist holds the counts of (round, warp): 8 * 32 at most.
+template <class Take, class Equal>
+__device__ void write_pages(SelectShared& sm, int rounds, int need, int among, Take take_of, Equal equal_of, int32_t* out) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5;
+  int taken_before = 0, equal_before = 0;
+  for (int j0 = 0; j0 < rounds; j0 += 8) {
+    unsigned equal = 0, take = 0;                            // one bit a round
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      equal |= (unsigned)equal_of(j0, x) << x;
+      take |= (unsigned)take_of(j0, x) << x;
+    }
+    if (need < among) {                                      // not all that match: by rank
+      __syncthreads();
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const unsigned m = __ballot_sync(0xffffffffu, equal >> x & 1);
+        if (lane == 0) sm.hist[x * warps + warp] = __popc(m);
+      }
+      __syncthreads();
+      if (warp == 0) {
+        const int total = scan256(sm.hist, 8 * warps);
+        if (lane == 0) sm.count = total;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const unsigned m = __ballot_sync(0xffffffffu, equal >> x & 1);
+        if ((equal >> x & 1) && equal_before + sm.hist[x * warps + warp] + __popc(m & ((1u << lane) - 1)) < need) take |= 1u << x;
+      }
+      equal_before += sm.count;
+    } else {
+      take |= equal;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const unsigned m = __ballot_sync(0xffffffffu, take >> x & 1);
+      if (lane == 0) sm.hist[x * warps + warp] = __popc(m);
+    }
+    __syncthreads();
+    if (warp == 0) {
+      const int total = scan256(sm.hist, 8 * warps);
+      if (lane == 0) sm.count = total;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const unsigned m = __ballot_sync(0xffffffffu, take >> x & 1);
+      if (take >> x & 1) out[taken_before + sm.hist[x * warps + warp] + __popc(m & ((1u << lane) - 1))] = (j0 + x) * threads + tid;
+    }
+    taken_before += sm.count;
+    __syncthreads();
+  }
+}
+
+// One block per (sequence, key head).  A thread holds every blockDim-th score, up to ROWS of them (ROWS is 8, or 0 for more
+// pages than that: then they are read again for every pass).
+template <typename T, typename B, int ROWS>
+__global__ void __launch_bounds__(1024) select_kernel(const wush_kv_select_args a, int group, Score* scores) {
+  __shared__ SelectShared sm;
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5;
@@ -492,142 +722,134 @@ __global__ void __launch_bounds__(1024) select_kernel(const wush_kv_select_args 
     for (int i = tid; i < n; i += threads) out[i] = i;
     return;
   }
-  const int begin = a.sink, end = n - a.recent;              // pages that compete
-  const unsigned long long* from = keys + item * a.table.width;
-  unsigned long long held[ROWS > 0 ? ROWS : 1];
-#pragma unroll
-  for (int j = 0; j < ROWS; ++j) {
-    const int i = j * threads + tid;
-    held[j] = i >= begin && i < end ? from[i] : 0;
-  }
+  const int begin = a.sink, end = n - a.recent, want = top - a.sink - a.recent;   // pages that compete
+  Score* mine = scores + item * a.table.width;
   const int rounds = ROWS > 0 ? ROWS : (n + threads - 1) / threads;
-  auto key_of = [&](int j) { return ROWS > 0 ? held[ROWS > 0 ? j : 0] : from[j * threads + tid]; };
-  auto competes = [&](int j) {
-    const int i = j * threads + tid;
-    return i >= begin && i < end;
-  };
-
-  // smallest and largest key: the bits before the first in which they differ need no passes
-  unsigned long long low = ~0ull, high = 0;
+  auto page_of = [&](int j) { return j * threads + tid; };
+  auto competes = [&](int j) { return page_of(j) >= begin && page_of(j) < end; };
+  auto forced = [&](int j) { return page_of(j) < n && !competes(j); };
+  auto load = [&](int j) { return *reinterpret_cast<const float2*>(mine + page_of(j)); };
+  uint32_t held[ROWS > 0 ? ROWS : 1];
+  float magnitude = 0.0f;
 #pragma unroll
-  for (int j = 0; j < rounds; ++j)
+  for (int j = 0; j < (ROWS > 0 ? ROWS : rounds); ++j)
     if (competes(j)) {
-      const unsigned long long k = key_of(j);
-      low = k < low ? k : low;
-      high = k > high ? k : high;
+      const float2 s = load(j);
+      if (ROWS > 0) held[ROWS > 0 ? j : 0] = float_key(s.x);
+      magnitude = fmaxf(magnitude, s.y);
     }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const unsigned long long x = __shfl_xor_sync(0xffffffffu, low, o), y = __shfl_xor_sync(0xffffffffu, high, o);
-    low = x < low ? x : low;
-    high = y > high ? y : high;
+  auto key_of = [&](int j) { return ROWS > 0 ? held[ROWS > 0 ? j : 0] : float_key(load(j).x); };
+  if (want == 0) {
+    for (int i = tid; i < top; i += threads) out[i] = i < begin ? i : n - top + i;
+    return;
   }
+  const Chosen<uint32_t> c = radix_select<uint32_t, ROWS>(sm, rounds, want, end - begin, key_of, competes);
+
+  // the k-th largest, the largest magnitude, and from them the pages above and between
+  uint32_t kth = ~0u;
+#pragma unroll
+  for (int j = 0; j < (ROWS > 0 ? ROWS : rounds); ++j)
+    if (competes(j)) {
+      const uint32_t k = key_of(j);
+      if (c.matches(k) || c.above(k)) kth = min(kth, k);
+    }
+  kth = __reduce_min_sync(0xffffffffu, kth);
+  const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(magnitude));       // (not negative: ordered as they are)
+  __syncthreads();
   if (lane == 0) {
-    sm_low[warp] = low;
-    sm_high[warp] = high;
+    sm.low[warp] = kth;
+    sm.high[warp] = most;
   }
   __syncthreads();
-  for (int w = 0; w < warps; ++w) {
-    low = sm_low[w] < low ? sm_low[w] : low;
-    high = sm_high[w] > high ? sm_high[w] : high;
-  }
-  int need = top - a.sink - a.recent, among = end - begin;   // wanted among the keys that match the prefix
-  int shift = low == high ? 0 : 64 - __clzll(low ^ high);    // bits of a key that are not known
-  unsigned long long prefix = shift == 64 ? 0 : high >> shift;
-  auto matches = [&](unsigned long long k) { return shift == 64 || k >> shift == prefix; };
-  while (need > 0 && need < among && shift > 0) {
-    const int bits = min(8, shift), next = shift - bits;
-    for (int i = tid; i < 256; i += threads) hist[i] = 0;
+  kth = __reduce_min_sync(0xffffffffu, lane < warps ? (uint32_t)sm.low[lane] : ~0u);
+  magnitude = __uint_as_float(__reduce_max_sync(0xffffffffu, lane < warps ? (uint32_t)sm.high[lane] : 0u));
+  // (17 + products / 2) * 2^-23 of the magnitude, and a sixteenth more for the magnitude's own rounding
+  const float eps = magnitude * (float)(17 + (a.kv.dim + 15) / 16) * (1.0625f / 8388608.0f);
+  const float center = key_float(kth), bottom = __fsub_rd(center, 2.0f * eps), roof = __fadd_ru(center, 2.0f * eps);
+  // a magnitude that is not finite leaves everything between (also where the k-th is a page outside the pool: all that are
+  // in it are above)
+  const bool sure = eps <= FLT_MAX && center >= -FLT_MAX;
+  auto is_above = [&](float v) { return sure ? v > roof : (eps <= FLT_MAX && v > center); };
+  auto is_between = [&](float v) { return sure ? v >= bottom && v <= roof : (eps <= FLT_MAX ? v == center : true); };
+  int n_above = 0, n_between = 0;
+#pragma unroll
+  for (int j = 0; j < (ROWS > 0 ? ROWS : rounds); ++j)
+    if (competes(j)) {
+      const float v = key_float(key_of(j));
+      n_above += is_above(v);
+      n_between += is_between(v);
+    }
+  const int2 sums = block_sums(sm, n_above, n_between);
+  const int need = want - sums.x, between = sums.y;
+  const int64_t seq = item / a.kv.heads;
+  const int head = (int)(item - seq * a.kv.heads);
+  const T* queries = reinterpret_cast<const T*>(a.q.data) + seq * a.q.row + (int64_t)head * group * a.q.head;
+  auto exact = [&](int lp, int g) {                          // 0 for a page outside the pool
+    const int page = lookup_page(a.table, seq, lp, a.kv.num_pages, a.status);
+    const B* lower = reinterpret_cast<const B*>(a.kv.bounds) + ((int64_t)max(page, 0) * a.kv.heads + head) * 2 * a.kv.dim;
+    const unsigned long long k = exact_key<T, B>(queries + g * a.q.head, lower, a.kv.dim);
+    return page < 0 ? 0ull : k;
+  };
+  const bool all_between = need == between;                  // the usual case: the k-th itself and nothing else
+  if (!all_between && between <= BORDER) {
+    // score the pages between again, rank them, and leave the verdict in place of their scores
     __syncthreads();
-#pragma unroll
-    for (int j = 0; j < rounds; ++j)
-      if (competes(j)) {
-        const unsigned long long k = key_of(j);
-        if (matches(k)) atomicAdd(&hist[(int)(k >> next) & ((1 << bits) - 1)], 1);
-      }
+    if (tid == 0) sm.count = 0;
+    for (int i = tid; i < between; i += threads) sm.border_key[i] = 0;
     __syncthreads();
-    if (warp == 0) {                                         // the digit that the need-th largest key has
-      int mine[8], sum = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sum += mine[i] = hist[255 - (lane * 8 + i)];
-      int before = sum;
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += y;
-      }
-      before -= sum;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (before < need && need <= before + mine[i]) {
-          sm_digit = 255 - (lane * 8 + i);
-          sm_need = need - before;
-          sm_count = mine[i];
-        }
-        before += mine[i];
-      }
+#pragma unroll 1
+    for (int i = begin + tid; i < end; i += threads)
+      if (is_between(mine[i].value)) sm.border[atomicAdd(&sm.count, 1)] = i;
+    __syncthreads();
+#pragma unroll 1
+    for (int i = warp; i < between * group; i += warps) {    // (page, query)
+      const unsigned long long k = exact(sm.border[i / group], i % group);
+      if (lane == 0) atomicMax(&sm.border_key[i / group], k);
     }
     __syncthreads();
-    prefix = (shift == 64 ? 0 : prefix << bits) | (unsigned)sm_digit;
-    need = sm_need;
-    among = sm_count;
-    shift = next;
-  }
-
-  // Take the keys above the prefix and the first `need` of those that match it; place them in the order of the pages, 8 rounds
-  // at a time.  hist holds the counts of (round, warp): 8 * 32 at most.
-  int taken_before = 0, equal_before = 0;
-  for (int j0 = 0; j0 < rounds; j0 += 8) {
-    unsigned equal = 0, take = 0;                            // one bit a round
-#pragma unroll
-    for (int x = 0; x < 8; ++x) {
-      const int j = j0 + x, i = j * threads + tid;
-      const bool in = need > 0 && competes(j);
-      const unsigned long long k = in ? key_of(ROWS > 0 ? x : j) : 0;
-      equal |= (unsigned)(in && matches(k)) << x;
-      take |= (unsigned)((i < n && (i < begin || i >= end)) || (in && shift < 64 && k >> shift > prefix)) << x;
+    for (int i = tid; i < between; i += threads) {
+      int better = 0;
+#pragma unroll 1
+      for (int o = 0; o < between; ++o)
+        better += sm.border_key[o] > sm.border_key[i] || (sm.border_key[o] == sm.border_key[i] && sm.border[o] < sm.border[i]);
+      mine[sm.border[i]].value = better < need ? INFINITY : -INFINITY;
     }
-    if (need < among) {                                      // not all that match: by rank
-      __syncthreads();
-#pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        const unsigned m = __ballot_sync(0xffffffffu, equal >> x & 1);
-        if (lane == 0) hist[x * warps + warp] = __popc(m);
-      }
-      __syncthreads();
-      if (warp == 0) {
-        const int total = scan256(hist, 8 * warps);
-        if (lane == 0) sm_count = total;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        const unsigned m = __ballot_sync(0xffffffffu, equal >> x & 1);
-        if ((equal >> x & 1) && equal_before + hist[x * warps + warp] + __popc(m & ((1u << lane) - 1)) < need) take |= 1u << x;
-      }
-      equal_before += sm_count;
-    } else {
-      take |= equal;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int x = 0; x < 8; ++x) {
-      const unsigned m = __ballot_sync(0xffffffffu, take >> x & 1);
-      if (lane == 0) hist[x * warps + warp] = __popc(m);
-    }
-    __syncthreads();
-    if (warp == 0) {
-      const int total = scan256(hist, 8 * warps);
-      if (lane == 0) sm_count = total;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int x = 0; x < 8; ++x) {
-      const unsigned m = __ballot_sync(0xffffffffu, take >> x & 1);
-      if (take >> x & 1) out[taken_before + hist[x * warps + warp] + __popc(m & ((1u << lane) - 1))] = (j0 + x) * threads + tid;
-    }
-    taken_before += sm_count;
+    __threadfence_block();
     __syncthreads();
   }
+  if (all_between || between <= BORDER) {
+    write_pages(sm, rounds, 0, 0, [&](int j0, int x) {
+      const int j = j0 + x;
+      if (!competes(j)) return forced(j);
+      const float v = key_float(key_of(ROWS > 0 ? x : j));   // (read again, without registers: the verdict already)
+      if (is_above(v) || (all_between && is_between(v))) return true;
+      if (ROWS == 0) return v == INFINITY;
+      return is_between(v) && *(volatile float*)&mine[page_of(j)].value == INFINITY;
+    }, [](int, int) { return false; }, out);
+    return;
+  }
+  // many between (equal pages, or magnitudes that are not finite): 64-bit keys in place of the scores, and another selection
+  unsigned long long* keys = reinterpret_cast<unsigned long long*>(mine);
+  for (int i = warp; i < n; i += warps) {
+    if (i < begin || i >= end) continue;
+    const float v = *(volatile float*)&mine[i].value;
+    unsigned long long k = is_above(v) ? ~0ull : 0;
+    if (is_between(v)) {
+      for (int g = 0; g < group; ++g) {
+        const unsigned long long x = exact(i, g);
+        k = k < x ? x : k;
+      }
+    }
+    __syncwarp();
+    if (lane == 0) keys[i] = k;
+  }
+  __threadfence_block();
+  __syncthreads();
+  const int all = (n + threads - 1) / threads;
+  auto wide_key = [&](int j) { return *(volatile unsigned long long*)&keys[page_of(j)]; };
+  const Chosen<unsigned long long> w = radix_select<unsigned long long, 0>(sm, all, want, end - begin, wide_key, competes);
+  write_pages(sm, all, w.need, w.among, [&](int j0, int x) { return competes(j0 + x) ? w.above(wide_key(j0 + x)) : forced(j0 + x); },
+              [&](int j0, int x) { return competes(j0 + x) && w.matches(wide_key(j0 + x)); }, out);
 }
 
 }  // namespace kv
@@ -718,8 +940,9 @@ extern "C" int wush_kv_select_pages(const wush_kv_select_args* args) {
   if (a.workspace_bytes < wush_kv_select_workspace_bytes(a.table.seqs, a.kv.heads, a.table.width)) return WUSH_ERR_WORKSPACE_TOO_SMALL;
   if (a.table.seqs * a.kv.heads > INT32_MAX) return WUSH_ERR_TOO_LARGE;
   if ((rc = require_sm100()) != 0) return rc;
-  unsigned long long* keys = reinterpret_cast<unsigned long long*>(a.workspace);
+  Score* scores = reinterpret_cast<Score*>(a.workspace);
   const int64_t units = a.table.seqs * a.kv.heads * ((a.table.width + SCORE_PAGES - 1) / SCORE_PAGES);
+  const int group = a.q_heads / a.kv.heads;
   // the kernels may be launched while the one before still runs, and wait for it before they read anything
   cudaLaunchAttribute early;
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -728,28 +951,24 @@ extern "C" int wush_kv_select_pages(const wush_kv_select_args* args) {
   cfg.stream = (cudaStream_t)a.stream;
   cfg.attrs = &early;
   cfg.numAttrs = 1;
-  cfg.blockDim = dim3(SCORE_WARPS * 32);
-  auto go = [&](auto kern, int steps) {
-    cfg.gridDim = dim3((unsigned)min(units, (int64_t)sm_count() * (steps <= 4 ? 4 : 3)));
-    cfg.dynamicSmemBytes = (size_t)steps * 512 * sizeof(double);
-    return (int)cudaLaunchKernelEx(&cfg, kern, a, a.q_heads / a.kv.heads, keys);
-  };
-  auto by_dim = [&](auto t, auto b) {
+  auto go = [&](auto t, auto b) {
     using T = decltype(t);
     using B = decltype(b);
-    return a.kv.dim <= 64 ? go(score_kernel<T, B, 2>, 2) : (a.kv.dim <= 128 ? go(score_kernel<T, B, 4>, 4) : go(score_kernel<T, B, 8>, 8));
+    const int per_sm = a.kv.dim <= 128 ? SCORE_BLOCKS : 2;
+    cfg.gridDim = dim3((unsigned)min((units + SCORE_WARPS - 1) / SCORE_WARPS, (int64_t)sm_count() * per_sm));
+    cfg.blockDim = dim3(SCORE_WARPS * 32);
+    auto kern = a.kv.dim <= 64 ? score_kernel<T, B, 2> : (a.kv.dim <= 128 ? score_kernel<T, B, 4> : score_kernel<T, B, 8>);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a, group, scores);
+    if (e != cudaSuccess) return (int)e;
+    // 8 scores a thread in registers while that is enough
+    int threads = 128;
+    while (threads < 1024 && threads * 8 < a.table.width) threads *= 2;
+    cfg.gridDim = dim3((unsigned)(a.table.seqs * a.kv.heads));
+    cfg.blockDim = dim3(threads);
+    return (int)cudaLaunchKernelEx(&cfg, threads * 8 >= a.table.width ? select_kernel<T, B, 8> : select_kernel<T, B, 0>, a, group, scores);
   };
   const __nv_bfloat16 bf = {};
   const __half hf = {};
-  if (a.type == WUSH_TYPE_BF16) rc = a.kv.bounds_type == WUSH_TYPE_BF16 ? by_dim(bf, bf) : by_dim(bf, hf);
-  else rc = a.kv.bounds_type == WUSH_TYPE_BF16 ? by_dim(hf, bf) : by_dim(hf, hf);
-  if (rc != 0) return rc;
-  // 8 keys a thread in registers while that is enough
-  int threads = 128;
-  while (threads < 1024 && threads * 8 < a.table.width) threads *= 2;
-  cfg.gridDim = dim3((unsigned)(a.table.seqs * a.kv.heads));
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = 0;
-  if (threads * 8 >= a.table.width) return (int)cudaLaunchKernelEx(&cfg, select_kernel<8>, a, (const unsigned long long*)keys);
-  return (int)cudaLaunchKernelEx(&cfg, select_kernel<0>, a, (const unsigned long long*)keys);
+  if (a.type == WUSH_TYPE_BF16) return a.kv.bounds_type == WUSH_TYPE_BF16 ? go(bf, bf) : go(bf, hf);
+  return a.kv.bounds_type == WUSH_TYPE_BF16 ? go(hf, bf) : go(hf, hf);
 }
