@@ -31,7 +31,7 @@ namespace kv {
 
 constexpr int WARPS = 4;
 constexpr int START = 4;                // units that an item is worth beyond its tokens
-constexpr int MIN_UNITS = 2;            // smallest number of units a block takes while others idle
+constexpr int MIN_UNITS = 1;            // smallest number of units a block takes while others idle
 constexpr int WHOLE_UNITS = 4;          // items of at most this many units are not split at all
 
 struct AttentionParams {
@@ -265,6 +265,7 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS)
     __syncthreads();
   }
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
 
   // Row r of a product is token token_row(r) of its 16 and lane 4 r + c reads piece piece_of(r) of a value row: with these
   // orders no two lanes that read together meet in a bank.
@@ -754,7 +755,8 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const AttentionPa
 #pragma unroll
     for (int x = 0; x < JOIN_ROWS; ++x) {
       const int i = base + warp + x * JOIN_WARPS;
-      const float2* from = reinterpret_cast<const float2*>(p.part_o + slot_of(min(i, parts - 1)) * DP) + lane;
+      if (i >= parts) break;
+      const float2* from = reinterpret_cast<const float2*>(p.part_o + slot_of(i) * DP) + lane;
 #pragma unroll
       for (int j = 0; j < E; ++j) row[x][j] = from[j * 32];
     }
@@ -776,11 +778,10 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const AttentionPa
 #pragma unroll
     for (int x = 0; x < JOIN_ROWS; ++x) {
       const int i = warp + x * JOIN_WARPS;
+      if (base + i >= parts) break;
       const float w = __shfl_sync(0xffffffffu, weight, i);
-      if (base + i < parts) {
 #pragma unroll
-        for (int j = 0; j < E; ++j) o[j] = make_float2(fmaf(row[x][j].x, w, o[j].x), fmaf(row[x][j].y, w, o[j].y));
-      }
+      for (int j = 0; j < E; ++j) o[j] = make_float2(fmaf(row[x][j].x, w, o[j].x), fmaf(row[x][j].y, w, o[j].y));
     }
   }
 #pragma unroll
@@ -811,26 +812,13 @@ static int launch(AttentionParams p, const CUtensorMap& k_map, const CUtensorMap
   const int64_t items = p.entries * (p.pages ? p.chunks : p.kv.heads * p.chunks);
   const int64_t most_units = (most_tokens + S::UNIT - 1) / S::UNIT;
   p.whole = most_units <= WHOLE_UNITS;
-  if (p.whole) {
-    kern<<<(unsigned)items, WARPS * 32, smem, stream>>>(p, k_map, v_map);
-    return (int)cudaGetLastError();
-  }
   const int64_t most_blocks = (items * most_units + MIN_UNITS - 1) / MIN_UNITS;
-  const int blocks = (int)min((int64_t)grid_blocks(DP, (int)sizeof(C), NT), most_blocks);
-  kern<<<blocks, WARPS * 32, smem, stream>>>(p, k_map, v_map);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess || blocks == 1) return (int)e;
-  // the join's launch overlaps the end of the attention, for which it waits
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(blocks - 1, min(S::HEADS, p.group));
-  cfg.blockDim = dim3(JOIN_WARPS * 32);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return (int)cudaLaunchKernelEx(&cfg, join_kernel<T, C, DP, NT>, p);
+  const int blocks = p.whole ? (int)items : (int)min((int64_t)grid_blocks(DP, (int)sizeof(C), NT), most_blocks);
+  // both launches overlap the end of the kernel before them, for which they wait
+  EarlyLaunch early(stream);
+  const cudaError_t e = cudaLaunchKernelEx(early.config(dim3(blocks), WARPS * 32, smem), kern, p, k_map, v_map);
+  if (e != cudaSuccess || p.whole || blocks == 1) return (int)e;
+  return (int)cudaLaunchKernelEx(early.config(dim3(blocks - 1, min(S::HEADS, p.group)), JOIN_WARPS * 32, 0), join_kernel<T, C, DP, NT>, p);
 }
 
 // Tensor map over a pool: boxes of 16 rows of at most 128 bytes of one head of one page.  (Lines are promoted to 128 bytes in

@@ -36,6 +36,8 @@ __device__ __forceinline__ void widen8(uint4 v, float (&x)[8]) {
 constexpr int APPEND_BATCH = 5, APPEND_THREADS = 128;
 template <typename T, typename C>
 __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendParams p, int span) {
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
   const int d = p.kv.dim, units = (d + 15) >> 4, lanes = APPEND_THREADS / units, turned = p.rotary >> 4;
   const int u = threadIdx.x % units, lane = threadIdx.x / units;
   if (lane >= lanes) return;
@@ -157,6 +159,8 @@ constexpr int BOUNDS_ROWS = 8, BOUNDS_SPAN = 8;
 template <typename C, typename B>
 __global__ void __launch_bounds__(128) bounds_kernel(const wush_kv_pages kv, const wush_kv_table table, const int32_t* seq_lens,
                                                      int64_t new_tokens, int64_t most, int span, int* status) {
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
   constexpr int CH = 16 / (int)sizeof(C), PAIRS = CH / 2;    // channels of a lane
   using P = typename std::conditional<std::is_same<C, __nv_bfloat16>::value, __nv_bfloat16, __half>::type;
   const int lane = threadIdx.x & 31;
@@ -708,7 +712,7 @@ __device__ void write_pages(SelectShared& sm, int rounds, int need, int among, T
 template <typename T, typename B, int ROWS>
 __global__ void __launch_bounds__(1024) select_kernel(const wush_kv_select_args a, int group, Score* scores) {
   __shared__ SelectShared sm;
-  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  // (no early launch of what follows: an attention that waits on the SMs slowed this kernel down by 1.5 us)
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5;
   const int64_t item = blockIdx.x;
@@ -885,8 +889,7 @@ extern "C" int wush_kv_append(const wush_kv_append_args* args) {
   const int span = p.rows >= sms ? all_heads : lanes;
   const dim3 grid((unsigned)min(p.rows, (int64_t)sms * 4), (all_heads + span - 1) / span);
   auto go = [&](auto kern) {
-    kern<<<grid, APPEND_THREADS, 0, (cudaStream_t)p.stream>>>(p, span);
-    return (int)cudaGetLastError();
+    return (int)cudaLaunchKernelEx(EarlyLaunch((cudaStream_t)p.stream).config(grid, APPEND_THREADS, 0), kern, p, span);
   };
   if (p.type == WUSH_TYPE_BF16)
     return p.kv.type == WUSH_TYPE_E4M3 ? go(append_kernel<__nv_bfloat16, __nv_fp8_e4m3>) : go(append_kernel<__nv_bfloat16, __nv_bfloat16>);
@@ -913,8 +916,8 @@ extern "C" int wush_kv_bounds(const wush_kv_bounds_args* args) {
   const int64_t warps = table.seqs * ((most + span - 1) / span) * kv.heads;
   const unsigned grid = (unsigned)min((warps + 3) / 4, (int64_t)sms * 64);
   auto go = [&](auto kern) {
-    kern<<<grid, 128, 0, (cudaStream_t)args->stream>>>(kv, table, args->seq_lens, args->new_tokens, most, span, args->status);
-    return (int)cudaGetLastError();
+    return (int)cudaLaunchKernelEx(EarlyLaunch((cudaStream_t)args->stream).config(dim3(grid), 128, 0), kern, kv, table, args->seq_lens,
+                                   args->new_tokens, most, span, args->status);
   };
   if (kv.type == WUSH_TYPE_BF16) return go(bounds_kernel<__nv_bfloat16, __nv_bfloat16>);
   if (kv.type == WUSH_TYPE_FP16) return go(bounds_kernel<__half, __half>);
@@ -943,29 +946,19 @@ extern "C" int wush_kv_select_pages(const wush_kv_select_args* args) {
   Score* scores = reinterpret_cast<Score*>(a.workspace);
   const int64_t units = a.table.seqs * a.kv.heads * ((a.table.width + SCORE_PAGES - 1) / SCORE_PAGES);
   const int group = a.q_heads / a.kv.heads;
-  // the kernels may be launched while the one before still runs, and wait for it before they read anything
-  cudaLaunchAttribute early;
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.stream = (cudaStream_t)a.stream;
-  cfg.attrs = &early;
-  cfg.numAttrs = 1;
+  EarlyLaunch early((cudaStream_t)a.stream);
   auto go = [&](auto t, auto b) {
     using T = decltype(t);
     using B = decltype(b);
     const int per_sm = a.kv.dim <= 128 ? SCORE_BLOCKS : 2;
-    cfg.gridDim = dim3((unsigned)min((units + SCORE_WARPS - 1) / SCORE_WARPS, (int64_t)sm_count() * per_sm));
-    cfg.blockDim = dim3(SCORE_WARPS * 32);
+    const dim3 grid((unsigned)min((units + SCORE_WARPS - 1) / SCORE_WARPS, (int64_t)sm_count() * per_sm));
     auto kern = a.kv.dim <= 64 ? score_kernel<T, B, 2> : (a.kv.dim <= 128 ? score_kernel<T, B, 4> : score_kernel<T, B, 8>);
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a, group, scores);
+    const cudaError_t e = cudaLaunchKernelEx(early.config(grid, SCORE_WARPS * 32, 0), kern, a, group, scores);
     if (e != cudaSuccess) return (int)e;
     // 8 scores a thread in registers while that is enough
     int threads = 128;
     while (threads < 1024 && threads * 8 < a.table.width) threads *= 2;
-    cfg.gridDim = dim3((unsigned)(a.table.seqs * a.kv.heads));
-    cfg.blockDim = dim3(threads);
-    return (int)cudaLaunchKernelEx(&cfg, threads * 8 >= a.table.width ? select_kernel<T, B, 8> : select_kernel<T, B, 0>, a, group, scores);
+    return (int)cudaLaunchKernelEx(early.config(dim3((unsigned)(a.table.seqs * a.kv.heads)), threads, 0), threads * 8 >= a.table.width ? select_kernel<T, B, 8> : select_kernel<T, B, 0>, a, group, scores);
   };
   const __nv_bfloat16 bf = {};
   const __half hf = {};

@@ -58,6 +58,26 @@ inline int check_pages(const wush_kv_pages* kv, const wush_kv_table* t, int type
   return WUSH_OK;
 }
 
+// Launch of a kernel that may start while the one before it in the stream still runs.  Such a kernel executes
+// griddepcontrol.wait in every thread before it touches global memory, and before any of its blocks ends.
+struct EarlyLaunch {
+  cudaLaunchAttribute attribute;
+  cudaLaunchConfig_t cfg;
+  explicit EarlyLaunch(cudaStream_t stream) : attribute{}, cfg{} {
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    cfg.stream = stream;
+    cfg.attrs = &attribute;
+    cfg.numAttrs = 1;
+  }
+  const cudaLaunchConfig_t* config(dim3 grid, int threads, size_t smem) {
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    return &cfg;
+  }
+};
+
 // ---- element types -----------------------------------------------------------------------------------------------
 template <typename T>
 __device__ __forceinline__ float2 to_float2(uint32_t two);
