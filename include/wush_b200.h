@@ -496,7 +496,8 @@ WUSH_API int wush_gptq_block_prepare(const double* gram, const double* basis, in
  *               multiples of 16 bytes
  *   type        WUSH_TYPE_BF16 / WUSH_TYPE_FP16 / WUSH_TYPE_E4M3
  *   dim         multiple of 8 (of 16 for E4M3), at most 256
- *   k_scale, v_scale  fp32 [heads] (DEVICE) for E4M3: the value is the stored number times the scale; null otherwise
+ *   k_scale, v_scale  fp32 [heads] (DEVICE), positive, for E4M3: the value is the stored number times the scale; null
+ *               otherwise
  *   bounds      null, or contiguous [num_pages, heads, 2, dim] of bounds_type (BF16 / FP16), 16-byte aligned: smallest
  *               and largest stored key of every channel over the filled rows of the page
  */

@@ -612,6 +612,46 @@ def test_another_stream_and_captured_graphs():
     _status_clear()
 
 
+def test_operators_captured_behind_copies_and_fills():
+    """The kernels may start while the one before them ends; in a graph that one can also be a copy or a memset."""
+    from wush_b200 import paged_kv
+    heads, kv, dim = 8, 2, 64
+    s = Setup([700, 33, 5], page=16, kv=kv, dim=dim, bounds=True, seed=41)
+    rope = paged_kv.rope_table(1024, dim, device=_dev())
+    ids = torch.arange(3, dtype=torch.int32, device=_dev())
+    src = [_randn(s.g, 3, heads + 2 * kv, dim).to(BF) for _ in range(3)]
+    x = torch.empty_like(src[0])
+    lens = s.seq_lens.clone()
+
+    def step():
+        y = torch.empty_like(x)
+        y.copy_(x)                                             # a device-to-device copy in front of the append's fill
+        q = paged_kv.paged_kv_append(s.cache, y[:, heads:heads + kv], y[:, heads + kv:], s.table, ids, lens - 1, q=y[:, :heads], rope=rope)
+        s.cache.bounds[int(0)].copy_(s.cache.bounds[int(0)].clone())
+        paged_kv.paged_kv_bounds(s.cache, s.table, lens)
+        z = torch.zeros(3, heads, dim, dtype=BF, device=_dev())
+        out = paged_kv.paged_decode_attention(q, s.cache, s.table, lens, out=z)
+        w = torch.zeros(4096, device=_dev())
+        pages, counts = paged_kv.paged_select_pages(q, s.cache, s.table, lens, 5)
+        w.zero_()
+        return out, pages, counts, paged_kv.paged_decode_attention(q, s.cache, s.table, lens, pages=pages, counts=counts)
+    want = []
+    for v in src:
+        x.copy_(v)
+        want.append([t.clone() for t in step()])
+    x.copy_(src[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(2):
+        for v, w in zip(src, want):
+            x.copy_(v)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, w))
+    _status_clear()
+
+
 def test_refusals():
     from wush_b200 import paged_kv
     s = Setup([40, 20], page=16, kv=2, dim=64, bounds=True)

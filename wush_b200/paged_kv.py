@@ -59,7 +59,7 @@ class PagedKVCache:
     float8_e4m3fn, with unit channel stride and any order of the other axes (``allocate(layout="hnd")`` keeps a head's
     rows of a page together).  head_dim is a multiple of 8 (16 for 8-bit pages) and at most 256.
 
-    8-bit pages hold key / k_scale and value / v_scale (float32 [n_kv_heads], given by the caller).  ``bounds``
+    8-bit pages hold key / k_scale and value / v_scale (float32 [n_kv_heads], positive, given by the caller).  ``bounds``
     [num_pages, n_kv_heads, 2, head_dim] (bfloat16 or float16; the type of 16-bit pages) is what ``paged_kv_bounds``
     fills and ``paged_select_pages`` reads.  The object keeps references to its tensors; replacing them needs a new one."""
 
@@ -227,7 +227,9 @@ def _on_its_device(op):
     def run(*args, **kwargs):
         cache = kwargs.get("cache")
         if cache is None:
-            cache = next(a for a in args if isinstance(a, PagedKVCache))
+            cache = next((a for a in args if isinstance(a, PagedKVCache)), None)
+            if cache is None:
+                raise TypeError(f"{op.__name__} needs a PagedKVCache")
         if torch.cuda.current_device() == cache._index:
             return op(*args, **kwargs)
         with torch.cuda.device(cache._index):
