@@ -32,7 +32,7 @@ namespace kv {
 constexpr int WARPS = 4;
 constexpr int START = 4;                // units that an item is worth beyond its tokens
 constexpr int MIN_UNITS = 1;            // smallest number of units a block takes while others idle
-constexpr int WHOLE_UNITS = 4;          // items of at most this many units are not split at all
+constexpr int WHOLE_UNITS = 8;          // items of at most this many units are not split at all
 
 struct AttentionParams {
   wush_kv_pages kv;
