@@ -1,8 +1,7 @@
 // Attention of one new token per sequence over a paged key-value cache: out = softmax(scale * q K^T) V.
 //
-// The kernel reads every key and value once and does 4 * G * bytes-worth of multiplications with them (G = query heads
-// that share a key head), so it is bound by HBM as long as the products run on the tensor cores and enough loads are in
-// flight.  Two decisions follow:
+// The kernel reads every key and value once and does G multiply-adds with each (G = query heads that share a key head), so it
+// is bound by HBM as long as the products run on the tensor cores and enough loads are in flight.
 //
 // Products.  All G queries of a key head are worked on together, with the tokens as the rows of m16n8k16 products:
 //     S^T [16 tokens x 8 heads] = K [16 tokens x 16 channels] . Q^T,     O^T [16 channels x 8 heads] += V^T . P^T.
@@ -14,12 +13,12 @@
 //
 // Copies.  Every warp has a ring of three tiles in shared memory, filled two tiles ahead by bulk tensor copies (16 rows of one
 // head of a page are one box), so a warp needs one instruction for 2 KB and no registers for what is in flight.  Measured on
-// 64 ragged sequences of up to 4096 tokens (364 MB): fragments straight into registers 110 us, per-lane 16-byte copies 90 us,
-// boxes 70 us.
+// 64 ragged sequences of up to 4096 tokens (364 MB), each with the work dealt as it was then: fragments straight into registers
+// 110 us, per-lane 16-byte copies 90 us, boxes 70 us (now 67: 84 % of the copy bandwidth; 6.65 TB/s on one of 500 000 tokens).
 //
 // Work.  The tokens of all (sequence, key head, chunk of queries) items are cut into units of 4 tiles (one per warp), the
 // units of all items are numbered through, and every block of a grid that fills the GPU exactly once takes an equal run
-// of them; lengths are read on the device.  A block that holds a whole item writes its result; a part of an item goes to
+// of them, teams of blocks the same run for neighbouring key heads; lengths are read on the device.  A block that holds a whole item writes its result; a part of an item goes to
 // the workspace, and a second kernel joins the parts (every block has at most two: its first and its last item).
 #include <type_traits>
 
@@ -30,9 +29,13 @@ namespace wush {
 namespace kv {
 
 constexpr int WARPS = 4;
-constexpr int START = 4;                // units that an item is worth beyond its tokens
-constexpr int MIN_UNITS = 1;            // smallest number of units a block takes while others idle
-constexpr int WHOLE_UNITS = 8;          // items of at most this many units are not split at all
+// Units that an item is worth beyond its tokens (64 ragged sequences up to 4096: 1 81 us, 2 75 us, 4 and 6 70 us).
+constexpr int START = 4;
+// Smallest number of units a block takes while others idle (a window of 1000 over 19 sequences: 1 13.1 us, 2 14.1 us).
+constexpr int MIN_UNITS = 1;
+// Items of at most this many units are not split: one launch instead of two (8 sequences of 512 tokens, 8 units: whole 9.3 us,
+// split 12.0 us; one of 1024, 16 units: whole 14.3 us, split 10.5 us).
+constexpr int WHOLE_UNITS = 8;
 
 struct AttentionParams {
   wush_kv_pages kv;
@@ -50,6 +53,7 @@ struct AttentionParams {
   int64_t window;
   int q_heads, group, chunks, top;
   int whole;                            // one block per item, no parts
+  int team;                             // neighbouring blocks that walk the same tokens of as many key heads
   int64_t entries;                      // sequences, or (sequence, key head) pairs when pages are selected
 };
 
@@ -66,7 +70,7 @@ __host__ __device__ constexpr int blocks_per_sm(int dp, int esize, int nt) {
 template <typename T, typename C, int DP, int NT>
 struct Shape {
   static constexpr bool E8 = sizeof(C) == 1;
-  // tokens a warp holds at a time: 4 KB of keys and as much of values, in 32 + 32 registers of a lane (128 channels)
+  // tokens of a warp's tile: 4 KB of keys and as much of values (128 channels)
   static constexpr int TT = tile_tokens(DP, (int)sizeof(C));
   static constexpr int MT = TT / 16;
   static constexpr int KJ = DP * (int)sizeof(C) / 64;       // 16-byte pieces of a key row per lane
@@ -94,6 +98,8 @@ struct Shape {
   static_assert(RING >= HEADS * PITCH * 4, "the ring also holds a warp's part of the result");
 };
 
+// Tiles of 8 query heads a block works on: two where a key head has more than 8 (16 queries a key head, 4096 tokens: two
+// 55.3 us, one and every key read twice 58.7 us), one at 256 channels for the registers.
 __host__ __device__ inline int pad_dim(int d) { return d <= 64 ? 64 : (d <= 128 ? 128 : 256); }
 __host__ __device__ inline int head_tiles(int dp, int group) { return dp == 256 || group <= 8 ? 1 : 2; }
 
@@ -276,6 +282,7 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS)
   const int v_0 = swizzled<S::PITCH_B>(c * S::PITCH_B + piece * S::VB), v_4 = swizzled<S::PITCH_B>((c + 4) * S::PITCH_B + piece * S::VB);
   const int v_8 = swizzled<S::PITCH_B>((c + 8) * S::PITCH_B + piece * S::VB), v_12 = swizzled<S::PITCH_B>((c + 12) * S::PITCH_B + piece * S::VB);
 
+  const int teams = p.whole ? copies : copies / p.team, member = p.whole ? 0 : blockIdx.x % p.team;   // teams' items an entry has
   int64_t t, t_end, t_first;
   Place at;
   if (p.whole) {
@@ -284,25 +291,25 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS)
     t = t_first = (int64_t)(blockIdx.x % copies) * (START + at.units);
     t_end = t + START + at.units;
   } else {
-    const int64_t total = total_units<FAST, S::UNIT>(p, copies);
-    const int64_t per = units_per_block(total, gridDim.x);
-    t = t_first = (int64_t)blockIdx.x * per;
+    const int64_t total = total_units<FAST, S::UNIT>(p, teams);
+    const int64_t per = units_per_block(total, gridDim.x / p.team);
+    t = t_first = (int64_t)(blockIdx.x / p.team) * per;
     t_end = min(total, t + per);
     if (threadIdx.x == 0) p.splits[2 * blockIdx.x].w = 0;
     if (t >= t_end) return;
-    at = locate<FAST, S::UNIT>(p, copies, t);
+    at = locate<FAST, S::UNIT>(p, teams, t);
   }
 
   int stage = 0;                                             // of the ring, for the tile that is worked on next
   uint32_t parity = 0;
   for (int64_t t_next; t < t_end; t = t_next) {
-    if (t >= at.base + (START + at.units) * copies) {        // the next entry
-      at.base += (START + at.units) * copies;
+    if (t >= at.base + (START + at.units) * teams) {         // the next entry
+      at.base += (START + at.units) * teams;
       at.entry += 1;
       at.units = units_of<FAST, S::UNIT>(p, at.entry);
     }
-    const int64_t copy = (t - at.base) / (START + at.units);
-    const int64_t within = t - at.base - copy * (START + at.units);
+    const int64_t its_team = (t - at.base) / (START + at.units), copy = p.whole ? its_team : its_team * p.team + member;
+    const int64_t within = t - at.base - its_team * (START + at.units);
     t_next = t + min(START + at.units - within, t_end - t);
     const int64_t u0 = max((int64_t)0, within - START), u1 = within + (t_next - t) - START;
     if (u1 <= u0) continue;                                  // only the item's START: the next block has its first tokens
@@ -316,25 +323,26 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS)
     constexpr int STEP = S::UNIT;
     const int first = (int)u0 * S::UNIT + warp * TT;         // the warp's tiles are first, first + STEP, ... below s1
     // A lookup goes in levels, each of which loads for the next: walked token -> logical page and row -> physical page.
-    struct Row { int page, row, pos; };                      // page -1: outside the table, -2: nothing there
+    struct Row { int page, row, pos; };
+    constexpr int NOTHING = INT32_MIN;                       // page of a token that is not there
     auto logical = [&](int v) -> Row {
-      if (v >= s1) return {-2, 0, 0};
+      if (v >= s1) return {NOTHING, 0, 0};
       const int at_v = v + w.origin, li = at_v / page_size, row = at_v - li * page_size;
       if (!list) return {li, row, at_v};
       const int lp = list[li];
       if (lp < 0 || lp >= p.table.width) {
         report_index(p.status);
-        return {-2, 0, 0};
+        return {NOTHING, 0, 0};
       }
       return {lp, row, lp * page_size + row};
     };
-    auto physical = [&](Row x) -> Row { return {x.page >= 0 && x.pos < w.len ? table[x.page] : -2, x.row, x.pos}; };
+    auto physical = [&](Row x) -> Row { return {x.page >= 0 && x.pos < w.len ? table[x.page] : NOTHING, x.row, x.pos}; };
     // the current page (0 where there is none) and row, and the tokens that count: one, or with FAST the 16 from there
     int page = 0, page_row = 0;
     unsigned counts16 = 0;
     auto resolve = [&](Row x) {
       const bool ok = x.page >= 0 && x.page < p.kv.num_pages;
-      if (!ok && x.page != -2) report_index(p.status);
+      if (!ok && x.page != NOTHING) report_index(p.status);
       page = ok ? x.page : 0;
       page_row = ok ? x.row : 0;
       const int lo = max(0, w.begin - x.pos), hi = min(16, w.len - x.pos);
@@ -732,7 +740,7 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS)
 
 // ---- join of the parts -------------------------------------------------------------------------------------------------
 // Block (k, h) joins the parts of the item that block k of the attention left unfinished, for query head h of its chunk: the
-// first part is block k's, the others are in slot 0 of the blocks after it.  32 parts at a time, eight a warp, all loaded
+// first part is block k's, the others are in slot 0 of the same member of the teams after it.  32 parts at a time, eight a warp, all loaded
 // before the first is used: the kernel is a chain of latencies (note, parts, result).
 constexpr int JOIN_WARPS = 4, JOIN_ROWS = 32 / JOIN_WARPS;
 template <typename T, typename C, int DP, int NT>
@@ -745,7 +753,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const AttentionPa
   const int4 item = p.splits[2 * blockIdx.x], more = p.splits[2 * blockIdx.x + 1];
   if (h >= item.w) return;
   const int parts = more.x;
-  auto slot_of = [&](int i) { return (2 * ((int64_t)blockIdx.x + i) + (i == 0 ? more.y : 0)) * S::HEADS + h; };
+  auto slot_of = [&](int i) { return (2 * ((int64_t)blockIdx.x + i * p.team) + (i == 0 ? more.y : 0)) * S::HEADS + h; };
   float top = -INFINITY, total = 0.0f;
   float2 o[E];
 #pragma unroll
@@ -812,13 +820,20 @@ static int launch(AttentionParams p, const CUtensorMap& k_map, const CUtensorMap
   const int64_t items = p.entries * (p.pages ? p.chunks : p.kv.heads * p.chunks);
   const int64_t most_units = (most_tokens + S::UNIT - 1) / S::UNIT;
   p.whole = most_units <= WHOLE_UNITS;
+  // Teams of up to 8 neighbouring key heads: their rows lie next to each other in token-major pages, and read together they
+  // come faster (one sequence of 131071 in E4M3: 53 us, each head by itself 58 us).  Selected pages differ from head to head.
+  p.team = 1;
+  if (!p.pages && !p.whole)
+    for (int g = 2; g <= 8; ++g)
+      if (p.kv.heads * p.chunks % g == 0) p.team = g;
   const int64_t most_blocks = (items * most_units + MIN_UNITS - 1) / MIN_UNITS;
-  const int blocks = p.whole ? (int)items : (int)min((int64_t)grid_blocks(DP, (int)sizeof(C), NT), most_blocks);
+  int blocks = p.whole ? (int)items : (int)min((int64_t)grid_blocks(DP, (int)sizeof(C), NT), most_blocks);
+  blocks -= blocks % p.team;                                 // (not 0: there are as many items as a team has members)
   // both launches overlap the end of the kernel before them, for which they wait
   EarlyLaunch early(stream);
   const cudaError_t e = cudaLaunchKernelEx(early.config(dim3(blocks), WARPS * 32, smem), kern, p, k_map, v_map);
-  if (e != cudaSuccess || p.whole || blocks == 1) return (int)e;
-  return (int)cudaLaunchKernelEx(early.config(dim3(blocks - 1, min(S::HEADS, p.group)), JOIN_WARPS * 32, 0), join_kernel<T, C, DP, NT>, p);
+  if (e != cudaSuccess || p.whole || blocks == p.team) return (int)e;
+  return (int)cudaLaunchKernelEx(early.config(dim3(blocks - p.team, min(S::HEADS, p.group)), JOIN_WARPS * 32, 0), join_kernel<T, C, DP, NT>, p);
 }
 
 // Tensor map over a pool: boxes of 16 rows of at most 128 bytes of one head of one page.  (Lines are promoted to 128 bytes in
@@ -836,8 +851,8 @@ inline bool make_pool_map(CUtensorMap* map, const wush_kv_pages& kv, void* base,
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Boxes where pages are made of whole groups of 16 tokens and the strides can be described (a stride of 0 cannot), rows
-// piece by piece otherwise.
+// Boxes where pages are made of whole groups of 16 tokens and a tensor map can describe the strides, rows piece by piece
+// otherwise (64 sequences of 1024: boxes 52.1 us, pieces 54.5 us; 32 ragged ones 16.4 and 18.7 us).
 template <typename T, typename C, int DP, int NT>
 static int by_page(const AttentionParams& p, int64_t most_tokens, cudaStream_t stream) {
   CUtensorMap k_map{}, v_map{};
