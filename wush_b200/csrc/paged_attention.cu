@@ -34,7 +34,8 @@ constexpr int START = 4;
 // Smallest number of units a block takes while others idle (a window of 1000 over 19 sequences: 1 13.1 us, 2 14.1 us).
 constexpr int MIN_UNITS = 1;
 // Items of at most this many units are not split: one launch instead of two (8 sequences of 512 tokens, 8 units: whole 9.3 us,
-// split 12.0 us; one of 1024, 16 units: whole 14.3 us, split 10.5 us).
+// split 12.0 us; one of 1024, 16 units: whole 14.3 us, split 10.5 us).  Twice as many where every SM has an item (64 of 1024:
+// whole 47 us, split 52 us), but not over selected pages (24 sequences with 128 of 16 tokens: 69 and 64 us).
 constexpr int WHOLE_UNITS = 8;
 
 struct AttentionParams {
@@ -819,7 +820,7 @@ static int launch(AttentionParams p, const CUtensorMap& k_map, const CUtensorMap
   if (const int rc = opt_in_smem(opted, kern, smem)) return rc;
   const int64_t items = p.entries * (p.pages ? p.chunks : p.kv.heads * p.chunks);
   const int64_t most_units = (most_tokens + S::UNIT - 1) / S::UNIT;
-  p.whole = most_units <= WHOLE_UNITS;
+  p.whole = most_units <= (items >= sm_count() && !p.pages ? 2 * WHOLE_UNITS : WHOLE_UNITS);
   // Teams of up to 8 neighbouring key heads: their rows lie next to each other in token-major pages, and read together they
   // come faster (one sequence of 131071 in E4M3: 53 us, each head by itself 58 us).  Selected pages differ from head to head.
   p.team = 1;
