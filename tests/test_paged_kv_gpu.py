@@ -478,6 +478,17 @@ def test_selection_where_fp32_scores_cannot_decide(typ, bounds, crowd, width):
     _status_clear()
 
 
+def test_selection_of_scores_below_the_smallest_fp32_number():
+    """Queries of 2^-70 and keys of 2^-70: fp32 products vanish, 64-bit ones do not."""
+    from wush_b200 import paged_kv
+    s = Setup([16 * 300], page=16, kv=1, dim=64, seed=2, bounds=True)
+    s.cache.bounds.copy_((_randn(s.g, 303, 1, 2, 64).sort(dim=2).values * 2.0 ** -70).to(BF))
+    q = (_randn(s.g, 1, 3, 64) * 2.0 ** -70).to(BF)
+    pages, _ = paged_kv.paged_select_pages(q, s.cache, s.table, s.seq_lens, 40, sink=1, recent=1)
+    assert pages[0, 0].tolist() == _expected_pages(s, q, 40, 1, 1)[0][0]
+    _status_clear()
+
+
 def test_selection_close_scores_do_not_depend_on_the_order_of_the_sum():
     """Pages whose scores differ only in the 40th bit: terms of 2^20 and -2^20 around one of 2^-20."""
     from wush_b200 import paged_kv

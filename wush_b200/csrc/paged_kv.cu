@@ -767,8 +767,9 @@ __global__ void __launch_bounds__(1024) select_kernel(const wush_kv_select_args 
   __syncthreads();
   kth = __reduce_min_sync(0xffffffffu, lane < warps ? (uint32_t)sm.low[lane] : ~0u);
   magnitude = __uint_as_float(__reduce_max_sync(0xffffffffu, lane < warps ? (uint32_t)sm.high[lane] : 0u));
-  // (17 + products / 2) * 2^-23 of the magnitude, and a sixteenth more for the magnitude's own rounding
-  const float eps = magnitude * (float)(17 + (a.kv.dim + 15) / 16) * (1.0625f / 8388608.0f);
+  // (17 + products / 2) * 2^-23 of the magnitude, a sixteenth more for the magnitude's own rounding, and what numbers below the
+  // smallest normal one may lose
+  const float eps = magnitude * (float)(17 + (a.kv.dim + 15) / 16) * (1.0625f / 8388608.0f) + 1024.0f * FLT_MIN;
   const float center = key_float(kth), bottom = __fsub_rd(center, 2.0f * eps), roof = __fadd_ru(center, 2.0f * eps);
   // a magnitude that is not finite leaves everything between (also where the k-th is a page outside the pool: all that are
   // in it are above)
