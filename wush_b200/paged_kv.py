@@ -220,21 +220,21 @@ def _q_heads(cache: PagedKVCache, q: torch.Tensor) -> int:
     return q.shape[1]
 
 
-def _on_its_device(op):
-    """Run an operator with the cache's device as the current one (switching costs more than a small call, so only when
-    it is another)."""
-    @functools.wraps(op)
-    def run(*args, **kwargs):
-        cache = kwargs.get("cache")
-        if cache is None:
-            cache = next((a for a in args if isinstance(a, PagedKVCache)), None)
-            if cache is None:
+def _on_its_device(at: int):
+    """Run an operator (its cache is positional argument `at`) with the cache's device as the current one.  Switching costs
+    more than a small call, so only when it is another."""
+    def decorate(op):
+        @functools.wraps(op)
+        def run(*args, **kwargs):
+            cache = args[at] if len(args) > at else kwargs.get("cache")
+            if not isinstance(cache, PagedKVCache):
                 raise TypeError(f"{op.__name__} needs a PagedKVCache")
-        if torch.cuda.current_device() == cache._index:
-            return op(*args, **kwargs)
-        with torch.cuda.device(cache._index):
-            return op(*args, **kwargs)
-    return run
+            if torch.cuda.current_device() == cache._index:
+                return op(*args, **kwargs)
+            with torch.cuda.device(cache._index):
+                return op(*args, **kwargs)
+        return run
+    return decorate
 
 
 def _stream(cache: PagedKVCache) -> int:
@@ -243,12 +243,13 @@ def _stream(cache: PagedKVCache) -> int:
 
 
 def _finish(cache: PagedKVCache, rc: int, what: str) -> None:
-    _lib.check(rc, what)
+    if rc:
+        _lib.check(rc, what)
     if _lib.CHECK_EVERY_OP:
         _lib.check_status(cache.device, what)
 
 
-@_on_its_device
+@_on_its_device(0)
 def paged_kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, seq_ids: torch.Tensor,
                     positions: torch.Tensor, q: Optional[torch.Tensor] = None, rope: Optional[torch.Tensor] = None,
                     interleaved: bool = False, q_out: Optional[torch.Tensor] = None,
@@ -279,7 +280,7 @@ def paged_kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, block
         n_heads = _q_heads(cache, q)
         hq = _heads(cache, q, rows, n_heads, typ, "q")
         if q_out is None:
-            q_out = torch.zeros(q.shape, dtype=typ, device=cache.device)
+            q_out = torch.zeros_like(q, memory_format=torch.contiguous_format)
         hqo = _heads(cache, q_out, rows, n_heads, typ, "q_out")
     elif q_out is not None:
         raise ValueError("q_out goes with q")
@@ -303,7 +304,7 @@ def paged_kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, block
     return q_out
 
 
-@_on_its_device
+@_on_its_device(0)
 def paged_kv_bounds(cache: PagedKVCache, block_table: torch.Tensor, seq_lens: torch.Tensor, new_tokens: int = 1) -> None:
     """Recompute ``cache.bounds`` for the pages that hold the last ``new_tokens`` of the ``seq_lens`` tokens of every
     sequence: the smallest and the largest stored key of every channel over the page's filled rows (NaN if one is).
@@ -318,7 +319,7 @@ def paged_kv_bounds(cache: PagedKVCache, block_table: torch.Tensor, seq_lens: to
     _finish(cache, rc, "wush_kv_bounds")
 
 
-@_on_its_device
+@_on_its_device(1)
 def paged_select_pages(q: torch.Tensor, cache: PagedKVCache, block_table: torch.Tensor, seq_lens: torch.Tensor, top: int,
                        sink: int = 1, recent: int = 1) -> Tuple[torch.Tensor, torch.Tensor]:
     """The pages worth attending to: (pages int32 [sequences, n_kv_heads, top], counts int32 [sequences, n_kv_heads]).
@@ -339,8 +340,8 @@ def paged_select_pages(q: torch.Tensor, cache: PagedKVCache, block_table: torch.
     n_heads = _q_heads(cache, q)
     hq = _heads(cache, q, seqs, n_heads, typ, "q")
     lens = _int32(seq_lens, (seqs,), "seq_lens", cache._index)
-    pages = torch.empty((seqs, cache.n_kv_heads, top), dtype=torch.int32, device=cache.device)
-    counts = torch.empty((seqs, cache.n_kv_heads), dtype=torch.int32, device=cache.device)
+    pages = seq_lens.new_empty((seqs, cache.n_kv_heads, top))
+    counts = seq_lens.new_empty((seqs, cache.n_kv_heads))
     if seqs == 0:
         return pages, counts
     lib, stream = _lib.load(), _stream(cache)
@@ -352,7 +353,7 @@ def paged_select_pages(q: torch.Tensor, cache: PagedKVCache, block_table: torch.
     return pages, counts
 
 
-@_on_its_device
+@_on_its_device(1)
 def paged_decode_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.Tensor, seq_lens: torch.Tensor,
                            scale: Optional[float] = None, window: int = 0, pages: Optional[torch.Tensor] = None,
                            counts: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
@@ -389,7 +390,7 @@ def paged_decode_attention(q: torch.Tensor, cache: PagedKVCache, block_table: to
         pages_ptr = _int32(pages, (seqs, cache.n_kv_heads, top), "pages", cache._index)
         counts_ptr = _int32(counts, (seqs, cache.n_kv_heads), "counts", cache._index)
     if out is None:
-        out = torch.empty((seqs, n_heads, cache.head_dim), dtype=typ, device=cache.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     ho = _heads(cache, out, seqs, n_heads, typ, "out")
     lse = torch.empty((seqs, n_heads), dtype=torch.float32, device=cache.device) if return_lse else None
     if seqs > 0:
