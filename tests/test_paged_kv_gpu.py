@@ -663,6 +663,45 @@ def test_operators_captured_behind_copies_and_fills():
     _status_clear()
 
 
+def test_operators_captured_on_forked_streams():
+    """The first kernel of a forked stream waits for another stream's work, and for two streams' after a join."""
+    from wush_b200 import paged_kv
+    s = Setup([900, 40], page=16, kv=2, dim=64, bounds=True, seed=43)
+    paged_kv.paged_kv_bounds(s.cache, s.table, s.seq_lens, 900)
+    x = _randn(s.g, 2, 8, 64).to(BF)
+    src = [x.clone(), _randn(s.g, 2, 8, 64).to(BF)]
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+
+    def step():
+        main = torch.cuda.current_stream()
+        q = x * 2
+        outs = []
+        for st in sides:
+            st.wait_stream(main)
+            with torch.cuda.stream(st):
+                outs.append(paged_kv.paged_decode_attention(q, s.cache, s.table, s.seq_lens))
+                outs += paged_kv.paged_select_pages(q, s.cache, s.table, s.seq_lens, 9)
+        for st in sides:
+            main.wait_stream(st)
+        outs.append(paged_kv.paged_decode_attention(outs[0], s.cache, s.table, s.seq_lens, pages=outs[4], counts=outs[5]))
+        return outs
+    want = []
+    for v in src:
+        x.copy_(v)
+        want.append([t.clone() for t in step()])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(3):
+        for v, w in zip(src, want):
+            x.copy_(v)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, w))
+    _status_clear()
+
+
 def test_refusals():
     from wush_b200 import paged_kv
     s = Setup([40, 20], page=16, kv=2, dim=64, bounds=True)
