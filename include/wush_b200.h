@@ -585,7 +585,9 @@ WUSH_API int wush_kv_bounds(const wush_kv_bounds_args* args);
  *   q        [seqs, q_heads, dim] of `type`; q_heads % kv.heads == 0
  *   pages    int32 [seqs, kv.heads, top] out: logical pages in ascending order, then -1
  *   counts   int32 [seqs, kv.heads] out: how many
- *   workspace  wush_kv_select_workspace_bytes(seqs, heads, width) bytes, 16-byte aligned
+ *   workspace  wush_kv_select_workspace_bytes(seqs, heads, width) bytes, 16-byte aligned; contents irrelevant.  The call
+ *              launches several kernels that pass data through it: calls that share one are made on one stream, and from
+ *              several threads only under a lock
  */
 typedef struct wush_kv_select_args {
   wush_kv_pages kv;
@@ -612,7 +614,8 @@ WUSH_API int wush_kv_select_pages(const wush_kv_select_args* args);
  *   pages, counts  null (all pages), or what wush_kv_select_pages writes: for every sequence and key head the first
  *              counts[b, h] entries of pages[b, h, top] are attended to, each cut at len (window must be 0)
  * A length beyond the table, or an entry outside it, sets *status = 2; tokens on such pages are left out.
- *   workspace  wush_kv_attention_workspace_bytes(kv, q_heads) bytes, 16-byte aligned
+ *   workspace  wush_kv_attention_workspace_bytes(kv, q_heads) bytes, 16-byte aligned; shared as that of
+ *              wush_kv_select_pages
  */
 typedef struct wush_kv_attention_args {
   wush_kv_pages kv;

@@ -702,6 +702,42 @@ def test_operators_captured_on_forked_streams():
     _status_clear()
 
 
+def test_threads_on_one_stream():
+    """Two threads call on the default stream, and so with one workspace: the kernels of a call stay together."""
+    import threading
+    from wush_b200 import paged_kv
+    calls, want = [], []
+    for seed, lens, heads in ((51, [3000, 5, 700], 8), (52, [90, 2048, 0, 4000, 333], 16)):
+        s = Setup(lens, page=16, kv=2, dim=128, bounds=True, seed=seed)
+        paged_kv.paged_kv_bounds(s.cache, s.table, s.seq_lens, max(lens))
+        q = _randn(s.g, len(lens), heads, 128).to(BF)
+
+        def call(s=s, q=q):
+            pages, counts = paged_kv.paged_select_pages(q, s.cache, s.table, s.seq_lens, 60)
+            return (pages, counts, paged_kv.paged_decode_attention(q, s.cache, s.table, s.seq_lens, pages=pages, counts=counts),
+                    paged_kv.paged_decode_attention(q, s.cache, s.table, s.seq_lens))
+        calls.append(call)
+        want.append(call())
+    got = [[], []]
+    start = threading.Barrier(2)
+
+    def work(i):
+        start.wait(30)
+        for _ in range(200):
+            got[i].append(calls[i]())
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert len(got[i]) == 200
+        for result in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(result, want[i]))
+    _status_clear()
+
+
 def test_refusals():
     from wush_b200 import paged_kv
     s = Setup([40, 20], page=16, kv=2, dim=64, bounds=True)

@@ -8,6 +8,7 @@ from __future__ import annotations
 import ctypes
 import os
 import re
+import threading
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("WUSH_B200_LIB") or os.path.join(HERE, "libwush_b200.so")
@@ -121,6 +122,9 @@ def check(rc: int, what: str) -> None:
 # --------------------------------------------------------------------------------------------
 _status_words: dict = {}
 _workspaces: dict = {}
+# Threads share the current stream, and so its workspace.  An op of several kernels takes the workspace and launches all of them
+# under this lock, so that another thread's kernels do not come between them.
+workspace_lock = threading.RLock()
 
 
 def status_word(device):

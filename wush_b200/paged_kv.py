@@ -345,10 +345,11 @@ def paged_select_pages(q: torch.Tensor, cache: PagedKVCache, block_table: torch.
     if seqs == 0:
         return pages, counts
     lib, stream = _lib.load(), _stream(cache)
-    work = _lib.stream_workspace(cache._index, stream, lib.wush_kv_select_workspace_bytes(seqs, cache.n_kv_heads, width))
-    rc = lib.wush_kv_select_pages(cache._packed + _SELECT.pack(
-        *table, *hq, lens, pages.data_ptr(), counts.data_ptr(), work.data_ptr(), work.numel(), cache._status, stream, TYPES[typ],
-        n_heads, top, sink, recent))
+    with _lib.workspace_lock:
+        work = _lib.stream_workspace(cache._index, stream, lib.wush_kv_select_workspace_bytes(seqs, cache.n_kv_heads, width))
+        rc = lib.wush_kv_select_pages(cache._packed + _SELECT.pack(
+            *table, *hq, lens, pages.data_ptr(), counts.data_ptr(), work.data_ptr(), work.numel(), cache._status, stream,
+            TYPES[typ], n_heads, top, sink, recent))
     _finish(cache, rc, "wush_kv_select_pages")
     return pages, counts
 
@@ -398,9 +399,10 @@ def paged_decode_attention(q: torch.Tensor, cache: PagedKVCache, block_table: to
         nbytes = cache._attention_scratch.get(n_heads)
         if nbytes is None:
             nbytes = cache._attention_scratch[n_heads] = lib.wush_kv_attention_workspace_bytes(cache._packed, n_heads)
-        work = _lib.stream_workspace(cache._index, stream, nbytes)
-        rc = lib.wush_kv_attention(cache._packed + _ATTENTION.pack(
-            *table, *hq, *ho, lse.data_ptr() if return_lse else 0, lens, pages_ptr, counts_ptr, work.data_ptr(), work.numel(),
-            cache._status, stream, window, TYPES[typ], n_heads, top, cache.head_dim ** -0.5 if scale is None else scale))
+        with _lib.workspace_lock:
+            work = _lib.stream_workspace(cache._index, stream, nbytes)
+            rc = lib.wush_kv_attention(cache._packed + _ATTENTION.pack(
+                *table, *hq, *ho, lse.data_ptr() if return_lse else 0, lens, pages_ptr, counts_ptr, work.data_ptr(), work.numel(),
+                cache._status, stream, window, TYPES[typ], n_heads, top, cache.head_dim ** -0.5 if scale is None else scale))
         _finish(cache, rc, "wush_kv_attention")
     return (out, lse) if return_lse else out

@@ -338,7 +338,7 @@ def matmul_fp4_blocked(x: torch.Tensor, w: torch.Tensor, xs_blocked: torch.Tenso
         raise ValueError(f"bias must be bfloat16 of shape ({n},)")
     lib = _lib.load()
     al = alpha.to(device=x.device, dtype=torch.float32).reshape(-1)[:1].contiguous()
-    with torch.cuda.device(x.device):
+    with torch.cuda.device(x.device), _lib.workspace_lock:
         ws_bytes = int(lib.wush_gemm_workspace_bytes(m, n, k, splits))
         work = _lib.gemm_workspace(x.device, ws_bytes) if ws_bytes else None
         rc = lib.wush_gemm_fp4_bf16_tn_fused(
