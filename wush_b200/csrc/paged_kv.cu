@@ -538,13 +538,17 @@ __device__ __forceinline__ int scan256(int* x, int count) {
 }
 
 constexpr int BORDER = 256;                                  // pages between that are ranked in shared memory
+constexpr int FEW = 32;                                      // keys that a warp ranks
 
 struct SelectShared {
   int hist[256];
   unsigned long long low[32], high[32];
   int digit, need, count;
   int sums[2][32];
-  int border[BORDER];
+  float most[32];
+  int few_count;
+  uint32_t few[FEW], kth;
+  int border[BORDER], border_page[BORDER];
   unsigned long long border_key[BORDER];
 };
 
@@ -557,11 +561,29 @@ struct Chosen {
   __device__ bool above(K k) const { return shift < (int)sizeof(K) * 8 && k >> shift > prefix; }
 };
 
+template <typename K>
+__device__ __forceinline__ K warp_min(K x) {
+  if constexpr (sizeof(K) == 4) {
+    return __reduce_min_sync(0xffffffffu, x);
+  } else {
+    for (int o = 16; o > 0; o >>= 1) {
+      const K y = __shfl_xor_sync(0xffffffffu, x, o);
+      x = y < x ? y : x;
+    }
+    return x;
+  }
+}
+template <typename K>
+__device__ __forceinline__ K warp_max(K x) {
+  return ~warp_min<K>(~x);
+}
+
 // The `need` largest of `among` keys, from the first bit in which they differ: 8 bits at a time the keys that share the
-// threshold's leading bits are counted by their next digit, until all of them are wanted or all bits are known.
+// threshold's leading bits are counted by their next digit, until all of them are wanted, no more than `few` are left or all
+// bits are known.
 // key(j) is the thread's j-th key, valid(j) whether it has one; ROWS rounds, or `rounds` where that is 0.
 template <typename K, int ROWS, class Key, class Valid>
-__device__ Chosen<K> radix_select(SelectShared& sm, int rounds, int need, int among, Key key, Valid valid) {
+__device__ Chosen<K> radix_select(SelectShared& sm, int rounds, int need, int among, int few, Key key, Valid valid) {
   constexpr int BITS = (int)sizeof(K) * 8;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5;
   const int end = ROWS > 0 ? ROWS : rounds;
@@ -573,28 +595,22 @@ __device__ Chosen<K> radix_select(SelectShared& sm, int rounds, int need, int am
       low = k < low ? k : low;
       high = k > high ? k : high;
     }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const K x = __shfl_xor_sync(0xffffffffu, low, o), y = __shfl_xor_sync(0xffffffffu, high, o);
-    low = x < low ? x : low;
-    high = y > high ? y : high;
-  }
+  low = warp_min<K>(low);
+  high = warp_max<K>(high);
   __syncthreads();
   if (lane == 0) {
     sm.low[warp] = low;
     sm.high[warp] = high;
   }
   __syncthreads();
-  for (int w = 0; w < warps; ++w) {
-    low = (K)sm.low[w] < low ? (K)sm.low[w] : low;
-    high = (K)sm.high[w] > high ? (K)sm.high[w] : high;
-  }
+  low = warp_min<K>(lane < warps ? (K)sm.low[lane] : ~(K)0);
+  high = warp_max<K>(lane < warps ? (K)sm.high[lane] : (K)0);
   Chosen<K> c;
   c.need = need;
   c.among = among;
   c.shift = low >= high ? 0 : 64 - __clzll((unsigned long long)low ^ (unsigned long long)high);   // bits that are not known
   c.prefix = c.shift == BITS ? 0 : high >> c.shift;
-  while (c.need > 0 && c.need < c.among && c.shift > 0) {
+  while (c.need > 0 && c.need < c.among && c.among > few && c.shift > 0) {
     const int bits = min(8, c.shift), next = c.shift - bits;
     for (int i = tid; i < 256; i += threads) sm.hist[i] = 0;
     __syncthreads();
@@ -628,9 +644,8 @@ __device__ Chosen<K> radix_select(SelectShared& sm, int rounds, int need, int am
     __syncthreads();
     c.prefix = (c.shift == BITS ? 0 : c.prefix << bits) | (K)sm.digit;
     c.need = sm.need;
-    c.among = sm.count;
+    c.among = sm.count;                                      // (written again two barriers from here)
     c.shift = next;
-    __syncthreads();
   }
   return c;
 }
@@ -747,26 +762,40 @@ __global__ void __launch_bounds__(1024) select_kernel(const wush_kv_select_args 
     for (int i = tid; i < top; i += threads) out[i] = i < begin ? i : n - top + i;
     return;
   }
-  const Chosen<uint32_t> c = radix_select<uint32_t, ROWS>(sm, rounds, want, end - begin, key_of, competes);
+  if (tid == 0) sm.few_count = 0;
+  const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(magnitude));       // (not negative: ordered as they are)
+  if (lane == 0) sm.most[warp] = __uint_as_float(most);
+  const Chosen<uint32_t> c = radix_select<uint32_t, ROWS>(sm, rounds, want, end - begin, FEW, key_of, competes);   // (with barriers)
+  magnitude = __uint_as_float(__reduce_max_sync(0xffffffffu, lane < warps ? __float_as_uint(sm.most[lane]) : 0u));
 
-  // the k-th largest, the largest magnitude, and from them the pages above and between
+  // the k-th largest: ranked among the few that are left (a radix selection to the last bit: 8 us instead of TODO), or the
+  // smallest of all that match
   uint32_t kth = ~0u;
 #pragma unroll
   for (int j = 0; j < (ROWS > 0 ? ROWS : rounds); ++j)
     if (competes(j)) {
       const uint32_t k = key_of(j);
-      if (c.matches(k) || c.above(k)) kth = min(kth, k);
+      if (!c.matches(k)) continue;
+      if (c.among <= FEW) sm.few[atomicAdd(&sm.few_count, 1)] = k;
+      else kth = min(kth, k);
     }
-  kth = __reduce_min_sync(0xffffffffu, kth);
-  const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(magnitude));       // (not negative: ordered as they are)
-  __syncthreads();
-  if (lane == 0) {
-    sm.low[warp] = kth;
-    sm.high[warp] = most;
+  if (c.among <= FEW) {
+    __syncthreads();
+    const uint32_t k = lane < c.among ? sm.few[lane] : 0u;
+#pragma unroll 1
+    for (int i = warp; i < c.among; i += warps) {
+      const uint32_t x = sm.few[i];
+      const int above = __popc(__ballot_sync(0xffffffffu, lane < c.among && k > x)), upto = __popc(__ballot_sync(0xffffffffu, lane < c.among && k >= x));
+      if (lane == 0 && above < c.need && c.need <= upto) sm.kth = x;       // (equal keys: the same from every warp)
+    }
+    __syncthreads();
+    kth = sm.kth;
+  } else {
+    kth = __reduce_min_sync(0xffffffffu, kth);
+    if (lane == 0) sm.low[warp] = kth;
+    __syncthreads();
+    kth = __reduce_min_sync(0xffffffffu, lane < warps ? (uint32_t)sm.low[lane] : ~0u);
   }
-  __syncthreads();
-  kth = __reduce_min_sync(0xffffffffu, lane < warps ? (uint32_t)sm.low[lane] : ~0u);
-  magnitude = __uint_as_float(__reduce_max_sync(0xffffffffu, lane < warps ? (uint32_t)sm.high[lane] : 0u));
   // (17 + products / 2) * 2^-23 of the magnitude, a sixteenth more for the magnitude's own rounding, and what numbers below the
   // smallest normal one may lose
   const float eps = magnitude * (float)(17 + (a.kv.dim + 15) / 16) * (1.0625f / 8388608.0f) + 1024.0f * FLT_MIN;
@@ -789,8 +818,7 @@ __global__ void __launch_bounds__(1024) select_kernel(const wush_kv_select_args 
   const int64_t seq = item / a.kv.heads;
   const int head = (int)(item - seq * a.kv.heads);
   const T* queries = reinterpret_cast<const T*>(a.q.data) + seq * a.q.row + (int64_t)head * group * a.q.head;
-  auto exact = [&](int lp, int g) {                          // 0 for a page outside the pool
-    const int page = lookup_page(a.table, seq, lp, a.kv.num_pages, a.status);
+  auto exact = [&](int page, int g) {                        // 0 for a page outside the pool
     const B* lower = reinterpret_cast<const B*>(a.kv.bounds) + ((int64_t)max(page, 0) * a.kv.heads + head) * 2 * a.kv.dim;
     const unsigned long long k = exact_key<T, B>(queries + g * a.q.head, lower, a.kv.dim);
     return page < 0 ? 0ull : k;
@@ -798,18 +826,28 @@ __global__ void __launch_bounds__(1024) select_kernel(const wush_kv_select_args 
   const bool all_between = need == between;                  // the usual case: the k-th itself and nothing else
   if (!all_between && between <= BORDER) {
     // score the pages between again, rank them, and leave the verdict in place of their scores
+    const int per = min(group, max(1, warps / between));
     __syncthreads();
     if (tid == 0) sm.count = 0;
     for (int i = tid; i < between; i += threads) sm.border_key[i] = 0;
     __syncthreads();
 #pragma unroll 1
     for (int i = begin + tid; i < end; i += threads)
-      if (is_between(mine[i].value)) sm.border[atomicAdd(&sm.count, 1)] = i;
+      if (is_between(mine[i].value)) {
+        const int at = atomicAdd(&sm.count, 1);
+        sm.border[at] = i;
+        sm.border_page[at] = lookup_page(a.table, seq, i, a.kv.num_pages, a.status);
+      }
     __syncthreads();
 #pragma unroll 1
-    for (int i = warp; i < between * group; i += warps) {    // (page, query)
-      const unsigned long long k = exact(sm.border[i / group], i % group);
-      if (lane == 0) atomicMax(&sm.border_key[i / group], k);
+    for (int i = warp; i < between * per; i += warps) {      // `per` warps share the queries of a page
+      unsigned long long k = 0;
+#pragma unroll 1
+      for (int g = i % per; g < group; g += per) {
+        const unsigned long long x = exact(sm.border_page[i / per], g);
+        k = k < x ? x : k;
+      }
+      if (lane == 0) atomicMax(&sm.border_key[i / per], k);
     }
     __syncthreads();
     for (int i = tid; i < between; i += threads) {
@@ -840,8 +878,9 @@ __global__ void __launch_bounds__(1024) select_kernel(const wush_kv_select_args 
     const float v = *(volatile float*)&mine[i].value;
     unsigned long long k = is_above(v) ? ~0ull : 0;
     if (is_between(v)) {
+      const int page = lookup_page(a.table, seq, i, a.kv.num_pages, a.status);
       for (int g = 0; g < group; ++g) {
-        const unsigned long long x = exact(i, g);
+        const unsigned long long x = exact(page, g);
         k = k < x ? x : k;
       }
     }
@@ -852,7 +891,7 @@ __global__ void __launch_bounds__(1024) select_kernel(const wush_kv_select_args 
   __syncthreads();
   const int all = (n + threads - 1) / threads;
   auto wide_key = [&](int j) { return *(volatile unsigned long long*)&keys[page_of(j)]; };
-  const Chosen<unsigned long long> w = radix_select<unsigned long long, 0>(sm, all, want, end - begin, wide_key, competes);
+  const Chosen<unsigned long long> w = radix_select<unsigned long long, 0>(sm, all, want, end - begin, 0, wide_key, competes);
   write_pages(sm, all, w.need, w.among, [&](int j0, int x) { return competes(j0 + x) ? w.above(wide_key(j0 + x)) : forced(j0 + x); },
               [&](int j0, int x) { return competes(j0 + x) && w.matches(wide_key(j0 + x)); }, out);
 }
