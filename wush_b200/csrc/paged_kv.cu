@@ -650,12 +650,11 @@ __device__ Chosen<K> radix_select(SelectShared& sm, int rounds, int need, int am
   return c;
 }
 
-// Sums of two numbers over the block, for every thread.
+// Sums of two numbers over the block, for every thread (once a kernel: no barrier before).
 __device__ __forceinline__ int2 block_sums(SelectShared& sm, int x, int y) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   x = __reduce_add_sync(0xffffffffu, x);
   y = __reduce_add_sync(0xffffffffu, y);
-  __syncthreads();
   if (lane == 0) {
     sm.sums[0][warp] = x;
     sm.sums[1][warp] = y;
@@ -723,7 +722,9 @@ __device__ void write_pages(SelectShared& sm, int rounds, int need, int among, T
 }
 
 // One block per (sequence, key head).  A thread holds every blockDim-th score, up to ROWS of them (ROWS is 8, or 0 for more
-// pages than that: then they are read again for every pass).
+// pages than that: then they are read again for every pass).  A chain of latencies: of barriers, and of instructions that come
+// for the first time, so few of them count (scores and selection of 64 of 2047 pages in a captured graph: 12.7 us with all bits
+// of the k-th found by counting, lengths before scores and three cases in every comparison; 10.6 us as it is).
 template <typename T, typename B, int ROWS>
 __global__ void __launch_bounds__(1024) select_kernel(const wush_kv_select_args a, int group, Score* scores) {
   __shared__ SelectShared sm;
@@ -731,6 +732,13 @@ __global__ void __launch_bounds__(1024) select_kernel(const wush_kv_select_args 
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5;
   const int64_t item = blockIdx.x;
+  Score* mine = scores + item * a.table.width;
+  auto page_of = [&](int j) { return j * threads + tid; };
+  auto load = [&](int j) { return *reinterpret_cast<const float2*>(mine + page_of(j)); };
+  float2 early[ROWS > 0 ? ROWS : 1];                         // (before the length is known: what lies behind it is not used)
+  if (ROWS > 0)
+#pragma unroll
+    for (int j = 0; j < ROWS; ++j) early[ROWS > 0 ? j : 0] = *reinterpret_cast<const float2*>(mine + min((int64_t)page_of(j), a.table.width - 1));
   const int len = (int)max((int64_t)0, min((int64_t)a.seq_lens[item / a.kv.heads], a.table.width * a.kv.page_size));
   const int n = (len + a.kv.page_size - 1) / a.kv.page_size, top = a.top;
   int32_t* out = a.pages + item * top;
@@ -742,18 +750,15 @@ __global__ void __launch_bounds__(1024) select_kernel(const wush_kv_select_args 
     return;
   }
   const int begin = a.sink, end = n - a.recent, want = top - a.sink - a.recent;   // pages that compete
-  Score* mine = scores + item * a.table.width;
   const int rounds = ROWS > 0 ? ROWS : (n + threads - 1) / threads;
-  auto page_of = [&](int j) { return j * threads + tid; };
   auto competes = [&](int j) { return page_of(j) >= begin && page_of(j) < end; };
   auto forced = [&](int j) { return page_of(j) < n && !competes(j); };
-  auto load = [&](int j) { return *reinterpret_cast<const float2*>(mine + page_of(j)); };
   uint32_t held[ROWS > 0 ? ROWS : 1];
   float magnitude = 0.0f;
 #pragma unroll
   for (int j = 0; j < (ROWS > 0 ? ROWS : rounds); ++j)
     if (competes(j)) {
-      const float2 s = load(j);
+      const float2 s = ROWS > 0 ? early[ROWS > 0 ? j : 0] : load(j);
       if (ROWS > 0) held[ROWS > 0 ? j : 0] = float_key(s.x);
       magnitude = fmaxf(magnitude, s.y);
     }
@@ -768,8 +773,7 @@ __global__ void __launch_bounds__(1024) select_kernel(const wush_kv_select_args 
   const Chosen<uint32_t> c = radix_select<uint32_t, ROWS>(sm, rounds, want, end - begin, FEW, key_of, competes);   // (with barriers)
   magnitude = __uint_as_float(__reduce_max_sync(0xffffffffu, lane < warps ? __float_as_uint(sm.most[lane]) : 0u));
 
-  // the k-th largest: ranked among the few that are left (a radix selection to the last bit: 8 us instead of TODO), or the
-  // smallest of all that match
+  // the k-th largest: ranked among the few that are left, or the smallest of all that match
   uint32_t kth = ~0u;
 #pragma unroll
   for (int j = 0; j < (ROWS > 0 ? ROWS : rounds); ++j)
@@ -799,22 +803,26 @@ __global__ void __launch_bounds__(1024) select_kernel(const wush_kv_select_args 
   // (17 + products / 2) * 2^-23 of the magnitude, a sixteenth more for the magnitude's own rounding, and what numbers below the
   // smallest normal one may lose
   const float eps = magnitude * (float)(17 + (a.kv.dim + 15) / 16) * (1.0625f / 8388608.0f) + 1024.0f * FLT_MIN;
-  const float center = key_float(kth), bottom = __fsub_rd(center, 2.0f * eps), roof = __fadd_ru(center, 2.0f * eps);
-  // a magnitude that is not finite leaves everything between (also where the k-th is a page outside the pool: all that are
-  // in it are above)
-  const bool sure = eps <= FLT_MAX && center >= -FLT_MAX;
-  auto is_above = [&](float v) { return sure ? v > roof : (eps <= FLT_MAX && v > center); };
-  auto is_between = [&](float v) { return sure ? v >= bottom && v <= roof : (eps <= FLT_MAX ? v == center : true); };
-  int n_above = 0, n_between = 0;
+  // a magnitude that is not finite leaves everything between; where the k-th is a page outside the pool, all that are in it
+  // are above
+  const float center = key_float(kth);
+  float bottom = -INFINITY, roof = INFINITY;
+  if (eps <= FLT_MAX) {
+    bottom = center >= -FLT_MAX ? __fsub_rd(center, 2.0f * eps) : center;
+    roof = center >= -FLT_MAX ? __fadd_ru(center, 2.0f * eps) : center;
+  }
+  auto is_above = [&](float v) { return v > roof; };
+  auto is_between = [&](float v) { return v >= bottom && v <= roof; };
+  int n_above = 0, n_upto = 0;                               // (and of those above or between)
 #pragma unroll
   for (int j = 0; j < (ROWS > 0 ? ROWS : rounds); ++j)
     if (competes(j)) {
       const float v = key_float(key_of(j));
-      n_above += is_above(v);
-      n_between += is_between(v);
+      n_above += v > roof;
+      n_upto += v >= bottom;
     }
-  const int2 sums = block_sums(sm, n_above, n_between);
-  const int need = want - sums.x, between = sums.y;
+  const int2 sums = block_sums(sm, n_above, n_upto);
+  const int need = want - sums.x, between = sums.y - sums.x;
   const int64_t seq = item / a.kv.heads;
   const int head = (int)(item - seq * a.kv.heads);
   const T* queries = reinterpret_cast<const T*>(a.q.data) + seq * a.q.row + (int64_t)head * group * a.q.head;
@@ -865,7 +873,7 @@ __global__ void __launch_bounds__(1024) select_kernel(const wush_kv_select_args 
       const int j = j0 + x;
       if (!competes(j)) return forced(j);
       const float v = key_float(key_of(ROWS > 0 ? x : j));   // (read again, without registers: the verdict already)
-      if (is_above(v) || (all_between && is_between(v))) return true;
+      if (v > roof || (all_between && v >= bottom)) return true;
       if (ROWS == 0) return v == INFINITY;
       return is_between(v) && *(volatile float*)&mine[page_of(j)].value == INFINITY;
     }, [](int, int) { return false; }, out);
