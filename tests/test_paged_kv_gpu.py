@@ -362,6 +362,35 @@ def test_attention_offsets_beyond_32_bits():
     s.check_attention(q, out, lse)
 
 
+def test_a_page_of_nearly_2_31_rows():
+    """One page that is a whole table: its rows and a length's, added up, pass 2^31 (34 GB; keys and values share it)."""
+    from wush_b200.paged_kv import PagedKVCache, paged_decode_attention, paged_kv_bounds, paged_select_pages
+    dev, rows, n, d = _dev(), 2 ** 31 - 2 ** 16 - 16, 70000, 16
+    if torch.cuda.mem_get_info()[0] < 40 * 2 ** 30:
+        pytest.skip("needs 34 GB")
+    s = Setup([1], page=16, kv=1, dim=d, cache=F8, seed=9)
+    pool = torch.empty(1, rows, 1, d, dtype=torch.uint8, device=dev).view(F8)
+    pool[0, :n] = _randn(s.g, n, 1, d).mul(8).clamp(-448, 448).to(F8)
+    one = torch.full((1,), 0.125, device=dev)
+    s.cache = PagedKVCache(pool, pool, k_scale=one, v_scale=one, bounds=torch.empty(1, 1, 2, d, dtype=BF, device=dev))
+    s.lens = [n]
+    s.table = torch.zeros(1, 1, dtype=torch.int32, device=dev)
+    s.seq_lens = torch.tensor([n], dtype=torch.int32, device=dev)
+    paged_kv_bounds(s.cache, s.table, s.seq_lens)
+    stored = pool[0, :n, 0].float() * 0.125                    # (exact)
+    s.rows = lambda b, head, which: stored.double()
+    assert torch.equal(s.cache.bounds[0, 0].float() * 0.125, torch.stack([stored.amin(0), stored.amax(0)]))
+    q = _randn(s.g, 1, 2, d).to(BF)
+    pages, counts = paged_select_pages(q, s.cache, s.table, s.seq_lens, 2)
+    assert pages.tolist() == [[[0, -1]]] and counts.tolist() == [[1]]
+    out, lse = paged_decode_attention(q, s.cache, s.table, s.seq_lens, return_lse=True)
+    _status_clear()
+    s.check_attention(q, out, lse)
+    out, lse = paged_decode_attention(q, s.cache, s.table, s.seq_lens, window=1000, return_lse=True)
+    _status_clear()
+    s.check_attention(q, out, lse, window=1000)
+
+
 # ---- selection ---------------------------------------------------------------------------------------------------------
 
 def _expected_pages(s, q, top, sink, recent):

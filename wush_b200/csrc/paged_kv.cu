@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(128) bounds_kernel(const wush_kv_pages kv, con
     const int head = (int)(w - slot * kv.heads);
     const int len = clamp_length(seq_lens[seq], table.width * kv.page_size, status);
     const int64_t first = (len > new_tokens ? len - new_tokens : 0) / kv.page_size + (slot - seq * groups) * span;
-    const int64_t behind = min((int64_t)(len + kv.page_size - 1) / kv.page_size, first + span);   // one past the last page
+    const int64_t behind = min((int64_t)pages_of_length(len, kv.page_size), first + span);   // one past the last page
     if (first >= behind) continue;
     const int pages = (int)(behind - first);
     const int my_page = lane < pages ? lookup_page(table, seq, (int)first + lane, kv.num_pages, status) : -1;
@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(SCORE_WARPS * 32, J <= 4 ? SCORE_BLOCKS : 2) s
   const int d = a.kv.dim, heads = a.kv.heads;
   auto pages_of = [&](int64_t seq) {
     const int len = clamp_length(a.seq_lens[seq], a.table.width * a.kv.page_size, a.status);
-    return (len + a.kv.page_size - 1) / a.kv.page_size;
+    return pages_of_length(len, a.kv.page_size);
   };
   auto units_of = [&](int64_t seq) -> int64_t {              // of one key head
     if (seq >= a.table.seqs) return 0;
@@ -740,7 +740,7 @@ __global__ void __launch_bounds__(1024) select_kernel(const wush_kv_select_args 
 #pragma unroll
     for (int j = 0; j < ROWS; ++j) early[ROWS > 0 ? j : 0] = *reinterpret_cast<const float2*>(mine + min((int64_t)page_of(j), a.table.width - 1));
   const int len = (int)max((int64_t)0, min((int64_t)a.seq_lens[item / a.kv.heads], a.table.width * a.kv.page_size));
-  const int n = (len + a.kv.page_size - 1) / a.kv.page_size, top = a.top;
+  const int n = pages_of_length(len, a.kv.page_size), top = a.top;
   int32_t* out = a.pages + item * top;
   const int count = min(n, top);
   if (tid == 0) a.counts[item] = count;

@@ -163,6 +163,11 @@ __device__ __forceinline__ int clamp_length(int len, int64_t capacity, int* stat
   return len < 0 ? 0 : len;
 }
 
+// (the sum passes 2^31 where pages are that large, not 2^32)
+__device__ __forceinline__ int pages_of_length(int len, int page_size) {
+  return (int)(((uint32_t)len + (uint32_t)page_size - 1) / (uint32_t)page_size);
+}
+
 // physical page of logical page lp (0 <= lp < width), or -1 and a report when the entry is outside the pool
 __device__ __forceinline__ int lookup_page(const wush_kv_table& t, int64_t seq, int lp, int64_t num_pages, int* status) {
   const int page = t.block_table[seq * t.stride + lp];
