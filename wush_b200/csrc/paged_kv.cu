@@ -546,9 +546,10 @@ struct SelectShared {
   int digit, need, count;
   int sums[2][32];
   float most[32];
-  int few_count;
+  int few_count, border_count;
   uint32_t few[FEW], kth;
   int border[BORDER], border_page[BORDER];
+  uint32_t taken[256];
   unsigned long long border_key[BORDER];
 };
 
@@ -664,34 +665,34 @@ __device__ __forceinline__ int2 block_sums(SelectShared& sm, int x, int y) {
                    __reduce_add_sync(0xffffffffu, lane < warps ? sm.sums[1][lane] : 0));
 }
 
-// Writes the taken pages in ascending order: those with take(j), and the first `need` of the `among` with equal(j).  8 rounds
+// Writes the taken pages in ascending order: those with take(j), and the first `need` of the `among` with equal(j).  R rounds
 // at a time; hist holds the counts of (round, warp): 8 * 32 at most.
-template <class Take, class Equal>
+template <int R, class Take, class Equal>
 __device__ void write_pages(SelectShared& sm, int rounds, int need, int among, Take take_of, Equal equal_of, int32_t* out) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5;
   int taken_before = 0, equal_before = 0;
-  for (int j0 = 0; j0 < rounds; j0 += 8) {
+  for (int j0 = 0; j0 < rounds; j0 += R) {
     unsigned equal = 0, take = 0;                            // one bit a round
 #pragma unroll
-    for (int x = 0; x < 8; ++x) {
+    for (int x = 0; x < R; ++x) {
       equal |= (unsigned)equal_of(j0, x) << x;
       take |= (unsigned)take_of(j0, x) << x;
     }
     if (need < among) {                                      // not all that match: by rank
       __syncthreads();
 #pragma unroll
-      for (int x = 0; x < 8; ++x) {
+      for (int x = 0; x < R; ++x) {
         const unsigned m = __ballot_sync(0xffffffffu, equal >> x & 1);
         if (lane == 0) sm.hist[x * warps + warp] = __popc(m);
       }
       __syncthreads();
       if (warp == 0) {
-        const int total = scan256(sm.hist, 8 * warps);
+        const int total = scan256(sm.hist, R * warps);
         if (lane == 0) sm.count = total;
       }
       __syncthreads();
 #pragma unroll
-      for (int x = 0; x < 8; ++x) {
+      for (int x = 0; x < R; ++x) {
         const unsigned m = __ballot_sync(0xffffffffu, equal >> x & 1);
         if ((equal >> x & 1) && equal_before + sm.hist[x * warps + warp] + __popc(m & ((1u << lane) - 1)) < need) take |= 1u << x;
       }
@@ -701,18 +702,18 @@ __device__ void write_pages(SelectShared& sm, int rounds, int need, int among, T
     }
     __syncthreads();
 #pragma unroll
-    for (int x = 0; x < 8; ++x) {
+    for (int x = 0; x < R; ++x) {
       const unsigned m = __ballot_sync(0xffffffffu, take >> x & 1);
       if (lane == 0) sm.hist[x * warps + warp] = __popc(m);
     }
     __syncthreads();
     if (warp == 0) {
-      const int total = scan256(sm.hist, 8 * warps);
+      const int total = scan256(sm.hist, R * warps);
       if (lane == 0) sm.count = total;
     }
     __syncthreads();
 #pragma unroll
-    for (int x = 0; x < 8; ++x) {
+    for (int x = 0; x < R; ++x) {
       const unsigned m = __ballot_sync(0xffffffffu, take >> x & 1);
       if (take >> x & 1) out[taken_before + sm.hist[x * warps + warp] + __popc(m & ((1u << lane) - 1))] = (j0 + x) * threads + tid;
     }
@@ -721,10 +722,10 @@ __device__ void write_pages(SelectShared& sm, int rounds, int need, int among, T
   }
 }
 
-// One block per (sequence, key head).  A thread holds every blockDim-th score, up to ROWS of them (ROWS is 8, or 0 for more
-// pages than that: then they are read again for every pass).  A chain of latencies: of barriers, and of instructions that come
+// One block per (sequence, key head).  A thread holds every blockDim-th score, up to ROWS of them (ROWS is 4 or 8, or 0
+// for more pages than that: then they are read again for every pass).  A chain of latencies: of barriers, and of instructions that come
 // for the first time, so few of them count (scores and selection of 64 of 2047 pages in a captured graph: 12.7 us with all bits
-// of the k-th found by counting, lengths before scores and three cases in every comparison; 10.6 us as it is).
+// of the k-th found by counting, lengths before scores, three cases in every comparison and 8 scores a thread; 9.6 us as it is).
 template <typename T, typename B, int ROWS>
 __global__ void __launch_bounds__(1024) select_kernel(const wush_kv_select_args a, int group, Score* scores) {
   __shared__ SelectShared sm;
@@ -750,6 +751,7 @@ __global__ void __launch_bounds__(1024) select_kernel(const wush_kv_select_args 
     return;
   }
   const int begin = a.sink, end = n - a.recent, want = top - a.sink - a.recent;   // pages that compete
+  constexpr int R = ROWS > 0 ? ROWS : 8;
   const int rounds = ROWS > 0 ? ROWS : (n + threads - 1) / threads;
   auto competes = [&](int j) { return page_of(j) >= begin && page_of(j) < end; };
   auto forced = [&](int j) { return page_of(j) < n && !competes(j); };
@@ -767,7 +769,7 @@ __global__ void __launch_bounds__(1024) select_kernel(const wush_kv_select_args 
     for (int i = tid; i < top; i += threads) out[i] = i < begin ? i : n - top + i;
     return;
   }
-  if (tid == 0) sm.few_count = 0;
+  if (tid == 0) sm.few_count = sm.border_count = 0;
   const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(magnitude));       // (not negative: ordered as they are)
   if (lane == 0) sm.most[warp] = __uint_as_float(most);
   const Chosen<uint32_t> c = radix_select<uint32_t, ROWS>(sm, rounds, want, end - begin, FEW, key_of, competes);   // (with barriers)
@@ -833,19 +835,23 @@ __global__ void __launch_bounds__(1024) select_kernel(const wush_kv_select_args 
   };
   const bool all_between = need == between;                  // the usual case: the k-th itself and nothing else
   if (!all_between && between <= BORDER) {
-    // score the pages between again, rank them, and leave the verdict in place of their scores
+    // score the pages between again and rank them; the verdict is a bit of `taken`, or is left in place of the score
     const int per = min(group, max(1, warps / between));
-    __syncthreads();
-    if (tid == 0) sm.count = 0;
-    for (int i = tid; i < between; i += threads) sm.border_key[i] = 0;
-    __syncthreads();
+    if (ROWS > 0)
+      for (int i = tid; i < ROWS * warps; i += threads) sm.taken[i] = 0;
+    for (int j0 = 0; j0 < rounds; j0 += R) {
+      unsigned mine_between = 0;                             // one bit a round
+#pragma unroll
+      for (int x = 0; x < R; ++x)
+        if (competes(j0 + x)) mine_between |= (unsigned)is_between(key_float(key_of(ROWS > 0 ? x : j0 + x))) << x;
 #pragma unroll 1
-    for (int i = begin + tid; i < end; i += threads)
-      if (is_between(mine[i].value)) {
-        const int at = atomicAdd(&sm.count, 1);
-        sm.border[at] = i;
-        sm.border_page[at] = lookup_page(a.table, seq, i, a.kv.num_pages, a.status);
+      for (; mine_between != 0; mine_between &= mine_between - 1) {
+        const int at = atomicAdd(&sm.border_count, 1), lp = page_of(j0 + __ffs(mine_between) - 1);
+        sm.border[at] = lp;
+        sm.border_key[at] = 0;
+        sm.border_page[at] = lookup_page(a.table, seq, lp, a.kv.num_pages, a.status);
       }
+    }
     __syncthreads();
 #pragma unroll 1
     for (int i = warp; i < between * per; i += warps) {      // `per` warps share the queries of a page
@@ -863,19 +869,21 @@ __global__ void __launch_bounds__(1024) select_kernel(const wush_kv_select_args 
 #pragma unroll 1
       for (int o = 0; o < between; ++o)
         better += sm.border_key[o] > sm.border_key[i] || (sm.border_key[o] == sm.border_key[i] && sm.border[o] < sm.border[i]);
-      mine[sm.border[i]].value = better < need ? INFINITY : -INFINITY;
+      const int lp = sm.border[i];
+      if (ROWS == 0) mine[lp].value = better < need ? INFINITY : -INFINITY;
+      else if (better < need) atomicOr(&sm.taken[lp >> 5], 1u << (lp & 31));
     }
     __threadfence_block();
     __syncthreads();
   }
   if (all_between || between <= BORDER) {
-    write_pages(sm, rounds, 0, 0, [&](int j0, int x) {
+    write_pages<R>(sm, rounds, 0, 0, [&](int j0, int x) {
       const int j = j0 + x;
       if (!competes(j)) return forced(j);
       const float v = key_float(key_of(ROWS > 0 ? x : j));   // (read again, without registers: the verdict already)
       if (v > roof || (all_between && v >= bottom)) return true;
       if (ROWS == 0) return v == INFINITY;
-      return is_between(v) && *(volatile float*)&mine[page_of(j)].value == INFINITY;
+      return !all_between && v >= bottom && (sm.taken[page_of(j) >> 5] >> (tid & 31) & 1);
     }, [](int, int) { return false; }, out);
     return;
   }
@@ -900,7 +908,7 @@ __global__ void __launch_bounds__(1024) select_kernel(const wush_kv_select_args 
   const int all = (n + threads - 1) / threads;
   auto wide_key = [&](int j) { return *(volatile unsigned long long*)&keys[page_of(j)]; };
   const Chosen<unsigned long long> w = radix_select<unsigned long long, 0>(sm, all, want, end - begin, 0, wide_key, competes);
-  write_pages(sm, all, w.need, w.among, [&](int j0, int x) { return competes(j0 + x) ? w.above(wide_key(j0 + x)) : forced(j0 + x); },
+  write_pages<8>(sm, all, w.need, w.among, [&](int j0, int x) { return competes(j0 + x) ? w.above(wide_key(j0 + x)) : forced(j0 + x); },
               [&](int j0, int x) { return competes(j0 + x) && w.matches(wide_key(j0 + x)); }, out);
 }
 
@@ -1003,10 +1011,20 @@ extern "C" int wush_kv_select_pages(const wush_kv_select_args* args) {
     auto kern = a.kv.dim <= 64 ? score_kernel<T, B, 2> : (a.kv.dim <= 128 ? score_kernel<T, B, 4> : score_kernel<T, B, 8>);
     const cudaError_t e = cudaLaunchKernelEx(early.config(grid, SCORE_WARPS * 32, 0), kern, a, group, scores);
     if (e != cudaSuccess) return (int)e;
-    // 8 scores a thread in registers while that is enough
-    int threads = 128;
-    while (threads < 1024 && threads * 8 < a.table.width) threads *= 2;
-    return (int)cudaLaunchKernelEx(early.config(dim3((unsigned)(a.table.seqs * a.kv.heads)), threads, 0), threads * 8 >= a.table.width ? select_kernel<T, B, 8> : select_kernel<T, B, 0>, a, group, scores);
+    // Up to 4 scores a thread in registers, with up to 512 threads as few as 2 (the warps share what is scored again: 64 items
+    // of 1024 pages 17.9 us, with 256 threads 19.3), while all blocks are on the SMs together (1024 threads by registers);
+    // else 8 (8 a thread: 24.5 us; 512 items of 2048 pages: 4 a thread 105.5, 8 102.5).  Times of scores and selection.
+    const int64_t items = a.table.seqs * a.kv.heads;
+    auto threads_for = [&](int rows, int from, int most) {
+      while (from < most && (int64_t)from * rows < a.table.width) from *= 2;
+      return from;
+    };
+    int threads = threads_for(4, threads_for(2, 128, 512), 1024);
+    const bool four = (int64_t)threads * 4 >= a.table.width && items * threads <= (int64_t)sm_count() * 1024;
+    if (!four) threads = threads_for(8, 128, 1024);
+    const bool eight = (int64_t)threads * 8 >= a.table.width;
+    auto select = four ? select_kernel<T, B, 4> : (eight ? select_kernel<T, B, 8> : select_kernel<T, B, 0>);
+    return (int)cudaLaunchKernelEx(early.config(dim3((unsigned)items), threads, 0), select, a, group, scores);
   };
   const __nv_bfloat16 bf = {};
   const __half hf = {};
