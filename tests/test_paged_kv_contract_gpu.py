@@ -1,0 +1,34 @@
+"""What the paged key-value cache operators promise beyond their formulas: precision of the weights, copies of a cache,
+lengths that the caller writes, reports of what is left out, refusals."""
+
+import pytest
+import torch
+
+from tests import paged_reference as ref
+from tests.test_paged_kv_gpu import BF, F8, HF, Setup, _dev, _randn, _status_clear
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("typ,cache", [(BF, F8), (HF, F8), (BF, BF), (HF, HF)])
+@pytest.mark.parametrize("n", [2, 34])
+def test_weights_enter_the_product_with_more_than_16_bits(typ, cache, n):
+    """Values a, -a, a, ... under nearly equal weights: the result is a small difference, whose own rounding is small, and
+    shows what the weights lost.  A weight of one fp16 term is off by up to 2^-11 of itself; allowed are the 2^-16 of two
+    terms (n + 64 additions and the exponentials come on top, see paged_reference.attention_tolerance)."""
+    from wush_b200 import paged_kv
+    s = Setup([n] * 8, page=16, kv=2, dim=64, cache=cache, seed=n)
+    v = torch.ones(64, device=_dev())
+    for b in range(8):
+        for p in range(n):
+            s.cache.v[int(s.table[b, p // 16]), p % 16] = ((1 - 2 * (p % 2)) * v).to(cache)
+    q = (0.005 * _randn(s.g, 8, 16, 64)).to(typ)
+    out = paged_kv.paged_decode_attention(q, s.cache, s.table, s.seq_lens)
+    _status_clear()
+    for b in range(8):
+        for h in range(16):
+            k, values = s.rows(b, h // 8, "k"), s.rows(b, h // 8, "v")
+            want, _, mass = ref.attend(q[b, h].double(), k, values, 64 ** -0.5)
+            tol = ref.attention_tolerance(want, n, 64, mass, float(values.abs().max()), typ, False)
+            err = (out[b, h].double() - want).abs()
+            assert bool((err <= tol).all()), (b, h, float((err / tol).max()))

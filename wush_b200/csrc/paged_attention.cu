@@ -8,8 +8,9 @@
 // A product does not care in which order its contracted index runs, nor which row is which channel, so a lane's fragment
 // of K is a 16-byte piece of a key row and its fragment of V neighbouring channels of four tokens, each one load from shared
 // memory, and the queries are loaded in the matching order.  P is turned from the layout of an accumulator into that of an
-// operand by movmatrix.  8-bit pages are widened to fp16 (exact).  (tcgen05.mma has at least 64 rows and 8 columns, wants P in
-// memory, and would be idle all the same: the tensor pipe is busy a seventh of the time.)
+// operand by movmatrix, as two 16-bit terms: one alone is off by up to 2^-9 (bf16) or 2^-12 (fp16) of a weight, and where
+// values cancel no rounding of the result hides that.  8-bit pages are widened to fp16 (exact).  (tcgen05.mma has at least 64
+// rows and 8 columns, wants P in memory, and would be idle all the same: the tensor pipe is busy a seventh of the time.)
 //
 // Copies.  Every warp has a ring of three tiles in shared memory, filled two tiles ahead by bulk tensor copies (16 rows of one
 // head of a page are one box), so a warp needs one instruction for 2 KB and no registers for what is in flight.  Measured on
@@ -87,8 +88,6 @@ struct Shape {
   static constexpr int HEADS = NT * 8;
   static constexpr int UNIT = WARPS * TT;                   // tokens of a unit
   static constexpr int STAGES = 3;                          // tiles of a warp in shared memory or on the way there
-  // P as two 16-bit terms: one term costs 2^-9 (bf16) or 2^-12 (fp16) of a weight, which a bf16 result hides only with fp16
-  static constexpr bool TWO = !(E8 && sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value);
   using M = typename std::conditional<E8, __half, T>::type; // operand type of the products
   static constexpr float RISE = 8.0f;                       // exponent that a weight may reach
   // fp16 weights are scaled by 2^7: the largest then are 2^15, and small ones stay normal numbers down to 2^-21
@@ -603,10 +602,8 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS)
             l[nt][1] += p1;
             const uint32_t hi = pack2<M>(p0, p1);
             ph[mt][nt][half] = transpose8(hi);
-            if (S::TWO) {
-              const float2 back = to_float2<M>(hi);
-              pl[mt][nt][half] = transpose8(pack2<M>(p0 - back.x, p1 - back.y));
-            }
+            const float2 back = to_float2<M>(hi);
+            pl[mt][nt][half] = transpose8(pack2<M>(p0 - back.x, p1 - back.y));
           }
       }
 
@@ -650,7 +647,7 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               mma<M>(o[nt][j][i], a0, a1, a2, a3, ph[mt][nt][0], ph[mt][nt][1]);
-              if (S::TWO) mma<M>(o[nt][j][i], a0, a1, a2, a3, pl[mt][nt][0], pl[mt][nt][1]);
+              mma<M>(o[nt][j][i], a0, a1, a2, a3, pl[mt][nt][0], pl[mt][nt][1]);
             }
           }
         }
