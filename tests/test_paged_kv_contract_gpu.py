@@ -1,6 +1,5 @@
 """What the paged key-value cache operators promise beyond their formulas: precision of the weights, copies of a cache,
 lengths that the caller writes, reports of what is left out, refusals."""
-
 import pytest
 import torch
 
@@ -32,3 +31,29 @@ def test_weights_enter_the_product_with_more_than_16_bits(typ, cache, n):
             tol = ref.attention_tolerance(want, n, 64, mass, float(values.abs().max()), typ, False)
             err = (out[b, h].double() - want).abs()
             assert bool((err <= tol).all()), (b, h, float((err / tol).max()))
+
+
+@pytest.mark.parametrize("typ", [BF, HF])
+@pytest.mark.parametrize("big,small", [(1.0, 2.0 ** -18), (1.0, 2.0 ** -13), (0.0, 2.0 ** -14), (49152.0, 0.25), (2.0 ** -12, 2.0 ** -14)])
+def test_small_elements_of_a_query_over_8_bit_pages_keep_their_bits(typ, big, small):
+    """One element of every query is large where all keys are zero; the others, far below it, make the logits.  They are
+    held to the tolerance of 16-bit pages: every product is exact, and only the sum is rounded."""
+    from wush_b200 import paged_kv
+    s = Setup([40, 7], page=16, kv=1, dim=64, cache=F8, seed=7)
+    for b in range(2):
+        for p in range(s.lens[b]):
+            s.cache.k[int(s.table[b, p // 16]), p % 16, 0, 5] = 0.0
+    q = (small * (1 + 0.5 * _randn(s.g, 2, 4, 64))).to(typ)
+    q[:, :, 5] = big
+    used = q.double().clone()
+    scale = 64 ** -0.5 / small / 0.03                         # (float32, as the call takes it)
+    scale = float(torch.tensor(scale, dtype=torch.float32))
+    out, lse = paged_kv.paged_decode_attention(q, s.cache, s.table, s.seq_lens, scale=scale, return_lse=True)
+    _status_clear()
+    for b, n in enumerate(s.lens):
+        k, v = s.rows(b, 0, "k"), s.rows(b, 0, "v")
+        for h in range(4):
+            want, want_lse, mass = ref.attend(used[b, h], k, v, scale)
+            assert abs(float(lse[b, h]) - want_lse) <= ref.lse_tolerance(want_lse, n, 64, mass), (b, h)
+            tol = ref.attention_tolerance(want, n, 64, mass, float(v.abs().max()), typ, False)
+            assert bool(((out[b, h].double() - want).abs() <= tol).all()), (b, h)

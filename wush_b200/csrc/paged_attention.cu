@@ -435,8 +435,8 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS)
         }
         factor[nt][0] = factor[nt][1] = to_exp2;
       } else {
-        // fp16 operands: every query is divided by the power of two below its largest element, so that nothing overflows
-        // and what underflows is below 2^-24 of that element
+        // fp16 operands: every query is scaled by a power of two that puts its largest element between 2^15 and 2^16, so that
+        // nothing overflows, elements keep all their bits down to 2^-29 of it and what they lose below is 2^-40 of it
         float x[KJ][16];
         float top = 0.0f;
 #pragma unroll
@@ -453,14 +453,14 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS)
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // exponent field of the largest element, kept where 2^e and 2^-e are normal numbers; infinities stay infinite
-        const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 253);
-        const float down = __uint_as_float((uint32_t)(254 - e) << 23);
-        const float up = __uint_as_float((uint32_t)e << 23) * to_exp2 * p.kv.k_scale[it.hk];
+        // exponent field of the largest element, kept where both powers are normal numbers; infinities stay infinite
+        const int e = min(max((int)(__float_as_uint(top) >> 23), 16), 254);
+        const float in = __uint_as_float((uint32_t)(254 + 15 - e) << 23);
+        const float up = __uint_as_float((uint32_t)(e - 15) << 23) * to_exp2 * p.kv.k_scale[it.hk];
 #pragma unroll
         for (int j = 0; j < KJ; ++j)
 #pragma unroll
-          for (int k = 0; k < 8; ++k) qf[nt][j * 4 + (k >> 1)][k & 1] = pack2<__half>(x[j][2 * k] * down, x[j][2 * k + 1] * down);
+          for (int k = 0; k < 8; ++k) qf[nt][j * 4 + (k >> 1)][k & 1] = pack2<__half>(x[j][2 * k] * in, x[j][2 * k + 1] * in);
         factor[nt][0] = __shfl_sync(0xffffffffu, up, 8 * c);         // lane 4 h holds head h
         factor[nt][1] = __shfl_sync(0xffffffffu, up, 8 * c + 4);
       }
