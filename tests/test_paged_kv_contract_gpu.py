@@ -1,5 +1,8 @@
 """What the paged key-value cache operators promise beyond their formulas: precision of the weights, copies of a cache,
 lengths that the caller writes, reports of what is left out, refusals."""
+import copy
+import pickle
+
 import pytest
 import torch
 
@@ -57,3 +60,32 @@ def test_small_elements_of_a_query_over_8_bit_pages_keep_their_bits(typ, big, sm
             assert abs(float(lse[b, h]) - want_lse) <= ref.lse_tolerance(want_lse, n, 64, mass), (b, h)
             tol = ref.attention_tolerance(want, n, 64, mass, float(v.abs().max()), typ, False)
             assert bool(((out[b, h].double() - want).abs() <= tol).all()), (b, h)
+
+
+@pytest.mark.parametrize("how", ["deepcopy", "pickle", "copy"])
+@pytest.mark.parametrize("cache", [BF, F8])
+def test_copies_of_a_cache(how, cache):
+    """A copied cache names the copy's pages, not those of the original (copy.copy: the same pages, as of any object)."""
+    from wush_b200 import paged_kv
+    s = Setup([20], page=16, kv=2, dim=64, cache=cache, bounds=True, seed=3, layout="hnd")
+    paged_kv.paged_kv_bounds(s.cache, s.table, s.seq_lens, 20)
+    other = {"deepcopy": copy.deepcopy, "pickle": lambda c: pickle.loads(pickle.dumps(c)), "copy": copy.copy}[how](s.cache)
+    bits = torch.uint8 if cache == F8 else torch.int16
+    before = [t.clone() for t in (s.cache.k.view(bits), s.cache.v.view(bits), s.cache.bounds.view(torch.int16))]
+    x = torch.full((1, 2, 64), 3.0, dtype=BF, device=_dev())
+    at = torch.tensor([19], dtype=torch.int32, device=_dev())
+    ids = torch.zeros_like(at)
+    paged_kv.paged_kv_append(other, x, x, s.table, ids, at)
+    paged_kv.paged_kv_bounds(other, s.table, s.seq_lens, 20)
+    q = _randn(s.g, 1, 4, 64).to(BF)
+    out = paged_kv.paged_decode_attention(q, other, s.table, s.seq_lens)
+    _status_clear()
+    now = (s.cache.k.view(bits), s.cache.v.view(bits), s.cache.bounds.view(torch.int16))
+    if how == "copy":
+        assert not torch.equal(now[0], before[0])
+        return
+    assert all(torch.equal(a, b) for a, b in zip(now, before))
+    page = int(s.table[0, 1])
+    assert not torch.equal(other.k[page, 3].float(), s.cache.k[page, 3].float())
+    paged_kv.paged_kv_append(s.cache, x, x, s.table, ids, at)            # the same token: then both give the same
+    assert torch.equal(paged_kv.paged_decode_attention(q, s.cache, s.table, s.seq_lens), out)

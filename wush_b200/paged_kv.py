@@ -61,7 +61,8 @@ class PagedKVCache:
 
     8-bit pages hold key / k_scale and value / v_scale (float32 [n_kv_heads], positive, given by the caller).  ``bounds``
     [num_pages, n_kv_heads, 2, head_dim] (bfloat16 or float16; the type of 16-bit pages) is what ``paged_kv_bounds``
-    fills and ``paged_select_pages`` reads.  The object keeps references to its tensors; replacing them needs a new one."""
+    fills and ``paged_select_pages`` reads.  The object keeps references to its tensors; replacing them needs a new one.
+    Copies (``copy``, ``pickle``) are made anew around their tensors, so a deep copy has pages of its own."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
                  v_scale: Optional[torch.Tensor] = None, bounds: Optional[torch.Tensor] = None):
@@ -80,6 +81,15 @@ class PagedKVCache:
         self._status = _lib.status_word(self.device).data_ptr()
         self._query_types = (torch.bfloat16, torch.float16) if k.dtype == torch.float8_e4m3fn else (k.dtype,)
         self._attention_scratch = {}                          # bytes by number of query heads
+
+    def __getstate__(self):
+        eight = self.dtype == torch.float8_e4m3fn             # (pickle does not know 8-bit floats)
+        k, v = (t.view(torch.uint8) if eight else t for t in (self.k, self.v))
+        return {"k": k, "v": v, "k_scale": self.k_scale, "v_scale": self.v_scale, "bounds": self.bounds}
+
+    def __setstate__(self, state):                            # the packed addresses become those of the copy's tensors
+        k, v = (t.view(torch.float8_e4m3fn) if t.dtype == torch.uint8 else t for t in (state["k"], state["v"]))
+        self.__init__(k, v, state["k_scale"], state["v_scale"], state["bounds"])
 
     @classmethod
     def allocate(cls, num_pages: int, page_size: int, n_kv_heads: int, head_dim: int, dtype=torch.bfloat16, device=None,
