@@ -10,7 +10,8 @@ namespace kv {
 // ---- append --------------------------------------------------------------------------------------------------------
 using AppendParams = wush_kv_append_args;
 
-// 16 bytes that are read once, past the L1 (not through the read-only path: the outputs may be the inputs)
+// 16 bytes that are read once, past the L1.  Nothing here goes through the read-only path (ld.global.nc): outputs may be the
+// inputs, and a kernel that is launched early is there while the one before it still writes what will be read.
 template <typename T>
 __device__ __forceinline__ uint4 load_once(const T* p) {
   uint4 v;
@@ -82,7 +83,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendPara
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int j = p.interleaved ? i * (p.rotary / 16) : i;
-        const float4 x = __ldg(c + j), y = __ldg(s + j);
+        const float4 x = __ldca(c + j), y = __ldca(s + j);       // (plain loads came later: 25000 tokens in 193 us, so 190)
         cosine[4 * i] = x.x, cosine[4 * i + 1] = x.y, cosine[4 * i + 2] = x.z, cosine[4 * i + 3] = x.w;
         sine[4 * i] = y.x, sine[4 * i + 1] = y.y, sine[4 * i + 2] = y.z, sine[4 * i + 3] = y.w;
       }
@@ -184,7 +185,7 @@ __global__ void __launch_bounds__(128) bounds_kernel(const wush_kv_pages kv, con
       const int page = max(0, __shfl_sync(0xffffffffu, my_page, i)), rows = rows_of(i);
       const C* k = base + page * kv.k_page;
 #pragma unroll
-      for (int x = 0; x < BOUNDS_ROWS; ++x) ahead[x] = ld_nc_v4(k + min(row0 < down ? r0 + row0 + x * down : 0, rows - 1) * kv.k_row);
+      for (int x = 0; x < BOUNDS_ROWS; ++x) ahead[x] = load_once(k + min(row0 < down ? r0 + row0 + x * down : 0, rows - 1) * kv.k_row);
     };
     uint32_t lo[PAIRS], hi[PAIRS];
     load(0, 0);
@@ -416,7 +417,7 @@ __global__ void __launch_bounds__(SCORE_WARPS * 32, J <= 4 ? SCORE_BLOCKS : 2) s
       for (int j = 0; j < J; ++j) {
         const int ch = (j * 4 + c) * 8;
 #pragma unroll
-        for (int y = 0; y < 2; ++y) raw[j][x][y] = ld_nc_v4(bound + y * d + (ch < d ? ch : 0));
+        for (int y = 0; y < 2; ++y) raw[j][x][y] = load_once(bound + y * d + (ch < d ? ch : 0));
       }
     }
     if (group > 8 || held_head != head || held_seq != now.seq) {
