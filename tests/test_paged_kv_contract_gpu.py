@@ -89,3 +89,39 @@ def test_copies_of_a_cache(how, cache):
     assert not torch.equal(other.k[page, 3].float(), s.cache.k[page, 3].float())
     paged_kv.paged_kv_append(s.cache, x, x, s.table, ids, at)            # the same token: then both give the same
     assert torch.equal(paged_kv.paged_decode_attention(q, s.cache, s.table, s.seq_lens), out)
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_decode_step_follows_lengths_written_by_the_caller(captured):
+    """A serving loop puts another sequence into a row by writing seq_lens in place; the token goes where the new length
+    says, in a captured step as well."""
+    from wush_b200 import paged_kv
+    s = Setup([40, 33, 20], page=16, kv=2, dim=64, seed=5)
+    step = paged_kv.DecodeStep(s.table, s.seq_lens.clone())
+    x = [_randn(s.g, 3, n, 64).to(BF) for n in (4, 2, 2)]
+    held = [t.clone() for t in x]
+    graph = None
+    if captured:
+        step.attend(s.cache, *held)                           # warm-up
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step.attend(s.cache, *held)
+    for lens in ([40, 33, 20], [7, 0, 20], [38, 1, 0]):
+        step.seq_lens.copy_(torch.tensor(lens, dtype=torch.int32, device=_dev()))
+        for t, v in zip(held, x):
+            t.copy_(v)
+        want = [(s.cache.k.clone(), s.cache.v.clone())]
+        for b, n in enumerate(lens):
+            if n > 0:
+                page, row = int(s.table[b, (n - 1) // 16]), (n - 1) % 16
+                want[0][0][page, row], want[0][1][page, row] = x[1][b], x[2][b]
+        if graph is not None:
+            graph.replay()
+        else:
+            step.attend(s.cache, *held)
+        _status_clear()
+        for got, w in zip((s.cache.k, s.cache.v), want[0]):
+            assert torch.equal(got.view(torch.int16), w.view(torch.int16)), lens
+        assert step.positions.tolist() == [n - 1 for n in lens]
+    step.advance()
+    assert step.seq_lens.tolist() == [39, 2, 0] and step.positions.tolist() == [38, 1, -1]

@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendPara
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int j = p.interleaved ? i * (p.rotary / 16) : i;
-        const float4 x = __ldca(c + j), y = __ldca(s + j);       // (plain loads came later: 25000 tokens in 193 us, so 190)
+        const float4 x = __ldca(c + j), y = __ldca(s + j);       // (plain loads: 25000 tokens 193 us, so 190)
         cosine[4 * i] = x.x, cosine[4 * i + 1] = x.y, cosine[4 * i + 2] = x.z, cosine[4 * i + 3] = x.w;
         sine[4 * i] = y.x, sine[4 * i + 1] = y.y, sine[4 * i + 2] = y.z, sine[4 * i + 3] = y.w;
       }

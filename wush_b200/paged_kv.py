@@ -115,7 +115,8 @@ class DecodeStep:
     the form of the attention.  ``wush_b200.block.ShardedDecoderBlock.decode`` takes it.
 
     block_table  int32 [sequences, pages]
-    seq_lens     int32 [sequences]: tokens of every sequence, the new one included; 0 for a padded row
+    seq_lens     int32 [sequences]: tokens of every sequence, the new one included; 0 for a padded row.  It may be written
+                 in place between steps (another sequence in a row), between replays of a captured step as well
     rope         fp32 table for ``paged_kv_append`` (None: no rotation), interleaved its pairing
     scale, window  of ``paged_decode_attention``
     top_pages    attend to this many selected pages per key head (0: all); needs caches with bounds
@@ -130,7 +131,7 @@ class DecodeStep:
         self.block_table, self.seq_lens, self.rope, self.interleaved = block_table, seq_lens, rope, interleaved
         self.scale, self.window, self.top_pages = scale, window, top_pages
         self.seq_ids = torch.arange(seq_lens.shape[0], dtype=torch.int32, device=seq_lens.device)
-        self.positions = seq_lens - 1                         # of the new tokens; -1 in a padded row
+        self.positions = seq_lens - 1                         # of the new tokens, -1 in a padded row; attend() writes it
 
     def advance(self) -> None:
         """The next token of every sequence (padded rows stay padding); in place, so that captured steps see it."""
@@ -140,6 +141,7 @@ class DecodeStep:
     def attend(self, cache: PagedKVCache, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
         """Append the new tokens' keys and values ([sequences, heads, head_dim]) to a layer's cache and attend.  ``q`` is
         overwritten, first by the rotated queries, then by the result, and returned."""
+        torch.sub(self.seq_lens, 1, out=self.positions)       # (here, in every layer: nothing tells when seq_lens was written)
         paged_kv_append(cache, k, v, self.block_table, self.seq_ids, self.positions, q=q, rope=self.rope,
                         interleaved=self.interleaved, q_out=q)
         if cache.bounds is not None:
