@@ -114,8 +114,8 @@ def _peer_table(peers, rank: int, world: int):
 
 class _Exchange:
     """Operand buffer of one GEMM input in symmetric memory: `world` slots, slot s holding the codes and the blocked
-    scale bytes rank s produced for its K shard.  put(): quantize the local columns into the own slot, copy the slot
-    into every peer's buffer, barrier."""
+    scale bytes rank s produced for its K shard.  put(): quantize the local columns into the own slot, copy the slot's
+    rows in use into every peer's buffer, barrier."""
 
     def __init__(self, rows: int, k_shard: int, group_size: int, world: int, rank: int, device, pg):
         self.rows, self.ks, self.g, self.world, self.rank = rows, k_shard, group_size, world, rank
@@ -146,9 +146,17 @@ class _Exchange:
         ops.fused_quantize_into(x, matrix, fmt, gs, self.my_codes[:m], self.my_scales, col0=0, sf_layout=_lib.SF_BLOCKED,
                                 row_scale=row_scale, col_scale=col_scale)
         if self.world > 1:
-            lo, hi = self.rank * self.slot, (self.rank + 1) * self.slot
-            _broadcast(self.flat, self.handle, self.peers, self.rank, self.world, lo, hi, self.table)
+            for lo, hi in self.ranges(m):
+                _broadcast(self.flat, self.handle, self.peers, self.rank, self.world, lo, hi, self.table)
             self.handle.barrier(channel=0)
+
+    def ranges(self, m: int):
+        """Bytes [lo, hi) of the buffer that hold m rows of the own slot: codes, and scales in blocks of 128 rows.  (One range
+        when all rows are in use; a step of a few tokens in a slot of 16384 rows moves KBs instead of the slot's MBs.)"""
+        lo = self.rank * self.slot
+        scales = lo + self.code_bytes
+        end = scales + (m + 127) // 128 * 128 * (self.ks // self.g)
+        return [(lo, end)] if m == self.rows else [(lo, lo + m * self.pitch), (scales, end)]
 
     def gemm(self, m: int, w: torch.Tensor, ws_blocked: torch.Tensor, alpha: torch.Tensor, fmt: str, **kw) -> torch.Tensor:
         if self.world == 1:
