@@ -613,7 +613,7 @@ WUSH_API int wush_kv_select_pages(const wush_kv_select_args* args);
  *   seq_lens   int32 [seqs]; a sequence without tokens (len <= 0) gives zeros
  *   pages, counts  null (all pages), or what wush_kv_select_pages writes: for every sequence and key head the first
  *              counts[b, h] entries of pages[b, h, top] are attended to, each cut at len (window must be 0)
- * A length beyond the table, or an entry outside it, sets *status = 2; tokens on such pages are left out.
+ * A length beyond the table, a count beyond `top`, or an entry outside the table sets *status = 2; such tokens are left out.
  *   workspace  wush_kv_attention_workspace_bytes(kv, q_heads) bytes, 16-byte aligned; shared as that of
  *              wush_kv_select_pages
  */

@@ -125,3 +125,22 @@ def test_decode_step_follows_lengths_written_by_the_caller(captured):
         assert step.positions.tolist() == [n - 1 for n in lens]
     step.advance()
     assert step.seq_lens.tolist() == [39, 2, 0] and step.positions.tolist() == [38, 1, -1]
+
+
+def test_counts_beyond_the_list_are_reported():
+    """More selected pages than the list holds: the whole list is attended to, and the count is reported."""
+    from wush_b200 import _lib, paged_kv
+    for page, top in ((16, 3), (16, 90), (24, 3)):            # whole items, cut ones, odd pages
+        s = Setup([page * top + 5, 33], page=page, kv=2, dim=64, seed=11)
+        q = _randn(s.g, 2, 8, 64).to(BF)
+        pages = torch.arange(top, dtype=torch.int32, device=_dev()).flip(0).expand(2, 2, top).contiguous()
+        counts = torch.full((2, 2), top, dtype=torch.int32, device=_dev())
+        counts[1] = 1
+        pages[1] = 0
+        want = paged_kv.paged_decode_attention(q, s.cache, s.table, s.seq_lens, pages=pages, counts=counts)
+        _status_clear()
+        counts[0, 1] = top + 1
+        got = paged_kv.paged_decode_attention(q, s.cache, s.table, s.seq_lens, pages=pages, counts=counts)
+        with pytest.raises(_lib.WushB200Error, match="outside its table"):
+            _lib.check_status(_dev())
+        assert torch.equal(got, want)

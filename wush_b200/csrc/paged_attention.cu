@@ -170,7 +170,7 @@ __device__ __forceinline__ Work work_of(const AttentionParams& p, int64_t entry)
   w.len = clamp_length(p.seq_lens[b], p.table.width * p.kv.page_size, p.status);
   w.begin = p.window > 0 && w.len > p.window ? (int)(w.len - p.window) : 0;
   w.origin = FAST ? w.begin & ~15 : w.begin;
-  w.tokens = p.pages ? max(0, min(p.counts[entry], p.top)) * p.kv.page_size : w.len - w.origin;
+  w.tokens = p.pages ? clamp_length(p.counts[entry], p.top, p.status) * p.kv.page_size : w.len - w.origin;
   return w;
 }
 

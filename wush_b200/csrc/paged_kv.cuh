@@ -154,7 +154,7 @@ __device__ __forceinline__ void store8<__nv_fp8_e4m3>(__nv_fp8_e4m3* p, const fl
                                             pack2_e4m3(x[4], x[5]) | (pack2_e4m3(x[6], x[7]) << 16));
 }
 
-// tokens of a sequence that its table can hold; a longer length is reported
+// tokens of a sequence that its table can hold (or pages that a list can); more than that is reported
 __device__ __forceinline__ int clamp_length(int len, int64_t capacity, int* status) {
   if (len > capacity) {
     report_index(status);

@@ -380,7 +380,7 @@ def paged_decode_attention(q: torch.Tensor, cache: PagedKVCache, block_table: to
     window     only the last ``window`` tokens; 0: all
     pages, counts  attend to the tokens of these pages only: for every sequence and key head the first counts[b, h]
                entries of pages[b, h], logical page numbers as ``paged_select_pages`` returns them (any order; a page
-               listed twice counts twice).  Not together with a window.
+               listed twice counts twice; no page at a count <= 0).  Not together with a window.
     out        receives the result instead of a new tensor; it may be ``q``, and must not overlap it otherwise
     """
     typ = _query_type(cache, q, "q")
