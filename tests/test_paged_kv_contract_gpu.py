@@ -144,3 +144,22 @@ def test_counts_beyond_the_list_are_reported():
         with pytest.raises(_lib.WushB200Error, match="outside its table"):
             _lib.check_status(_dev())
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("page", [16, 24])
+@pytest.mark.parametrize("entry", [-2 ** 31, -1, 2 ** 31 - 1])
+def test_every_table_entry_outside_the_pool_is_reported(page, entry):
+    from wush_b200 import _lib, paged_kv
+    s = Setup([3 * page], page=page, kv=2, dim=64, seed=6)
+    q = _randn(s.g, 1, 4, 64).to(BF)
+    good = s.table.clone()
+    s.table[0, 1] = entry
+    out = paged_kv.paged_decode_attention(q, s.cache, s.table, s.seq_lens)
+    with pytest.raises(_lib.WushB200Error, match="outside its table"):
+        _lib.check_status(_dev())
+    pages = torch.tensor([[[0, 2]] * 2], dtype=torch.int32, device=_dev())
+    counts = torch.full((1, 2), 2, dtype=torch.int32, device=_dev())
+    want = paged_kv.paged_decode_attention(q, s.cache, good, s.seq_lens, pages=pages, counts=counts)
+    _status_clear()
+    # the same 2 * page tokens, in tiles that start elsewhere: both within the tolerance of the float64 result
+    assert float((out.float() - want.float()).abs().max()) <= 2 * 2.0 ** -8 * float(want.float().abs().max()) + 1e-4

@@ -336,7 +336,8 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS)
       }
       return {lp, row, lp * page_size + row};
     };
-    auto physical = [&](Row x) -> Row { return {x.page >= 0 && x.pos < w.len ? table[x.page] : NOTHING, x.row, x.pos}; };
+    // (a negative entry becomes -1, so that none of them is NOTHING)
+    auto physical = [&](Row x) -> Row { return {x.page >= 0 && x.pos < w.len ? max(table[x.page], -1) : NOTHING, x.row, x.pos}; };
     // the current page (0 where there is none) and row, and the tokens that count: one, or with FAST the 16 from there
     int page = 0, page_row = 0;
     unsigned counts16 = 0;
