@@ -163,3 +163,25 @@ def test_every_table_entry_outside_the_pool_is_reported(page, entry):
     _status_clear()
     # the same 2 * page tokens, in tiles that start elsewhere: both within the tolerance of the float64 result
     assert float((out.float() - want.float()).abs().max()) <= 2 * 2.0 ** -8 * float(want.float().abs().max()) + 1e-4
+
+
+def test_outputs_whose_rows_or_heads_share_memory_are_refused():
+    from wush_b200 import paged_kv
+    s = Setup([40, 20], page=16, kv=2, dim=64)
+    q, k = _randn(s.g, 2, 4, 64).to(BF), _randn(s.g, 2, 2, 64).to(BF)
+    ids = torch.arange(2, dtype=torch.int32, device=_dev())
+    for bad in (q[:1].expand(2, 4, 64), q[:, :1].expand(2, 4, 64)):
+        with pytest.raises(ValueError, match="overlap"):
+            paged_kv.paged_decode_attention(q, s.cache, s.table, s.seq_lens, out=bad)
+        with pytest.raises(ValueError, match="overlap"):
+            paged_kv.paged_kv_append(s.cache, k, k, s.table, ids, ids, q=q, q_out=bad)
+    for bad in (k[:1].expand(2, 2, 64), k[:, :1].expand(2, 2, 64)):
+        with pytest.raises(ValueError, match="overlap"):
+            paged_kv.paged_kv_append(s.cache, k, k, s.table, ids, ids, k_out=bad)
+    # inputs may: one key for all heads, one query for all sequences
+    same = k[:, :1].expand(2, 2, 64)
+    paged_kv.paged_kv_append(s.cache, same, same, s.table, ids, ids)
+    got = paged_kv.paged_decode_attention(q[:1].expand(2, 4, 64), s.cache, s.table, s.seq_lens)
+    _status_clear()
+    want = paged_kv.paged_decode_attention(q[:1].expand(2, 4, 64).contiguous(), s.cache, s.table, s.seq_lens)
+    assert torch.equal(got, want) and torch.equal(s.cache.k[int(s.table[1, 0]), 1, 1], k[1, 0])

@@ -219,6 +219,14 @@ def _heads(cache: PagedKVCache, t: torch.Tensor, rows: int, heads: int, dtype, w
     return p, row, head
 
 
+def _output(cache: PagedKVCache, t: torch.Tensor, rows: int, heads: int, dtype, what: str):
+    """_heads of a tensor that is written: its rows and heads must not be one and the same (an expanded tensor)."""
+    p, row, head = _heads(cache, t, rows, heads, dtype, what)
+    if (row == 0 and rows > 1) or (head == 0 and heads > 1):
+        raise ValueError(f"{what}: rows and heads must not overlap")
+    return p, row, head
+
+
 def _query_type(cache: PagedKVCache, t: torch.Tensor, what: str):
     """Element type of a call's queries, keys and values: that of 16-bit pages, either 16-bit type for 8-bit pages."""
     if t.dtype not in cache._query_types:
@@ -293,11 +301,11 @@ def paged_kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, block
         hq = _heads(cache, q, rows, n_heads, typ, "q")
         if q_out is None:
             q_out = torch.zeros_like(q, memory_format=torch.contiguous_format)
-        hqo = _heads(cache, q_out, rows, n_heads, typ, "q_out")
+        hqo = _output(cache, q_out, rows, n_heads, typ, "q_out")
     elif q_out is not None:
         raise ValueError("q_out goes with q")
     if k_out is not None:
-        hko = _heads(cache, k_out, rows, kv_heads, typ, "k_out")
+        hko = _output(cache, k_out, rows, kv_heads, typ, "k_out")
     rope_ptr, rope_rows, rotary = 0, 0, 0
     if rope is not None:
         if rope.dim() != 2 or rope.dtype is not torch.float32 or not rope.is_contiguous() or rope.get_device() != cache._index \
@@ -404,7 +412,7 @@ def paged_decode_attention(q: torch.Tensor, cache: PagedKVCache, block_table: to
         counts_ptr = _int32(counts, (seqs, cache.n_kv_heads), "counts", cache._index)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    ho = _heads(cache, out, seqs, n_heads, typ, "out")
+    ho = _output(cache, out, seqs, n_heads, typ, "out")
     lse = torch.empty((seqs, n_heads), dtype=torch.float32, device=cache.device) if return_lse else None
     if seqs > 0:
         lib, stream = _lib.load(), _stream(cache)
