@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from tests import paged_reference as ref
-from tests.test_paged_kv_gpu import BF, F8, HF, Setup, _dev, _randn, _status_clear
+from tests.test_paged_kv_gpu import BF, F8, HF, Setup, _dev, _gen, _randn, _status_clear
 
 pytestmark = pytest.mark.gpu
 
@@ -185,3 +185,68 @@ def test_outputs_whose_rows_or_heads_share_memory_are_refused():
     _status_clear()
     want = paged_kv.paged_decode_attention(q[:1].expand(2, 4, 64).contiguous(), s.cache, s.table, s.seq_lens)
     assert torch.equal(got, want) and torch.equal(s.cache.k[int(s.table[1, 0]), 1, 1], k[1, 0])
+
+
+def _fp32_scores(q, cache, table, lens, top):
+    """(value, magnitude) float32 [sequences, key heads, pages]: what the scoring kernel leaves in the call's workspace."""
+    from wush_b200 import _lib, paged_kv
+    lib = _lib.load()
+    seqs, width, kv = table.shape[0], table.shape[1], cache.n_kv_heads
+    work = torch.zeros(lib.wush_kv_select_workspace_bytes(seqs, kv, width), dtype=torch.uint8, device=_dev())
+    pages = torch.empty(seqs, kv, top, dtype=torch.int32, device=_dev())
+    counts = torch.empty(seqs, kv, dtype=torch.int32, device=_dev())
+    rc = lib.wush_kv_select_pages(cache._packed + paged_kv._SELECT.pack(
+        table.data_ptr(), table.stride(0), seqs, width, q.data_ptr(), q.stride(0), q.stride(1), lens.data_ptr(), pages.data_ptr(),
+        counts.data_ptr(), work.data_ptr(), work.numel(), cache._status, torch.cuda.current_stream().cuda_stream,
+        paged_kv.TYPES[q.dtype], q.shape[1], top, 0, 0))
+    assert rc == 0
+    torch.cuda.synchronize()
+    return work.view(torch.float32).view(seqs, kv, width, 2).unbind(-1)
+
+
+@pytest.mark.parametrize("typ,bounds", [(BF, BF), (HF, HF), (HF, BF), (BF, HF)])
+@pytest.mark.parametrize("dim", [8, 16, 40, 64, 80, 128, 208, 256])
+def test_fp32_scores_stay_within_the_bound_that_the_selection_uses(typ, bounds, dim):
+    """The selection trusts fp32 scores up to a bound: each product of 16 terms is off by at most 17 * 2^-23 of its terms'
+    magnitude, and 4 * ceil(dim / 32) products are added with 2^-24 of the magnitude each.  Terms of very mixed size: every
+    addend's own cut counts.  (1 + 2^-10: errors of errors.)"""
+    from wush_b200.paged_kv import PagedKVCache
+    width, kv, group = 400, 2, 3
+    g, dev = _gen(dim), _dev()
+    cache = typ if typ == bounds else F8
+    dim = -(-dim // 16) * 16 if cache == F8 else dim
+    one = torch.ones(kv, device=dev)
+    data = torch.zeros(width, 1, kv, dim, dtype=cache, device=dev)
+    pool = PagedKVCache(data, data, k_scale=one if cache == F8 else None, v_scale=one if cache == F8 else None,
+                        bounds=torch.zeros(width, kv, 2, dim, dtype=bounds, device=dev))
+    spread = lambda *shape: torch.exp2(torch.randint(-13, 1, shape, generator=g, device=dev).float())
+    x = _randn(g, width, kv, 2, dim) * spread(width, kv, 1, dim)
+    # a third of the pages: one large term a product, the others around the last bit of it and of one sign
+    some = torch.arange(width, device=dev) % 3 == 0
+    small = (1 + torch.rand(width, kv, 1, dim, generator=g, device=dev)) * 2.0 ** -11
+    small[..., ::16] = 1.0 + torch.rand(width, kv, 1, dim, generator=g, device=dev)[..., ::16]
+    x[some] = small.expand(width, kv, 2, dim)[some]
+    if cache == F8:                                           # bounds of 8-bit keys are 8-bit numbers
+        x = (x * 128).clamp(-448, 448).to(F8).float()
+    low, high = x.amin(2).to(bounds), x.amax(2).to(bounds)
+    pool.bounds[:, :, 0], pool.bounds[:, :, 1] = low, high
+    table = torch.randperm(width, generator=g, device=dev).to(torch.int32)[None]
+    lens = torch.tensor([width], dtype=torch.int32, device=dev)
+    q = (_randn(g, 1, kv * group, dim) * spread(1, kv * group, dim)).to(typ)
+    q[0, 0] = 2.0 ** -12 * (1 + torch.rand(dim, generator=g, device=dev)).to(typ)
+    q[0, 0, ::16] = 1.5
+    value, magnitude = _fp32_scores(q, pool, table, lens, 5)
+    _status_clear()
+    rel = (17 + 2 * -(-dim // 32)) * 2.0 ** -23 * (1 + 2.0 ** -10)
+    at = table[0].long()
+    worst = 0.0
+    for h in range(kv):
+        qs = q[0, h * group:(h + 1) * group].double()
+        lo, hi = low[at, h].double(), high[at, h].double()
+        exact = torch.maximum(qs[:, None] * lo, qs[:, None] * hi).sum(2).amax(0)
+        most = (qs.abs()[:, None] * torch.maximum(lo.abs(), hi.abs())).sum(2).amax(0)
+        err = (value[0, h].double() - exact).abs()
+        worst = max(worst, float((err / (rel * most)).max()))
+        assert bool((err <= rel * most + 2.0 ** -120).all()), float((err / (rel * most)).max())
+        assert bool((magnitude[0, h].double() >= most * (1 - 1 / 32)).all())
+    print(f"dim {dim}: worst error {worst:.3f} of the bound")

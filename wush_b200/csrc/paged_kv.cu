@@ -285,9 +285,11 @@ __global__ void __launch_bounds__(128) bounds_kernel(const wush_kv_pages kv, con
 //      are scored again in 64 bits and ranked.
 // Error of an fp32 score: an m16n8k16 product of its own (nothing to add to) adds 16 exact products; if each addend and the
 // result is cut to 24 bits at the scale of the largest, it is off by at most 17 * 2^-23 of its terms' magnitude.  The
-// 2 * ceil(dim / 16) products of a score are added in fp32, 2^-24 of the magnitude each.  (Chained through the product's
-// accumulator every product would add 18 * 2^-23 of the whole magnitude: 16 times as many pages lay between, and scoring them
-// again took 5 to 10 us.)
+// 4 * ceil(dim / 32) products of a score (a step of 32 channels makes two with the upper bounds and two with the lower) are
+// added in fp32, 2^-24 of the magnitude each.  PTX leaves open how a product's sum is rounded; measured over terms of very
+// mixed size the errors stay below an eighth of this bound (tests/test_paged_kv_contract_gpu.py holds them to it).  (Chained
+// through the product's accumulator every product would add 18 * 2^-23 of the whole magnitude: 16 times as many pages lay
+// between, and scoring them again took 5 to 10 us.)
 struct Score {
   float value, magnitude;               // magnitude: infinity when the score has to be computed again in any case
 };
@@ -805,7 +807,7 @@ __global__ void __launch_bounds__(1024) select_kernel(const wush_kv_select_args 
   }
   // (17 + products / 2) * 2^-23 of the magnitude, a sixteenth more for the magnitude's own rounding, and what numbers below the
   // smallest normal one may lose
-  const float eps = magnitude * (float)(17 + (a.kv.dim + 15) / 16) * (1.0625f / 8388608.0f) + 1024.0f * FLT_MIN;
+  const float eps = magnitude * (float)(17 + 2 * ((a.kv.dim + 31) / 32)) * (1.0625f / 8388608.0f) + 1024.0f * FLT_MIN;
   // a magnitude that is not finite leaves everything between; where the k-th is a page outside the pool, all that are in it
   // are above
   const float center = key_float(kth);
