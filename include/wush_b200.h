@@ -580,8 +580,9 @@ WUSH_API int wush_kv_bounds(const wush_kv_bounds_args* args);
  * Select, for every sequence and key head, at most `top` pages to attend to: the first `sink` and the last `recent`
  * pages of the sequence, then those with the largest scores; equal scores: the lowest page.
  * score = max over the head's queries of sum_d max(q_d lower_d, q_d upper_d), an upper bound of every logit on the page
- * (before the softmax scale), accumulated in 64 bits.  A page one of whose bounds is not finite, and a score that is not
- * finite, count as +infinity; a page outside the pool comes last.
+ * (before the softmax scale); near the border accumulated in 64 bits, which is exact while the terms and partial sums of a
+ * page fit 53 bits.  A page one of whose bounds is not finite, and a score that is not finite, count as +infinity; a page
+ * outside the pool comes last.
  *   q        [seqs, q_heads, dim] of `type`; q_heads % kv.heads == 0
  *   pages    int32 [seqs, kv.heads, top] out: logical pages in ascending order, then -1
  *   counts   int32 [seqs, kv.heads] out: how many

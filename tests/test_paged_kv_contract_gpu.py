@@ -1,6 +1,7 @@
 """What the paged key-value cache operators promise beyond their formulas: precision of the weights, copies of a cache,
 lengths that the caller writes, reports of what is left out, refusals."""
 import copy
+import math
 import pickle
 
 import pytest
@@ -250,3 +251,31 @@ def test_fp32_scores_stay_within_the_bound_that_the_selection_uses(typ, bounds, 
         assert bool((err <= rel * most + 2.0 ** -120).all()), float((err / (rel * most)).max())
         assert bool((magnitude[0, h].double() >= most * (1 - 1 / 32)).all())
     print(f"dim {dim}: worst error {worst:.3f} of the bound")
+
+
+@pytest.mark.parametrize("span", [20, 40, 100])
+def test_choice_of_scores_that_64_bits_cannot_hold(span):
+    """Terms of 2^span and -2^span around small ones.  What is chosen has the largest exact scores, up to the rounding of 64-bit
+    sums: 64 additions (and as many products, exact) of 2^-53 of the magnitude each, on either side."""
+    from wush_b200.paged_kv import PagedKVCache, paged_select_pages
+    width, dim = 500, 64
+    g, dev = _gen(span), _dev()
+    pool = PagedKVCache.allocate(width, 1, 1, dim, device=dev, bounds=True)
+    x = _randn(g, width, dim) * torch.exp2(torch.randint(-span, span // 2, (width, dim), generator=g, device=dev).float())
+    at = torch.randint(0, dim // 2, (width,), generator=g, device=dev)
+    rows = torch.arange(width, device=dev)
+    x[rows, at], x[rows, at + dim // 2] = 2.0 ** span, -2.0 ** span
+    pool.bounds[:, 0] = x.to(BF)[:, None]
+    q = torch.ones(1, 1, dim, dtype=BF, device=dev)
+    table = torch.arange(width, dtype=torch.int32, device=dev)[None]
+    lens = torch.tensor([width], dtype=torch.int32, device=dev)
+    terms = x.to(BF).double().tolist()
+    exact = [math.fsum(t) for t in terms]
+    slack = 2 * dim * 2.0 ** -53 * max(sum(abs(y) for y in t) for t in terms)
+    for top in (1, 60, 300):
+        pages, counts = paged_select_pages(q, pool, table, lens, top, sink=0, recent=0)
+        chosen = set(pages[0, 0].tolist())
+        assert len(chosen) == top == int(counts[0, 0])
+        worst, best = min(exact[i] for i in chosen), max(exact[i] for i in range(width) if i not in chosen)
+        assert worst >= best - slack, (top, worst, best, slack)
+    _status_clear()

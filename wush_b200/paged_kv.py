@@ -346,10 +346,12 @@ def paged_select_pages(q: torch.Tensor, cache: PagedKVCache, block_table: torch.
 
     For every sequence and key head: its first ``sink`` and last ``recent`` pages, then the pages with the largest
     scores up to ``top`` in all (equal scores: the lowest page first).  A page's score is the largest, over the queries
-    that share the key head, of sum_d max(q_d lower_d, q_d upper_d): no logit on the page exceeds it.  It is summed in
-    64 bits, so that the choice does not depend on the order of the sum.  A page one of whose bounds is not finite, and a
-    score that is not finite, count as +infinity.  Pages come in ascending order, followed by -1; a sequence of at most ``top`` pages gets all of them.  q: [sequences, heads,
-    head_dim], as ``paged_decode_attention`` takes it; ``cache.bounds`` must be up to date (``paged_kv_bounds``)."""
+    that share the key head, of sum_d max(q_d lower_d, q_d upper_d): no logit on the page exceeds it.  Scores near the border
+    are summed in 64 bits: exactly, whatever the order, where the terms of a page and their partial sums fit 53 bits, and to
+    64-bit rounding (dim * 2^-53 of the terms' magnitude) otherwise.  A page one of whose bounds is not finite, and a score
+    that is not finite, count as +infinity.  Pages come in ascending order, followed by -1; a sequence of at most ``top``
+    pages gets all of them.  q: [sequences, heads, head_dim], as ``paged_decode_attention`` takes it; ``cache.bounds`` must be
+    up to date (``paged_kv_bounds``)."""
     if cache.bounds is None:
         raise ValueError("the cache has no bounds")
     if top < 1 or sink < 0 or recent < 0 or sink + recent > top:
