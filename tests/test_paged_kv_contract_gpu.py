@@ -279,3 +279,20 @@ def test_choice_of_scores_that_64_bits_cannot_hold(span):
         worst, best = min(exact[i] for i in chosen), max(exact[i] for i in range(width) if i not in chosen)
         assert worst >= best - slack, (top, worst, best, slack)
     _status_clear()
+
+
+@pytest.mark.parametrize("width", [34, 130, 700, 2100, 9000])
+def test_selection_among_pages_that_are_all_equal(width):
+    from wush_b200.paged_kv import PagedKVCache, paged_select_pages
+    dev, seqs = _dev(), 40
+    pool = PagedKVCache.allocate(width, 1, 2, 16, device=dev, bounds=True)
+    table = torch.arange(width, dtype=torch.int32, device=dev).expand(seqs, width)
+    lens = torch.full((seqs,), width, dtype=torch.int32, device=dev)
+    q = torch.ones(seqs, 4, 16, dtype=BF, device=dev)
+    for value in (0.0, 3.0):                                  # bounds not filled yet, and filled alike
+        pool.bounds.fill_(value)
+        for top, sink, recent in ((33, 0, 0), (width // 2, 1, 3), (1, 0, 1)):
+            pages, counts = paged_select_pages(q, pool, table, lens, top, sink=sink, recent=recent)
+            want = list(range(top - recent)) + list(range(width - recent, width))
+            assert bool((counts == top).all()) and bool((pages == torch.tensor(want, dtype=torch.int32, device=dev)).all())
+    _status_clear()

@@ -541,7 +541,7 @@ __device__ __forceinline__ int scan256(int* x, int count) {
 }
 
 constexpr int BORDER = 256;                                  // pages between that are ranked in shared memory
-constexpr int FEW = 32;                                      // keys that a warp ranks
+constexpr int FEW = 32;                                      // keys that a warp ranks (and as many warps at most)
 
 struct SelectShared {
   int hist[256];
@@ -800,10 +800,11 @@ __global__ void __launch_bounds__(1024) select_kernel(const wush_kv_select_args 
     __syncthreads();
     kth = sm.kth;
   } else {
+    // (`few`, which nobody reads on this way: the selection's own words may still be read by a warp that is behind)
     kth = __reduce_min_sync(0xffffffffu, kth);
-    if (lane == 0) sm.low[warp] = kth;
+    if (lane == 0) sm.few[warp] = kth;
     __syncthreads();
-    kth = __reduce_min_sync(0xffffffffu, lane < warps ? (uint32_t)sm.low[lane] : ~0u);
+    kth = __reduce_min_sync(0xffffffffu, lane < warps ? sm.few[lane] : ~0u);
   }
   // (17 + products / 2) * 2^-23 of the magnitude, a sixteenth more for the magnitude's own rounding, and what numbers below the
   // smallest normal one may lose
