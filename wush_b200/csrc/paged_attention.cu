@@ -19,8 +19,9 @@
 //
 // Work.  The tokens of all (sequence, key head, chunk of queries) items are cut into units of 4 tiles (one per warp), the
 // units of all items are numbered through, and every block of a grid that fills the GPU exactly once takes an equal run
-// of them, teams of blocks the same run for neighbouring key heads; lengths are read on the device.  A block that holds a whole item writes its result; a part of an item goes to
-// the workspace, and a second kernel joins the parts (every block has at most two: its first and its last item).
+// of them, teams of blocks the same run for neighbouring key heads; lengths are read on the device.  A block that holds a
+// whole item writes its result; a part of an item goes to the workspace, and a second kernel joins the parts (every block has
+// at most two: its first and its last item).
 #include <type_traits>
 
 #include "paged_kv.cuh"
@@ -125,18 +126,6 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
 template <int PITCH_B>
 __device__ __forceinline__ constexpr int swizzled(int at) {
   return at ^ ((at >> 3) & (PITCH_B == 128 ? 0x70 : 0x30));
-}
-
-template <typename M>
-__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  if (std::is_same<M, __half>::value)
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  else
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 // transpose of an 8 x 8 matrix of 16-bit numbers held by the warp (row = lane / 4, two columns per lane)
@@ -739,8 +728,8 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, C, DP, NT>::BLOCKS)
 
 // ---- join of the parts -------------------------------------------------------------------------------------------------
 // Block (k, h) joins the parts of the item that block k of the attention left unfinished, for query head h of its chunk: the
-// first part is block k's, the others are in slot 0 of the same member of the teams after it.  32 parts at a time, eight a warp, all loaded
-// before the first is used: the kernel is a chain of latencies (note, parts, result).
+// first part is block k's, the others are in slot 0 of the same member of the teams after it.  32 parts at a time, eight a
+// warp, all loaded before the first is used: the kernel is a chain of latencies (note, parts, result).
 constexpr int JOIN_WARPS = 4, JOIN_ROWS = 32 / JOIN_WARPS;
 template <typename T, typename C, int DP, int NT>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const AttentionParams p) {

@@ -29,11 +29,11 @@ __device__ __forceinline__ void widen8(uint4 v, float (&x)[8]) {
   }
 }
 
-// One block per row and `span` heads.  A thread has one unit of 16 channels (two chunks of 8 that are turned against each
-// other, or two that are only copied) of every `lanes`-th head, so that the angles of its unit are loaded once for all of them.
-// A pure pass over memory: q, k and v once in, once out.  BATCH heads are under way while the row's position and page are
-// looked up (position, then page and angles: a chain of two latencies that a block would otherwise wait for with nothing
-// in flight).
+// A block takes `span` heads of a row, and the grid walks over the rows.  A thread has one unit of 16 channels (two chunks of 8
+// that are turned against each other, or two that are only copied) of every `lanes`-th head, so that the angles of its unit are
+// loaded once for all of them.  A pure pass over memory: q, k and v once in, once out.  BATCH heads are under way while the
+// row's position and page are looked up (position, then page and angles: a chain of two latencies that a block would otherwise
+// wait for with nothing in flight).
 constexpr int APPEND_BATCH = 5, APPEND_THREADS = 128;
 template <typename T, typename C>
 __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendParams p, int span) {
@@ -307,18 +307,6 @@ __device__ __forceinline__ unsigned long long score_key(double s) {
   return b < 0 ? ~(unsigned long long)b : (unsigned long long)b | 0x8000000000000000ull;
 }
 
-template <typename T>
-__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if (std::is_same<T, __half>::value)
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
 // A pair of bounds in the queries' type; NaN where that is not exact (E4M3 keys are exact in both).
 template <typename T, typename B>
 __device__ __forceinline__ uint32_t as_query_type(uint32_t pair) {
@@ -463,13 +451,13 @@ __global__ void __launch_bounds__(SCORE_WARPS * 32, J <= 4 ? SCORE_BLOCKS : 2) s
           const uint32_t al[4] = {lo[0][i], lo[1][i], lo[0][i + 1], lo[1][i + 1]}, ah[4] = {hi[0][i], hi[1][i], hi[0][i + 1], hi[1][i + 1]};
           const uint32_t ab[4] = {big[0][i], big[1][i], big[0][i + 1], big[1][i + 1]};
           float plus[4] = {}, minus[4] = {};
-          mma_16816<T>(plus, ah, max2<T>(qw[i], 0), max2<T>(qw[i + 1], 0));
-          mma_16816<T>(minus, al, min2<T>(qw[i], 0), min2<T>(qw[i + 1], 0));
+          mma<T>(plus, ah[0], ah[1], ah[2], ah[3], max2<T>(qw[i], 0), max2<T>(qw[i + 1], 0));
+          mma<T>(minus, al[0], al[1], al[2], al[3], min2<T>(qw[i], 0), min2<T>(qw[i + 1], 0));
 #pragma unroll
           for (int x = 0; x < 4; ++x) s[x] += plus[x];
 #pragma unroll
           for (int x = 0; x < 4; ++x) s[x] += minus[x];
-          mma_16816<T>(m, ab, qw[i] & 0x7fff7fffu, qw[i + 1] & 0x7fff7fffu);
+          mma<T>(m, ab[0], ab[1], ab[2], ab[3], qw[i] & 0x7fff7fffu, qw[i + 1] & 0x7fff7fffu);
         }
       }
       // the lane has pages r and r + 8, and queries g0 + 2c and g0 + 2c + 1
@@ -725,10 +713,11 @@ __device__ void write_pages(SelectShared& sm, int rounds, int need, int among, T
   }
 }
 
-// One block per (sequence, key head).  A thread holds every blockDim-th score, up to ROWS of them (ROWS is 4 or 8, or 0
-// for more pages than that: then they are read again for every pass).  A chain of latencies: of barriers, and of instructions that come
-// for the first time, so few of them count (scores and selection of 64 of 2047 pages in a captured graph: 12.7 us with all bits
-// of the k-th found by counting, lengths before scores, three cases in every comparison and 8 scores a thread; 9.6 us as it is).
+// One block per (sequence, key head).  A thread holds every blockDim-th score, up to ROWS of them (ROWS is 4 or 8, or 0 for
+// more pages than that: then they are read again for every pass).  A chain of latencies: of barriers, and of instructions that
+// come for the first time, so few of them count (scores and selection of 64 of 2047 pages in a captured graph: 12.7 us with
+// all bits of the k-th found by counting, lengths before scores, three cases in every comparison and 8 scores a thread; 9.6 us
+// as it is).
 template <typename T, typename B, int ROWS>
 __global__ void __launch_bounds__(1024) select_kernel(const wush_kv_select_args a, int group, Score* scores) {
   __shared__ SelectShared sm;

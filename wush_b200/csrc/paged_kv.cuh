@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -103,25 +104,20 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&p);
 }
 
-// two E4M3 bytes (low byte first) <-> two numbers; NaN stays NaN, the store saturates at +-448
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two_bytes) {
-  uint32_t h;
-  asm("{\n.reg .b16 t;\ncvt.u16.u32 t, %1;\ncvt.rn.f16x2.e4m3x2 %0, t;\n}\n" : "=r"(h) : "r"(two_bytes));
-  return h;
-}
-// the same for all four bytes of a word
+// four E4M3 bytes as two pairs of fp16 (exact; NaN stays NaN)
 __device__ __forceinline__ void e4m3x4_to_f16x4(uint32_t four_bytes, uint32_t& lo, uint32_t& hi) {
   asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\ncvt.rn.f16x2.e4m3x2 %0, l;\ncvt.rn.f16x2.e4m3x2 %1, h;\n}\n"
       : "=r"(lo), "=r"(hi)
       : "r"(four_bytes));
 }
+// two numbers as E4M3 bytes, low byte first; NaN stays NaN, the rest saturates at +-448
 __device__ __forceinline__ uint32_t pack2_e4m3(float lo, float hi) {
   uint16_t h;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(h) : "f"(hi), "f"(lo));
   return h;
 }
 
-// 8 channels of a row as fp32; `p` points at the first of them
+// 8 channels of a row of 16-bit numbers as fp32; `p` points at the first of them
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
   const uint4 v = *reinterpret_cast<const uint4*>(p);
@@ -129,17 +125,6 @@ __device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 f = to_float2<T>(w[i]);
-    x[2 * i] = f.x;
-    x[2 * i + 1] = f.y;
-  }
-}
-template <>
-__device__ __forceinline__ void load8<__nv_fp8_e4m3>(const __nv_fp8_e4m3* p, float (&x)[8]) {
-  const uint2 v = *reinterpret_cast<const uint2*>(p);
-  const uint32_t w[2] = {v.x, v.y};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = to_float2<__half>(e4m3x2_to_f16x2(w[i >> 1] >> (16 * (i & 1))));
     x[2 * i] = f.x;
     x[2 * i + 1] = f.y;
   }
@@ -152,6 +137,20 @@ template <>
 __device__ __forceinline__ void store8<__nv_fp8_e4m3>(__nv_fp8_e4m3* p, const float (&x)[8]) {
   *reinterpret_cast<uint2*>(p) = make_uint2(pack2_e4m3(x[0], x[1]) | (pack2_e4m3(x[2], x[3]) << 16),
                                             pack2_e4m3(x[4], x[5]) | (pack2_e4m3(x[6], x[7]) << 16));
+}
+
+// ---- products ------------------------------------------------------------------------------------------------------
+// d [16 x 8] += a [16 x 16] . b [16 x 8] of fp16 (M is __half) or bf16 numbers
+template <typename M>
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if (std::is_same<M, __half>::value)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 // tokens of a sequence that its table can hold (or pages that a list can); more than that is reported
