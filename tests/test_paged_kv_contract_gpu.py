@@ -296,3 +296,41 @@ def test_selection_among_pages_that_are_all_equal(width):
             want = list(range(top - recent)) + list(range(width - recent, width))
             assert bool((counts == top).all()) and bool((pages == torch.tensor(want, dtype=torch.int32, device=dev)).all())
     _status_clear()
+
+
+@pytest.mark.parametrize("width,odd", [(300, 1), (300, 40), (300, 290), (2047, 3), (2047, 700), (9000, 5), (9000, 300)])
+@pytest.mark.parametrize("typ,bounds", [(BF, BF), (HF, HF), (BF, HF)])
+def test_pages_with_a_bound_that_is_not_finite_do_not_hide_the_others(typ, bounds, width, odd):
+    """Such a page counts as +infinity; the fp32 scores of all others stand, and the choice is that of exact scores."""
+    from wush_b200.paged_kv import PagedKVCache, paged_select_pages
+    g, dev, dim, kv = _gen(width + odd), _dev(), 48, 2
+    cache = typ if typ == bounds else F8
+    one = torch.ones(kv, device=dev)
+    data = torch.zeros(width, 1, kv, dim, dtype=cache, device=dev)
+    pool = PagedKVCache(data, data, k_scale=one if cache == F8 else None, v_scale=one if cache == F8 else None,
+                        bounds=torch.zeros(width, kv, 2, dim, dtype=bounds, device=dev))
+    pool.bounds.copy_(_randn(g, width, kv, 2, dim).sort(dim=2).values.to(F8).to(bounds) if cache == F8 else
+                      _randn(g, width, kv, 2, dim).sort(dim=2).values.to(bounds))
+    table = torch.randperm(width, generator=g, device=dev).to(torch.int32)[None]
+    who = torch.randperm(width, generator=g, device=dev)[:odd]          # logical pages
+    channel = torch.randint(0, dim, (odd,), generator=g, device=dev)
+    kinds = torch.tensor([math.inf, -math.inf, math.nan], device=dev)[torch.arange(odd, device=dev) % 3].to(bounds)
+    pool.bounds[table[0][who].long(), 0, torch.arange(odd, device=dev) % 2, channel] = kinds      # key head 0 only
+    q = _randn(g, 1, 6, dim).to(typ)
+    q[0, 1, channel[0]] = 0.0
+    lens = torch.tensor([width], dtype=torch.int32, device=dev)
+    _, magnitude = _fp32_scores(q, pool, table, lens, min(odd + 5, width - 1))       # (fewer: hundreds of equal ones at the border)
+    at = table[0].long()
+    low, high = pool.bounds[at, :, 0].double(), pool.bounds[at, :, 1].double()
+    strange = torch.zeros(width, dtype=torch.bool, device=dev)
+    strange[who] = True
+    assert bool(magnitude.isfinite().all())
+    for top, sink, recent in ((max(1, odd // 2), 0, 0), (min(odd, width - 1), 0, 0), (min(odd + 20, width - 1), 1, 1)):
+        pages, counts = paged_select_pages(q, pool, table, lens, top, sink=sink, recent=recent)
+        for h in range(kv):
+            qs = q[0, 3 * h:3 * h + 3].double()
+            score = torch.maximum(qs[:, None] * low[:, h], qs[:, None] * high[:, h]).sum(2).amax(0)
+            if h == 0:
+                score[strange] = math.inf
+            assert pages[0, h].tolist() == ref.select(score.tolist(), top, sink, recent), (top, h)
+    _status_clear()

@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(128) bounds_kernel(const wush_kv_pages kv, con
 // through the product's accumulator every product would add 18 * 2^-23 of the whole magnitude: 16 times as many pages lay
 // between, and scoring them again took 5 to 10 us.)
 struct Score {
-  float value, magnitude;               // magnitude: infinity when the score has to be computed again in any case
+  float value, magnitude;               // magnitude: infinity when fp32 does not hold the score
 };
 
 __device__ __forceinline__ uint32_t float_key(float x) {     // same order; equal numbers, equal keys
@@ -319,6 +319,12 @@ __device__ __forceinline__ uint32_t as_query_type(uint32_t pair) {
     return (p & (back.x == f.x ? 0xffffu : 0u)) | (back.x == f.x ? 0u : 0x7fffu) | (p & (back.y == f.y ? 0xffff0000u : 0u)) |
            (back.y == f.y ? 0u : 0x7fff0000u);
   }
+}
+
+// not 0 where one of a pair is infinite or NaN: the exponent's ones carry into the sign's place
+template <typename B>
+__device__ __forceinline__ uint32_t not_finite2(uint32_t pair) {
+  return ((pair & 0x7fff7fffu) + (std::is_same<B, __half>::value ? 0x04000400u : 0x00800080u)) & 0x80008000u;
 }
 
 // fp32 scores: products [16 pages x 16 channels] . [16 channels x 8 queries] of the upper bounds with the queries' positive
@@ -479,7 +485,25 @@ __global__ void __launch_bounds__(SCORE_WARPS * 32, J <= 4 ? SCORE_BLOCKS : 2) s
         magnitude[x] = fmaxf(magnitude[x], __shfl_xor_sync(0xffffffffu, magnitude[x], o));
       }
       const int lp = now.page0 + x * 8 + r;
-      const bool known = __shfl_sync(0xffffffffu, now.my_page, x * 8 + r) >= 0;
+      const int page = __shfl_sync(0xffffffffu, now.my_page, x * 8 + r);
+      const bool known = page >= 0;
+      // A sum that is not finite: because a bound is not, then the score is +infinity and needs no second look (looked at as
+      // one that 64 bits have to decide, it would take all other pages with it), or because fp32 does not hold it.
+      if (__any_sync(0xffffffffu, magnitude[x] > FLT_MAX)) {
+        const B* bound = reinterpret_cast<const B*>(a.kv.bounds) + ((int64_t)max(page, 0) * heads + head) * 2 * d;
+        uint32_t odd = 0;
+#pragma unroll 1
+        for (int ch = c * 8; ch < 2 * d; ch += 32) {
+          const uint4 v = load_once(bound + ch);
+          odd |= not_finite2<B>(v.x) | not_finite2<B>(v.y) | not_finite2<B>(v.z) | not_finite2<B>(v.w);
+        }
+        odd |= __shfl_xor_sync(0xffffffffu, odd, 1);
+        odd |= __shfl_xor_sync(0xffffffffu, odd, 2);
+        if (odd) {
+          best[x] = INFINITY;
+          magnitude[x] = 0.0f;
+        }
+      }
       // a page outside the pool comes last (-infinity): the attention would leave it out
       if (c == 0 && lp < now.n)
         *reinterpret_cast<float2*>(scores + (now.seq * heads + head) * a.table.width + lp) =
@@ -799,7 +823,7 @@ __global__ void __launch_bounds__(1024) select_kernel(const wush_kv_select_args 
   // smallest normal one may lose
   const float eps = magnitude * (float)(17 + 2 * ((a.kv.dim + 31) / 32)) * (1.0625f / 8388608.0f) + 1024.0f * FLT_MIN;
   // a magnitude that is not finite leaves everything between; where the k-th is a page outside the pool, all that are in it
-  // are above
+  // are above, and where it is one with a bound that is not finite, those are between
   const float center = key_float(kth);
   float bottom = -INFINITY, roof = INFINITY;
   if (eps <= FLT_MAX) {
@@ -880,7 +904,8 @@ __global__ void __launch_bounds__(1024) select_kernel(const wush_kv_select_args 
     }, [](int, int) { return false; }, out);
     return;
   }
-  // many between (equal pages, or magnitudes that are not finite): 64-bit keys in place of the scores, and another selection
+  // many between (equal pages, or queries that are not finite): 64-bit keys in place of the scores, and another selection (not
+  // fast: 2047 pages whose bounds are all 0, with 8 queries, 0.7 ms)
   unsigned long long* keys = reinterpret_cast<unsigned long long*>(mine);
   for (int i = warp; i < n; i += warps) {
     if (i < begin || i >= end) continue;
