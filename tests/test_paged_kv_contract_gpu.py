@@ -334,3 +334,12 @@ def test_pages_with_a_bound_that_is_not_finite_do_not_hide_the_others(typ, bound
                 score[strange] = math.inf
             assert pages[0, h].tolist() == ref.select(score.tolist(), top, sink, recent), (top, h)
     _status_clear()
+
+
+@pytest.mark.parametrize("cache", [BF, F8])
+def test_results_carry_no_gradient(cache):
+    from wush_b200 import paged_kv
+    s = Setup([40], page=16, kv=2, dim=64, cache=cache, bounds=True)
+    q = _randn(s.g, 1, 4, 64).to(BF).requires_grad_()
+    out, lse = paged_kv.paged_decode_attention(q, s.cache, s.table, s.seq_lens, return_lse=True)
+    assert not out.requires_grad and not lse.requires_grad

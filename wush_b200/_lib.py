@@ -141,7 +141,7 @@ def status_word(device):
 
 def check_status(device, what: str = "kernel") -> None:
     """Synchronize the current stream of `device` and raise WushB200Error if any kernel launched so far reported
-    a device-side timeout (its output is invalid).  Called at the points where the host waits anyway
+    a device-side timeout (its output is invalid) or an index outside its table (what it names was skipped).  Called at the points where the host waits anyway
     (HostQuantizer.synchronize, DistributedHessian.num_samples, the column sweep) and after every op when the
     environment variable WUSH_B200_CHECK_STATUS=1 is set."""
     import torch

@@ -10,12 +10,13 @@
 // memory, and the queries are loaded in the matching order.  P is turned from the layout of an accumulator into that of an
 // operand by movmatrix, as two 16-bit terms: one alone is off by up to 2^-9 (bf16) or 2^-12 (fp16) of a weight, and where
 // values cancel no rounding of the result hides that.  8-bit pages are widened to fp16 (exact).  (tcgen05.mma has at least 64
-// rows and 8 columns, wants P in memory, and would be idle all the same: the tensor pipe is busy a seventh of the time.)
+// rows and 8 columns, wants P in memory, and would be idle all the same: the tensor pipe is busy 14 % of the time, 27 % over
+// 8-bit pages.)
 //
 // Copies.  Every warp has a ring of three tiles in shared memory, filled two tiles ahead by bulk tensor copies (16 rows of one
 // head of a page are one box), so a warp needs one instruction for 2 KB and no registers for what is in flight.  Measured on
 // 64 ragged sequences of up to 4096 tokens (364 MB), each with the work dealt as it was then: fragments straight into registers
-// 110 us, per-lane 16-byte copies 90 us, boxes 70 us (now 67: 84 % of the copy bandwidth; 6.65 TB/s on one of 500 000 tokens).
+// 110 us, per-lane 16-byte copies 90 us, boxes 70 us (now 67: 84 % of the copy bandwidth; one of 500 000 tokens comes at 6.5 TB/s).
 //
 // Work.  The tokens of all (sequence, key head, chunk of queries) items are cut into units of 4 tiles (one per warp), the
 // units of all items are numbered through, and every block of a grid that fills the GPU exactly once takes an equal run

@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(128) bounds_kernel(const wush_kv_pages kv, con
 
 // ---- selection -----------------------------------------------------------------------------------------------------
 // The score of a page for a key head is max over its queries of sum_d max(q_d lower_d, q_d upper_d), and the choice has to be
-// the one that exact scores give.  64-bit sums of all of them cost 35 us where their bounds can be read in 6 (64-bit products,
+// the one that exact scores give.  64-bit sums of all of them cost 35 us where their bounds can be read in 11 (64-bit products,
 // on either pipe, were the limit), so the work is divided:
 //   1. score_kernel computes every score on the tensor cores in fp32, with the sum of the terms' magnitudes;
 //   2. select_kernel finds the k-th largest of them, and from the magnitudes an eps by which no score is off.  What is more

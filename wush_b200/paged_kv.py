@@ -15,7 +15,7 @@ another library's models, whose cache and attention they use.  ``wush_b200.block
 operators (``prefill`` and ``decode``); they can equally be called by themselves.
 
 Every operator runs on the current stream of its tensors' device, without a host synchronization, and can be captured
-into a CUDA graph.  Lengths, positions, tables and selected pages are int32 tensors on the device.  An entry that lies
+into a CUDA graph.  Inference only: results carry no gradient.  Lengths, positions, tables and selected pages are int32 tensors on the device.  An entry that lies
 outside what it indexes (a page outside the pool, a length beyond the table, ...) is skipped by the kernels and
 reported by ``_lib.check_status(device)``.
 """
@@ -350,7 +350,8 @@ def paged_select_pages(q: torch.Tensor, cache: PagedKVCache, block_table: torch.
     are summed in 64 bits: exactly, whatever the order, where the terms of a page and their partial sums fit 53 bits, and to
     64-bit rounding (dim * 2^-53 of the terms' magnitude) otherwise.  A page one of whose bounds is not finite, and a score
     that is not finite, count as +infinity.  Pages come in ascending order, followed by -1; a sequence of at most ``top``
-    pages gets all of them.  q: [sequences, heads, head_dim], as ``paged_decode_attention`` takes it; ``cache.bounds`` must be
+    pages gets all of them.  (Right but slow where more than 256 pages share the score at the border, as with bounds that
+    nobody filled, or a query is not finite: 0.7 ms for 2047 pages.)  q: [sequences, heads, head_dim], as ``paged_decode_attention`` takes it; ``cache.bounds`` must be
     up to date (``paged_kv_bounds``)."""
     if cache.bounds is None:
         raise ValueError("the cache has no bounds")
@@ -385,7 +386,9 @@ def paged_decode_attention(q: torch.Tensor, cache: PagedKVCache, block_table: to
     ``return_lse``, float32 [sequences, heads]: the log of the sum of exponentials).
 
     q          [sequences, heads, head_dim]; query head h reads key head h // (heads / n_kv_heads)
-    seq_lens   int32 [sequences]: tokens in the cache, the new one included.  No token (<= 0): zeros, and -inf.
+    seq_lens   int32 [sequences]: tokens in the cache, the new one included.  No token (<= 0): zeros, and -inf.  A key or
+               value that is not finite in a token that counts makes what it meets NaN or infinite (a logit of -inf weighs
+               nothing); in one that does not count it has no effect.
     scale      softmax scale, 1 / sqrt(head_dim) by default
     window     only the last ``window`` tokens; 0: all
     pages, counts  attend to the tokens of these pages only: for every sequence and key head the first counts[b, h]
