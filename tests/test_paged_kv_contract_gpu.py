@@ -92,6 +92,20 @@ def test_copies_of_a_cache(how, cache):
     assert torch.equal(paged_kv.paged_decode_attention(q, s.cache, s.table, s.seq_lens), out)
 
 
+def test_copies_of_a_cache_keep_their_shape_and_what_hangs_on_them():
+    from wush_b200 import paged_kv
+    dev = _dev()
+    pool = torch.zeros(4, 2, 16, 2, 64, dtype=BF, device=dev)
+    cache = paged_kv.PagedKVCache(pool[:, 0], pool[:, 1])     # keys and values interleaved
+    cache.layer = 7
+    twin = copy.deepcopy(cache)
+    again = pickle.loads(pickle.dumps(cache))
+    assert twin.v.data_ptr() - twin.k.data_ptr() == cache.v.data_ptr() - cache.k.data_ptr()      # still interleaved
+    for c in (twin, again):
+        assert c.layer == 7 and c.k.stride() == cache.k.stride() and c.v.stride() == cache.v.stride()
+        assert c.k.data_ptr() != cache.k.data_ptr() and c._packed[:8] == c.k.data_ptr().to_bytes(8, "little")
+
+
 @pytest.mark.parametrize("captured", [False, True])
 def test_decode_step_follows_lengths_written_by_the_caller(captured):
     """A serving loop puts another sequence into a row by writing seq_lens in place; the token goes where the new length

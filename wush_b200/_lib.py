@@ -141,9 +141,9 @@ def status_word(device):
 
 def check_status(device, what: str = "kernel") -> None:
     """Synchronize the current stream of `device` and raise WushB200Error if any kernel launched so far reported
-    a device-side timeout (its output is invalid) or an index outside its table (what it names was skipped).  Called at the points where the host waits anyway
-    (HostQuantizer.synchronize, DistributedHessian.num_samples, the column sweep) and after every op when the
-    environment variable WUSH_B200_CHECK_STATUS=1 is set."""
+    a device-side timeout (its output is invalid) or an index outside its table (what it names was skipped).  Called at the
+    points where the host waits anyway (HostQuantizer.synchronize, DistributedHessian.num_samples, the column sweep) and after
+    every op when the environment variable WUSH_B200_CHECK_STATUS=1 is set."""
     import torch
     w = status_word(device)
     with torch.cuda.device(w.device):

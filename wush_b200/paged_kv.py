@@ -15,9 +15,9 @@ another library's models, whose cache and attention they use.  ``wush_b200.block
 operators (``prefill`` and ``decode``); they can equally be called by themselves.
 
 Every operator runs on the current stream of its tensors' device, without a host synchronization, and can be captured
-into a CUDA graph.  Inference only: results carry no gradient.  Lengths, positions, tables and selected pages are int32 tensors on the device.  An entry that lies
-outside what it indexes (a page outside the pool, a length beyond the table, ...) is skipped by the kernels and
-reported by ``_lib.check_status(device)``.
+into a CUDA graph.  Inference only: results carry no gradient.  Lengths, positions, tables and selected pages are int32
+tensors on the device.  An entry that lies outside what it indexes (a page outside the pool, a length beyond the table,
+...) is skipped by the kernels and reported by ``_lib.check_status(device)``.
 """
 from __future__ import annotations
 
@@ -85,11 +85,13 @@ class PagedKVCache:
     def __getstate__(self):
         eight = self.dtype == torch.float8_e4m3fn             # (pickle does not know 8-bit floats)
         k, v = (t.view(torch.uint8) if eight else t for t in (self.k, self.v))
-        return {"k": k, "v": v, "k_scale": self.k_scale, "v_scale": self.v_scale, "bounds": self.bounds}
+        return {**self.__dict__, "k": k, "v": v}
 
     def __setstate__(self, state):                            # the packed addresses become those of the copy's tensors
         k, v = (t.view(torch.float8_e4m3fn) if t.dtype == torch.uint8 else t for t in (state["k"], state["v"]))
         self.__init__(k, v, state["k_scale"], state["v_scale"], state["bounds"])
+        for name, value in state.items():                     # (what a caller has hung on the object)
+            self.__dict__.setdefault(name, value)
 
     @classmethod
     def allocate(cls, num_pages: int, page_size: int, n_kv_heads: int, head_dim: int, dtype=torch.bfloat16, device=None,
@@ -351,8 +353,8 @@ def paged_select_pages(q: torch.Tensor, cache: PagedKVCache, block_table: torch.
     64-bit rounding (dim * 2^-53 of the terms' magnitude) otherwise.  A page one of whose bounds is not finite, and a score
     that is not finite, count as +infinity.  Pages come in ascending order, followed by -1; a sequence of at most ``top``
     pages gets all of them.  (Right but slow where more than 256 pages share the score at the border, as with bounds that
-    nobody filled, or a query is not finite: 0.7 ms for 2047 pages.)  q: [sequences, heads, head_dim], as ``paged_decode_attention`` takes it; ``cache.bounds`` must be
-    up to date (``paged_kv_bounds``)."""
+    nobody filled, or a query is not finite: 0.7 ms for 2047 pages.)  q: [sequences, heads, head_dim], as
+    ``paged_decode_attention`` takes it; ``cache.bounds`` must be up to date (``paged_kv_bounds``)."""
     if cache.bounds is None:
         raise ValueError("the cache has no bounds")
     if top < 1 or sink < 0 or recent < 0 or sink + recent > top:
